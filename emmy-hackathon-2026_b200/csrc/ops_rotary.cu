@@ -1,0 +1,162 @@
+/*
+ * Rotary positions:  (a, b) -> magnitude * (a cos t - b sin t, a sin t + b cos t) for each pair
+ * of a head, t = position * frequency.
+ *
+ * The angle is kept in turns as a 64-bit fraction: position * turns wraps exactly where the
+ * angle does, so a far position keeps the precision of a near one (a 32-bit product of a
+ * position of 2^20 would be off by 0.03 radians).  Its upper 32 bits go to sincospif.
+ *
+ * The bytes bound it: every element is read and written once.  A block takes a few tokens,
+ * computes their cosines and sines once into shared memory, and every head of both tensors
+ * uses them.
+ */
+#include "ops_common.cuh"
+
+namespace {
+
+struct RotaryParams {
+    const char *x[2];
+    char *out[2];
+    int64_t x_token[2], x_head[2], out_token[2], out_head[2];
+    int heads[2];
+    const void *positions;
+    const uint64_t *turns;
+    int64_t tokens;
+    int positions_64, pairs, rest, per_block, transpose, copies;
+    float magnitude;
+};
+
+/* V pairs a step (half: V elements of either half; interleaved: 2 V consecutive elements) */
+template <typename T, int V, bool HALF>
+__global__ void __launch_bounds__(256) rotary(RotaryParams p) {
+    extern __shared__ float2 table[];             /* [per_block][pairs] (cos, sin) */
+    enter_grid();
+    const int64_t first = (int64_t)blockIdx.x * p.per_block;
+    const int live = (int)min((int64_t)p.per_block, p.tokens - first);
+    for (int i = threadIdx.x; i < live * p.pairs; i += blockDim.x) {
+        const int token = i / p.pairs, pair = i - token * p.pairs;
+        const int64_t position = p.positions_64 ? ((const int64_t *)p.positions)[first + token]
+                                                : ((const int32_t *)p.positions)[first + token];
+        const uint64_t turn = (uint64_t)position * p.turns[pair];
+        float s, c;
+        sincospif((float)(int32_t)(turn >> 32) * 0x1p-31f, &s, &c);
+        table[i] = make_float2(c * p.magnitude, (p.transpose ? -s : s) * p.magnitude);
+    }
+    __syncthreads();
+    const int units = p.pairs / V, rest = p.copies ? p.rest / V : 0;
+    const int per_head = units + rest, heads = p.heads[0] + p.heads[1], per_token = heads * per_head;
+    for (int i = threadIdx.x; i < live * per_token; i += blockDim.x) {
+        const int token = i / per_token, r = i - token * per_token, head = r / per_head, unit = r - head * per_head;
+        const int which = head >= p.heads[0], h = which ? head - p.heads[0] : head;
+        const T *x = (const T *)p.x[which] + (first + token) * p.x_token[which] + h * p.x_head[which];
+        T *out = (T *)p.out[which] + (first + token) * p.out_token[which] + h * p.out_head[which];
+        if (unit >= units) {
+            const int e = 2 * p.pairs + (unit - units) * V;
+            *(Pack<T, V> *)(out + e) = *(const Pack<T, V> *)(x + e);
+            continue;
+        }
+        const float2 *cs = table + token * p.pairs + unit * V;
+        if (HALF) {
+            const int e = unit * V;
+            const Pack<T, V> a = *(const Pack<T, V> *)(x + e), b = *(const Pack<T, V> *)(x + p.pairs + e);
+            Pack<T, V> ra, rb;
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float2 q = cs[j];
+                const float u = to_f32(a.at[j]), v = to_f32(b.at[j]);
+                ra.at[j] = from_f32<T>(u * q.x - v * q.y);
+                rb.at[j] = from_f32<T>(u * q.y + v * q.x);
+            }
+            *(Pack<T, V> *)(out + e) = ra;
+            *(Pack<T, V> *)(out + p.pairs + e) = rb;
+        } else {
+            /* two accesses of V elements hold V pairs */
+            const int e = 2 * unit * V;
+            Pack<T, V> a[2] = {*(const Pack<T, V> *)(x + e), *(const Pack<T, V> *)(x + e + V)}, r[2];
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const float2 q = cs[j];
+                const float u = to_f32(a[2 * j / V].at[2 * j % V]), v = to_f32(a[(2 * j + 1) / V].at[(2 * j + 1) % V]);
+                r[2 * j / V].at[2 * j % V] = from_f32<T>(u * q.x - v * q.y);
+                r[(2 * j + 1) / V].at[(2 * j + 1) % V] = from_f32<T>(u * q.y + v * q.x);
+            }
+            *(Pack<T, V> *)(out + e) = r[0];
+            *(Pack<T, V> *)(out + e + V) = r[1];
+        }
+    }
+}
+
+template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, uint64_t stream) {
+    /* tokens a block: enough for two steps of its 256 threads where there are many, one where
+     * there are few, as long as the table fits 32 KB */
+    const int per_token = (p.heads[0] + p.heads[1]) * (p.pairs / V + (p.copies ? p.rest / V : 0));
+    int64_t per = 512 / (per_token > 0 ? per_token : 1);
+    const int64_t spread = p.tokens / (148 * 4);
+    if (per > spread) per = spread;
+    const int64_t most = 32768 / ((int64_t)p.pairs * 8);
+    if (per > most) per = most;
+    p.per_block = per < 1 ? 1 : (int)per;
+    const dim3 grid((unsigned)((p.tokens + p.per_block - 1) / p.per_block));
+    const size_t smem = (size_t)p.per_block * p.pairs * 8;
+    return layout == EMMY_OPS_ROTARY_HALF ? launch(rotary<T, V, true>, grid, dim3(256), smem, stream, p)
+                                          : launch(rotary<T, V, false>, grid, dim3(256), smem, stream, p);
+}
+
+}  // namespace
+
+EMMY_EXPORT int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint64_t stream) {
+    if (!a) return ops_fail(EMMY_RT_EINVAL, "no arguments");
+    if (!known_dtype(a->dtype)) return ops_fail(EMMY_RT_EINVAL, "element type %d", a->dtype);
+    if (a->rotary < 2 || a->rotary % 2 || a->rotary > a->dim || a->dim > 8192)
+        return ops_fail(EMMY_RT_EINVAL, "rotary %d of dim %d", a->rotary, a->dim);
+    if (a->layout != EMMY_OPS_ROTARY_HALF && a->layout != EMMY_OPS_ROTARY_INTERLEAVED)
+        return ops_fail(EMMY_RT_EINVAL, "layout %d", a->layout);
+    if (a->tokens < 0 || a->tokens > 0x7fffffffLL) return ops_fail(EMMY_RT_EINVAL, "tokens %lld", (long long)a->tokens);
+    if (a->heads[0] < 0 || a->heads[1] < 0 || (int64_t)(a->heads[0] + (int64_t)a->heads[1]) * a->dim > (1 << 24))
+        return ops_fail(EMMY_RT_EINVAL, "heads %d and %d", a->heads[0], a->heads[1]);
+    if (a->tokens == 0 || (a->heads[0] == 0 && a->heads[1] == 0)) return 0;
+    if (!a->positions || !a->turns || !aligned(a->positions, a->positions_64 ? 8 : 4) || !aligned(a->turns, 8))
+        return ops_fail(EMMY_RT_EINVAL, "positions and turns are needed, aligned to their elements");
+    const int es = elem_size(a->dtype);
+    RotaryParams p = {};
+    int bytes = 16;
+    for (int i = 0; i < 2; ++i) {
+        p.heads[i] = a->heads[i];
+        if (!a->heads[i]) continue;
+        if (!a->x[i] || !a->out[i] || !aligned(a->x[i], es) || !aligned(a->out[i], es))
+            return ops_fail(EMMY_RT_EINVAL, "x and out are needed, aligned to their elements");
+        const int64_t strides[] = {a->x_token[i], a->x_head[i], a->out_token[i], a->out_head[i]};
+        while (bytes > es) {
+            bool ok = aligned(a->x[i], bytes) && aligned(a->out[i], bytes);
+            for (int64_t s : strides) ok = ok && s * es % bytes == 0;
+            if (ok) break;
+            bytes = bytes == 16 && es == 2 ? 4 : es;
+        }
+        p.x[i] = (const char *)(uintptr_t)a->x[i];
+        p.out[i] = (char *)(uintptr_t)a->out[i];
+        p.x_token[i] = a->x_token[i], p.x_head[i] = a->x_head[i];
+        p.out_token[i] = a->out_token[i], p.out_head[i] = a->out_head[i];
+        p.copies |= a->x[i] != a->out[i] || a->x_token[i] != a->out_token[i] || a->x_head[i] != a->out_head[i];
+    }
+    p.pairs = a->rotary / 2;
+    p.rest = a->dim - a->rotary;
+    while (bytes > es && (p.pairs % (bytes / es) || p.rest % (bytes / es))) bytes = bytes == 16 && es == 2 ? 4 : es;
+    p.positions = (const void *)(uintptr_t)a->positions;
+    p.turns = (const uint64_t *)(uintptr_t)a->turns;
+    p.tokens = a->tokens, p.positions_64 = a->positions_64 != 0, p.transpose = a->transpose != 0;
+    p.magnitude = a->magnitude;
+    DeviceScope scope(device);
+    if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
+    cudaError_t e;
+    if (a->dtype == EMMY_OPS_F32)
+        e = bytes == 16 ? go<float, 4>(p, a->layout, stream) : go<float, 1>(p, a->layout, stream);
+    else if (a->dtype == EMMY_OPS_F16)
+        e = bytes == 16  ? go<__half, 8>(p, a->layout, stream)
+            : bytes == 4 ? go<__half, 2>(p, a->layout, stream)
+                         : go<__half, 1>(p, a->layout, stream);
+    else
+        e = bytes == 16  ? go<__nv_bfloat16, 8>(p, a->layout, stream)
+            : bytes == 4 ? go<__nv_bfloat16, 2>(p, a->layout, stream)
+                         : go<__nv_bfloat16, 1>(p, a->layout, stream);
+    return ops_cuda(e, "rotary");
+}

@@ -90,8 +90,9 @@ for _name, (_args, _res) in SIGNATURES.items():
 
 
 class EmmyRTError(RuntimeError):
-    def __init__(self, status: int, what: str):
-        msg = lib.emmy_rt_last_error().decode(errors="replace")
+    def __init__(self, status: int, what: str, msg: str | None = None):
+        if msg is None:
+            msg = lib.emmy_rt_last_error().decode(errors="replace")
         super().__init__(f"{what}: status {status}: {msg}")
         self.status = status
 
@@ -118,6 +119,15 @@ def init(device: int = 0) -> None:
         return
     check(lib.emmy_rt_init(device), "emmy_rt_init")
     _initialised[device] = True
+
+
+def current_device() -> int:
+    """The ordinal of the calling thread's current device."""
+    v = ctypes.c_int()
+    status = ops_lib().emmy_ops_current_device(ctypes.byref(v))
+    if status:
+        raise EmmyRTError(status, "current device", ops_lib().emmy_ops_last_error().decode(errors="replace"))
+    return v.value
 
 
 def device_attribute(attr: int, device: int = 0) -> int:
@@ -445,3 +455,68 @@ def static_scratch_lib():
             fn.restype = res
         _static_lib = lib2
     return _static_lib
+
+
+# ---------------------------------------------------------------------------
+# operators of a served decoder layer (libemmyrt_ops.so, C ABI in include/emmyrt_ops.h)
+
+OPS_LIB_PATH = _HERE / "libemmyrt_ops.so"
+
+
+class Cache4Memory(ctypes.Structure):
+    """emmy_ops_cache4"""
+    _fields_ = [("k", _u64), ("v", _u64), ("k_meta", _u64), ("v_meta", _u64), ("pages", ctypes.c_int64),
+                ("heads", ctypes.c_int32), ("page", ctypes.c_int32), ("dim", ctypes.c_int32)]
+
+
+class NormArgs(ctypes.Structure):
+    """emmy_ops_norm_args"""
+    _fields_ = [(n, _u64) for n in ("x", "block", "y", "h")] + \
+        [(n, ctypes.c_int64) for n in ("x_stride", "block_stride", "y_stride", "h_stride")] + \
+        [(n, _u64) for n in ("post_weight", "post_bias", "gate", "pre_weight", "pre_bias")] + \
+        [(n, ctypes.c_int64) for n in ("gate_stride", "rows_per_gate", "rows", "dim")] + \
+        [(n, ctypes.c_int32) for n in ("dtype", "post_weight_dtype", "post_bias_dtype", "gate_dtype", "pre_weight_dtype",
+                                       "pre_bias_dtype", "kind", "post_norm")] + \
+        [("eps", ctypes.c_float), ("scale", ctypes.c_float)]
+
+
+class RotaryArgs(ctypes.Structure):
+    """emmy_ops_rotary_args"""
+    _fields_ = [("x", _u64 * 2), ("out", _u64 * 2), ("x_token", ctypes.c_int64 * 2), ("x_head", ctypes.c_int64 * 2),
+                ("out_token", ctypes.c_int64 * 2), ("out_head", ctypes.c_int64 * 2), ("heads", ctypes.c_int32 * 2),
+                ("positions", _u64), ("turns", _u64), ("tokens", ctypes.c_int64)] + \
+        [(n, ctypes.c_int32) for n in ("positions_64", "dtype", "dim", "rotary", "layout", "transpose")] + \
+        [("magnitude", ctypes.c_float)]
+
+
+class Cache4AppendArgs(ctypes.Structure):
+    """emmy_ops_cache4_append_args"""
+    _fields_ = [("cache", Cache4Memory)] + [(n, _u64) for n in ("k", "v", "slots", "k_stored", "v_stored")] + \
+        [(n, ctypes.c_int64) for n in ("k_token", "k_head", "v_token", "v_head", "tokens")] + \
+        [("slots_64", ctypes.c_int32), ("dtype", ctypes.c_int32)]
+
+
+# every symbol declared in include/emmyrt_ops.h, with its ctypes signature
+OPS_SIGNATURES = {
+    "emmy_ops_last_error": ([], ctypes.c_char_p),
+    "emmy_ops_current_device": ([_P(_int)], _int),
+    "emmy_ops_residual_norm": ([_P(NormArgs), _int, _u64], _int),
+    "emmy_ops_rotary": ([_P(RotaryArgs), _int, _u64], _int),
+    "emmy_ops_cache4_append": ([_P(Cache4AppendArgs), _int, _u64], _int),
+}
+_ops_lib = None
+
+
+def ops_lib():
+    """The library with the decoder-layer operators."""
+    global _ops_lib
+    if _ops_lib is None:
+        if not OPS_LIB_PATH.exists():
+            raise ImportError(f"{OPS_LIB_PATH} is not built; run __graft_entry__.build()")
+        lib2 = ctypes.CDLL(str(OPS_LIB_PATH))
+        for name, (args, res) in OPS_SIGNATURES.items():
+            fn = getattr(lib2, name)
+            fn.argtypes = args
+            fn.restype = res
+        _ops_lib = lib2
+    return _ops_lib
