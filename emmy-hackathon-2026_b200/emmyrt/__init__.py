@@ -463,10 +463,9 @@ def static_scratch_lib():
 OPS_LIB_PATH = _HERE / "libemmyrt_ops.so"
 
 
-class Cache4Memory(ctypes.Structure):
-    """emmy_ops_cache4"""
-    _fields_ = [("k", _u64), ("v", _u64), ("k_meta", _u64), ("v_meta", _u64), ("pages", ctypes.c_int64),
-                ("heads", ctypes.c_int32), ("page", ctypes.c_int32), ("dim", ctypes.c_int32)]
+# the fields of emmy_ops_cache4, at the head of the blocks that hold one
+_CACHE4 = [(n, _u64) for n in ("cache_k", "cache_v", "cache_k_meta", "cache_v_meta")] + \
+    [("cache_pages", ctypes.c_int64)] + [(n, ctypes.c_int32) for n in ("cache_heads", "cache_page", "cache_dim", "_pad")]
 
 
 class NormArgs(ctypes.Structure):
@@ -482,16 +481,17 @@ class NormArgs(ctypes.Structure):
 
 class RotaryArgs(ctypes.Structure):
     """emmy_ops_rotary_args"""
-    _fields_ = [("x", _u64 * 2), ("out", _u64 * 2), ("x_token", ctypes.c_int64 * 2), ("x_head", ctypes.c_int64 * 2),
-                ("out_token", ctypes.c_int64 * 2), ("out_head", ctypes.c_int64 * 2), ("heads", ctypes.c_int32 * 2),
-                ("positions", _u64), ("turns", _u64), ("tokens", ctypes.c_int64)] + \
+    _fields_ = [(n, _u64) for n in ("x0", "x1", "out0", "out1")] + \
+        [(f"{n}{i}", ctypes.c_int64) for n in ("x_token", "x_head", "out_token", "out_head") for i in (0, 1)] + \
+        [("heads0", ctypes.c_int32), ("heads1", ctypes.c_int32), ("positions", _u64), ("turns", _u64),
+         ("tokens", ctypes.c_int64)] + \
         [(n, ctypes.c_int32) for n in ("positions_64", "dtype", "dim", "rotary", "layout", "transpose")] + \
         [("magnitude", ctypes.c_float)]
 
 
 class Cache4AppendArgs(ctypes.Structure):
     """emmy_ops_cache4_append_args"""
-    _fields_ = [("cache", Cache4Memory)] + [(n, _u64) for n in ("k", "v", "slots", "k_stored", "v_stored")] + \
+    _fields_ = _CACHE4 + [(n, _u64) for n in ("k", "v", "slots", "k_stored", "v_stored")] + \
         [(n, ctypes.c_int64) for n in ("k_token", "k_head", "v_token", "v_head", "tokens")] + \
         [("slots_64", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 

@@ -6,13 +6,13 @@ stands for ``level * step + least``.  At head dim 128 that is 68 bytes instead o
 
 from __future__ import annotations
 
-from . import Cache4AppendArgs, Cache4Memory, DeviceBuffer
-from .operands import (CODE, FLOATS, INDICES, Array, apart, call, contiguous, operand, own_device, shaped)
+from . import Cache4AppendArgs, DeviceBuffer
+from .operands import CODE, FLOATS, INDICES, Array, Operator, Plan, apart, contiguous, operand, overlaps, shaped
 
 DIMS = (64, 128)
 
 
-class Cache4:
+class Cache4(Operator):
     """Pages of ``page`` token rows each, shared by all sequences; a slot is ``page index * page + row``.
 
     ``k`` and ``v`` are u8 [pages, heads, page, dim / 2] (element 2 i in the low half of byte i), ``k_meta`` and
@@ -20,7 +20,8 @@ class Cache4:
     """
 
     def __init__(self, k, k_meta, v, v_meta):
-        self.device = d = own_device()
+        super().__init__()
+        d = self.device
         self.k = contiguous(operand(k, "k", ("u8",), 4, d), "k")
         self.pages, self.heads, self.page, half = self.k.shape
         self.dim = 2 * half
@@ -45,34 +46,31 @@ class Cache4:
             made.append(Array(buffer, dtype, (pages, heads, page, last)))
         return cls(*made)
 
-    def memory(self) -> Cache4Memory:
-        return Cache4Memory(k=self.k.ptr, v=self.v.ptr, k_meta=self.k_meta.ptr, v_meta=self.v_meta.ptr, pages=self.pages,
-                            heads=self.heads, page=self.page, dim=self.dim)
-
     def append(self, k, v, slots, *, k_stored=None, v_stored=None, stream: int = 0) -> None:
         """Quantises ``k`` and ``v`` [tokens, heads, dim] into ``slots`` [tokens] (int32 or int64).  A token whose slot is
         negative or past the cache is left out (padding); two tokens of one call must not have the same slot.
         ``k_stored`` / ``v_stored`` receive the values that the cache then stands for, in the operands' type."""
+        self._call((k, v, slots, k_stored, v_stored, *self.arrays), None, stream)
+
+    _FIELDS = ("k", "v", "slots", "k_stored", "v_stored", "cache_k", "cache_v", "cache_k_meta", "cache_v_meta")
+
+    def _plan(self, operands, options) -> Plan:
+        k, v, slots, k_stored, v_stored = operands[:5]
         d = self.device
         k = operand(k, "k", FLOATS, 3, d)
         n = k.shape[0]
         shaped(k, "k", (n, self.heads, self.dim))
         v = shaped(operand(v, "v", (k.dtype,), 3, d), "v", k.shape)
         slots = shaped(operand(slots, "slots", INDICES, 1, d), "slots", (n,))
-        a = Cache4AppendArgs(cache=self.memory(), k=k.ptr, v=v.ptr, slots=slots.ptr, k_token=k.strides[0],
-                             k_head=k.strides[1], v_token=v.strides[0], v_head=v.strides[1], tokens=n,
-                             slots_64=slots.dtype == "i64", dtype=CODE[k.dtype])
-        outs = []
-        for name, out in (("k_stored", k_stored), ("v_stored", v_stored)):
+        a = Cache4AppendArgs(cache_pages=self.pages, cache_heads=self.heads, cache_page=self.page, cache_dim=self.dim,
+                             k_token=k.strides[0], k_head=k.strides[1], v_token=v.strides[0],
+                             v_head=v.strides[1], tokens=n, slots_64=slots.dtype == "i64", dtype=CODE[k.dtype])
+        ins, outs = [(0, k, "k"), (1, v, "v"), (2, slots, "slots")], []
+        for place, name, out in ((3, "k_stored", k_stored), (4, "v_stored", v_stored)):
             if out is not None:
-                out = contiguous(shaped(operand(out, name, (k.dtype,), 3, d), name, k.shape), name)
-                if out.ptr % 16:
-                    raise ValueError(f"{name} does not start on 16 bytes")
-                setattr(a, name, out.ptr)
-                for other in (*outs, k, v, slots, *self.arrays):
-                    apart(out, other, name, same=False)
-                outs.append(out)
-        for part in self.arrays:
-            for other in (k, v, slots):
-                apart(part, other, "an operand", same=False)
-        call("emmy_ops_cache4_append", a, d, stream)
+                outs.append((place, contiguous(shaped(operand(out, name, (k.dtype,), 3, d), name, k.shape), name), name))
+        held = [(5 + i, part, "the cache") for i, part in enumerate(self.arrays)]
+        checks = overlaps(outs, ins)
+        for part in held:
+            checks += overlaps([part], ins + outs)
+        return Plan("emmy_ops_cache4_append", a, self._FIELDS, checks)

@@ -120,21 +120,38 @@ def written(a: Array, name: str) -> Array:
     return a
 
 
+class Apart:
+    """The check that an output does not overlap another operand, prepared for two places of a call."""
+
+    __slots__ = ("i", "j", "span_i", "span_j", "same", "step", "row_i", "row_j", "name")
+
+    def __init__(self, i: int, out: Array, j: int, other: Array, name: str, same: bool):
+        self.i, self.j, self.span_i, self.span_j, self.name = i, j, span(out), span(other), name
+        self.same = same and tuple(out.shape) == tuple(other.shape) and out.dtype == other.dtype and \
+            all(p == q for p, q, n in zip(out.strides, other.strides, out.shape) if n > 1)
+        # rows side by side in wider rows, as the parts of one projection are
+        self.step = 0
+        if self.span_i and self.span_j and out.shape and other.shape:
+            step = out.strides[0] * ITEMSIZE[out.dtype]
+            if step > 0 and step == other.strides[0] * ITEMSIZE[other.dtype]:
+                self.step, self.row_i, self.row_j = step, row_span(out), row_span(other)
+
+    def meets(self, p: int, q: int) -> None:
+        """``p`` and ``q`` are the operands' addresses, whose spans overlap."""
+        if self.same and p == q:
+            return
+        if self.step:
+            gap = (q - p) % self.step
+            if self.row_i <= gap and gap + self.row_j <= self.step:
+                return
+        raise ValueError(f"{self.name} overlaps another operand of the call")
+
+
 def apart(out: Array, other: Array, name: str, *, same: bool) -> None:
     """``out`` must not overlap ``other``; with ``same`` it may be the very same elements."""
-    if out.ptr >= other.ptr + span(other) or other.ptr >= out.ptr + span(out):
-        return
-    # rows side by side in wider rows, as the parts of one projection are
-    if out.shape and other.shape and out.strides and other.strides:
-        step = out.strides[0] * ITEMSIZE[out.dtype]
-        if step > 0 and step == other.strides[0] * ITEMSIZE[other.dtype]:
-            gap = (other.ptr - out.ptr) % step
-            if row_span(out) <= gap and gap + row_span(other) <= step:
-                return
-    if same and out.ptr == other.ptr and tuple(out.shape) == tuple(other.shape) and out.dtype == other.dtype and \
-            all(p == q for p, q, n in zip(out.strides, other.strides, out.shape) if n > 1):
-        return
-    raise ValueError(f"{name} overlaps another operand of the call")
+    check = Apart(0, out, 1, other, name, same)
+    if out.ptr < other.ptr + check.span_j and other.ptr < out.ptr + check.span_i:
+        check.meets(out.ptr, other.ptr)
 
 
 def own_device() -> int:
@@ -142,7 +159,71 @@ def own_device() -> int:
     return current_device()
 
 
-def call(entry: str, args: ctypes.Structure, device: int, stream: int) -> None:
-    status = getattr(ops_lib(), entry)(ctypes.byref(args), device, stream)
-    if status:
-        raise EmmyRTError(status, entry, ops_lib().emmy_ops_last_error().decode(errors="replace"))
+class Plan:
+    """What calls with operands of the same types, shapes and strides have in common: the argument block without its
+    addresses (``fields`` names them, one for each operand) and the overlaps to look for."""
+
+    __slots__ = ("entry", "name", "args", "type", "fields", "checks")
+
+    def __init__(self, name: str, args: ctypes.Structure, fields, checks):
+        self.name, self.entry, self.args, self.type = name, getattr(ops_lib(), name), args, type(args)
+        self.fields = fields
+        self.checks = [(c.i, c.j, c.span_i, c.span_j, c) for c in checks if c.span_i and c.span_j]
+
+
+class Operator:
+    """An operator of one device.  A call's operands are checked in full the first time that their types, shapes and
+    strides come; later calls like it look only at the addresses.  Calls keep no state, so threads may share one."""
+
+    PLANS = 512         # calls of so many kinds are remembered
+
+    def __init__(self):
+        self.device = own_device()
+        self._plans: dict = {}
+
+    def _plan(self, operands, options) -> Plan:
+        raise NotImplementedError
+
+    def _call(self, operands, options, stream: int) -> None:
+        key = [options]
+        try:
+            for x in operands:
+                if x is None:
+                    key.append(None)
+                elif type(x) is Array:
+                    key += (x.dtype, x.shape, x.strides, x.device)
+                else:
+                    key += (x.dtype, x.shape, x.stride(), x.device)
+            key = tuple(key)
+            plan = self._plans.get(key)
+        except (AttributeError, TypeError):
+            plan = key = None       # the full check says what is wrong
+        if plan is None:
+            plan = self._plan(operands, options)
+            if key is not None:
+                if len(self._plans) >= self.PLANS:
+                    self._plans.clear()
+                self._plans[key] = plan
+        at = [0 if x is None else x.ptr if type(x) is Array else x.data_ptr() for x in operands]
+        for i, j, span_i, span_j, check in plan.checks:
+            p, q = at[i], at[j]
+            if p < q + span_j and q < p + span_i:
+                check.meets(p, q)
+        args = plan.type.from_buffer_copy(plan.args)
+        for field, p in zip(plan.fields, at):
+            setattr(args, field, p)
+        status = plan.entry(ctypes.byref(args), self.device, stream)
+        if status:
+            raise EmmyRTError(status, plan.name, ops_lib().emmy_ops_last_error().decode(errors="replace"))
+
+
+def overlaps(outs, others, *, same=()) -> list:
+    """The checks of every output against the others and against each other: ``outs`` and ``others`` are
+    (place, Array or None, name); ``same`` the pairs of places that may be the very same elements."""
+    checks = []
+    outs = [o for o in outs if o[1] is not None]
+    for n, (i, out, name) in enumerate(outs):
+        for j, other, _ in (*outs[:n], *others):
+            if other is not None:
+                checks.append(Apart(i, out, j, other, name, (i, j) in same))
+    return checks

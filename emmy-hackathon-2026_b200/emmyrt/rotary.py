@@ -12,7 +12,7 @@ import math
 import numpy as np
 
 from . import DeviceBuffer, RotaryArgs
-from .operands import CODE, FLOATS, INDICES, apart, call, operand, own_device, shaped, written
+from .operands import CODE, FLOATS, INDICES, Operator, Plan, operand, overlaps, shaped, written
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = ("none", "linear", "base", "parts")
@@ -51,7 +51,7 @@ def frequencies(rotary_dim: int, base: float = 10000.0, scaling: str = "none", f
     return f
 
 
-class Rotary:
+class Rotary(Operator):
     """Rotates the first ``rotary_dim`` elements of each head of ``dim``; the others are copied.
 
     ``layout="half"`` pairs element i with i + rotary_dim / 2, ``"interleaved"`` 2 i with 2 i + 1.  Pairs are
@@ -73,7 +73,7 @@ class Rotary:
         if not math.isfinite(magnitude):
             raise ValueError(f"magnitude {magnitude}")
         self.dim, self.rotary_dim, self.layout, self.magnitude = int(dim), int(rotary_dim), layout, float(magnitude)
-        self.device = own_device()
+        super().__init__()
         # whole turns do nothing: the fraction in 64 bits (53 of them known)
         turns = np.array([int((v / (2 * math.pi)) % 1.0 * 2.0 ** 64) for v in f.tolist()], dtype=np.uint64)
         self._turns = DeviceBuffer(turns.nbytes)
@@ -83,37 +83,33 @@ class Rotary:
         """``q`` (and ``k``, in the same launch) are [tokens, heads, dim], of one type;
         ``positions`` [tokens] int32 or int64.  ``q_out`` / ``k_out`` receive them; without one its operand is rotated in
         place.  ``inverse`` turns the other way: the gradient of the rotation (and its inverse where magnitude is 1)."""
+        self._call((positions, q, k, q if q_out is None else q_out, k if k_out is None else k_out), bool(inverse), stream)
+
+    _FIELDS = ("positions", "x0", "x1", "out0", "out1")
+
+    def _plan(self, operands, inverse) -> Plan:
         d = self.device
-        positions = operand(positions, "positions", INDICES, 1, d)
+        positions = operand(operands[0], "positions", INDICES, 1, d)
         n = positions.shape[0]
-        a = RotaryArgs(positions=positions.ptr, turns=self._turns.ptr, tokens=n, positions_64=positions.dtype == "i64",
-                       dim=self.dim, rotary=self.rotary_dim, layout=LAYOUTS[self.layout], transpose=bool(inverse),
-                       magnitude=self.magnitude)
-        if k is None and k_out is not None:
+        a = RotaryArgs(turns=self._turns.ptr, tokens=n, positions_64=positions.dtype == "i64", dim=self.dim,
+                       rotary=self.rotary_dim, layout=LAYOUTS[self.layout], transpose=inverse, magnitude=self.magnitude)
+        if operands[2] is None and operands[4] is not None:
             raise ValueError("k_out without k")
-        dtype, ins, outs = None, [], []
-        for i, (v, out) in enumerate(((q, q_out), (k, k_out))):
-            if v is None:
+        dtype, ins, outs = None, [(0, positions, "positions")], []
+        for i, name in enumerate(("q", "k")):
+            if i and operands[2] is None:
                 continue
-            name = "k" if i else "q"
-            v = operand(v, name, FLOATS if dtype is None else (dtype,), 3, d)
+            v = operand(operands[1 + i], name, FLOATS if dtype is None else (dtype,), 3, d)
             dtype = v.dtype
             if v.shape[0] != n or v.shape[2] != self.dim:
                 raise ValueError(f"{name} has shape {tuple(v.shape)}, wanted ({n}, heads, {self.dim})")
-            if out is None:
-                o = v
-            else:
-                o = shaped(operand(out, name + "_out", (dtype,), 3, d), name + "_out", v.shape)
+            o = shaped(operand(operands[3 + i], name + "_out", (dtype,), 3, d), name + "_out", v.shape)
             written(o, name + "_out")
-            a.x[i], a.out[i], a.heads[i] = v.ptr, o.ptr, v.shape[1]
-            a.x_token[i], a.x_head[i], a.out_token[i], a.out_head[i] = v.strides[0], v.strides[1], o.strides[0], o.strides[1]
-            ins.append(v)
-            outs.append(o)
-        for i, o in enumerate(outs):
-            apart(o, positions, "an output", same=False)
-            for j, v in enumerate(ins):
-                apart(o, v, "an output", same=i == j)
-            for j in range(i):
-                apart(o, outs[j], "an output", same=False)
+            setattr(a, f"heads{i}", v.shape[1])
+            for field, stride in (("x_token", v.strides[0]), ("x_head", v.strides[1]), ("out_token", o.strides[0]),
+                                  ("out_head", o.strides[1])):
+                setattr(a, f"{field}{i}", stride)
+            ins.append((1 + i, v, name))
+            outs.append((3 + i, o, name + "_out"))
         a.dtype = CODE[dtype]
-        call("emmy_ops_rotary", a, d, stream)
+        return Plan("emmy_ops_rotary", a, self._FIELDS, overlaps(outs, ins, same=((3, 1), (4, 2))))
