@@ -1,0 +1,643 @@
+/*
+ * Attention over the paged 4-bit cache.
+ *
+ * For one key / value head the queries are the rows (token, head of the group); with n the
+ * levels, s and z the steps and least values of a cached token t:
+ *
+ *     score[t, r] = scale * (s_k[t] * sum_d q[r, d] n_k[t, d] + z_k[t] * sum_d q[r, d])
+ *     out[r, d]   = (sum_t (p[t, r] s_v[t]) n_v[t, d] + sum_t p[t, r] z_v[t]) / sum_t p[t, r]
+ *
+ * so the products run on the bare levels, and steps and least values are applied to the
+ * scores and probabilities, once per token instead of once per element.
+ *
+ * The bytes of the cache bound it: a token is (dim / 2 + 4) * 2 bytes per head.  A level in
+ * bits 0..3 of a 16-bit half IS an f16 number, level * 2^-24 (a subnormal one), and one in
+ * bits 4..7 is level * 2^-20; the tensor cores multiply subnormal f16 exactly.  So unpacking is
+ * one AND per two elements and one shift per eight, with no conversion; the powers of two
+ * are put into q's odd elements and into the results.  The queries are scaled by a power of
+ * two per row so that their largest element is just below 2^14, which leaves f16 no less exact
+ * than the 16-bit type they come in.
+ *
+ * Products are transposed: keys and values are the left operand (m16 n8 k16), queries the
+ * right one, so a group of 8 rows fills the narrow side and no half of a tile is idle.
+ * S^T = K Q^T has tokens as rows; movmatrix turns P^T into the right operand of
+ * O^T = V^T P^T.  The order of the dims in Q K^T and of the tokens in V^T P^T is free, and is
+ * chosen so that each thread's share of a token is consecutive bytes.
+ *
+ * Work is a list of tiles of 128 tokens over all (sequence, head, group of rows), cut into
+ * equal runs, one for each block, whatever the lengths are.  A block's four warps take 32
+ * tokens of each tile with their own running maxima and sums and their own ring of
+ * asynchronous copies, and join at the end of a sequence; a sequence that runs over several
+ * blocks leaves 32-bit partial sums in the workspace, which a second kernel joins in order.
+ */
+#include "ops_common.cuh"
+
+int ops_check_cache4(const emmy_ops_cache4 &c);
+
+namespace {
+
+constexpr int WARPS = 4, WARP_TOKENS = 32, TILE = WARPS * WARP_TOKENS, STAGES = 3;
+/* what registers and shared memory let an SM hold of 8-row and of 16-row blocks */
+template <int NT> constexpr int BLOCKS_PER_SM = NT == 1 ? 3 : 2;
+constexpr int MAX_BATCH = 4096;
+
+struct AttendParams {
+    const char *k, *v;
+    const __half2 *k_meta, *v_meta;
+    const char *q;
+    char *out;
+    const int32_t *table, *lengths;
+    float *partial;                     /* [blocks][2][rows][dim], then [blocks][2][rows][2] (max, sum) */
+    int64_t pages, q_batch, q_token, q_head, out_batch, out_token, out_head, table_stride;
+    int batch, tokens, heads, group, row_groups, page, max_positions;
+    float scale_log2;
+};
+
+/* where tile `t` of the list lies */
+struct Place {
+    int sequence, head, row_group, tile, tiles, length;
+};
+
+/* the list of tiles: sequence b's part starts at before[b] * heads * row_groups */
+struct List {
+    int total;                          /* tiles of one (head, row group) over all sequences */
+    int64_t tiles;                      /* of all */
+};
+
+__device__ __forceinline__ int sequence_length(const AttendParams &p, int b) {
+    return max(0, min(p.lengths[b], p.max_positions));
+}
+__device__ __forceinline__ int sequence_tiles(int length) { return max(1, (length + TILE - 1) / TILE); }
+
+/* exclusive sums of the sequences' tiles into shared memory; all threads of the block */
+__device__ __forceinline__ int sum_tiles(const AttendParams &p, int32_t *before, int *warp_sums) {
+    int carry = 0;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+    for (int base = 0; base < p.batch; base += blockDim.x) {
+        const int b = base + threadIdx.x;
+        const int own = b < p.batch ? sequence_tiles(sequence_length(p, b)) : 0;
+        int upto = own;
+#pragma unroll
+        for (int d = 1; d < 32; d <<= 1) {
+            const int o = __shfl_up_sync(~0u, upto, d);
+            if (lane >= d) upto += o;
+        }
+        if (lane == 31) warp_sums[warp] = upto;
+        __syncthreads();
+        int pre = carry, all = 0;
+        for (int w = 0; w < warps; ++w) {
+            if (w < warp) pre += warp_sums[w];
+            all += warp_sums[w];
+        }
+        if (b < p.batch) before[b] = pre + upto - own;
+        carry += all;
+        __syncthreads();
+    }
+    if (threadIdx.x == 0) before[p.batch] = carry;
+    __syncthreads();
+    return carry;
+}
+
+__device__ __forceinline__ int64_t run_start(int64_t tiles, int64_t block, int64_t blocks) { return tiles * block / blocks; }
+/* the last block whose run starts at or before tile t */
+__device__ __forceinline__ int64_t run_of(int64_t tiles, int64_t t, int64_t blocks) { return ((t + 1) * blocks - 1) / tiles; }
+
+__device__ __forceinline__ Place find(const AttendParams &p, const int32_t *before, int64_t t) {
+    const int per = p.heads * p.row_groups;
+    int lo = 0, hi = p.batch - 1;
+    while (lo < hi) {                   /* the last sequence that starts at or before t */
+        const int mid = (lo + hi + 1) / 2;
+        if ((int64_t)before[mid] * per <= t) lo = mid; else hi = mid - 1;
+    }
+    Place at;
+    at.sequence = lo;
+    at.tiles = before[lo + 1] - before[lo];
+    const int64_t r = t - (int64_t)before[lo] * per;
+    const int segment = (int)(r / at.tiles);
+    at.tile = (int)(r - (int64_t)segment * at.tiles);
+    at.head = segment / p.row_groups;
+    at.row_group = segment - at.head * p.row_groups;
+    at.length = sequence_length(p, lo);
+    return at;
+}
+
+__device__ __forceinline__ void advance(const AttendParams &p, const int32_t *before, Place &at) {
+    if (++at.tile < at.tiles) return;
+    at.tile = 0;
+    if (++at.row_group < p.row_groups) return;
+    at.row_group = 0;
+    if (++at.head < p.heads) return;
+    at.head = 0;
+    if (++at.sequence >= p.batch) return;
+    at.tiles = before[at.sequence + 1] - before[at.sequence];
+    at.length = sequence_length(p, at.sequence);
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void *from, bool live) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy4(uint32_t to, const void *from, bool live) {
+    asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(live ? 4 : 0) : "memory");
+}
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
+    return v;
+}
+__device__ __forceinline__ uint32_t packed(float low, float high) {
+    const __half2 h = __floats2half2_rn(low, high);
+    return *(const uint32_t *)&h;
+}
+__device__ __forceinline__ float exp2_approx(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+/* The token that row r (0 .. 7) of an eight-token group stands for.  A warp reads a token's keys by
+ * r = lane / 4 and its values by the pairs r = 2 (lane % 4) + {0, 1}; these orders (with the
+ * swizzle below at dim 128) put both into different banks. */
+template <int DIM> __device__ __forceinline__ int token_of(int r) {
+    return DIM == 128 ? r ^ ((r >> 1) & 1) : (r & 1 ? 4 + ((r >> 1) ^ 2) : r >> 1);
+}
+template <int DIM> __device__ __forceinline__ int swizzled(int token, int byte) {
+    return DIM == 128 ? byte ^ ((token & 4) << 3) : byte;
+}
+
+template <int DIM> struct alignas(16) Stage {
+    unsigned char k[WARP_TOKENS * DIM / 2], v[WARP_TOKENS * DIM / 2];
+    __half2 k_meta[WARP_TOKENS], v_meta[WARP_TOKENS];
+    uint32_t held;                      /* bit t: token t is in the sequence, on a page of the cache */
+};
+
+template <int DIM, int NT> struct Shared {
+    Stage<DIM> ring[WARPS][STAGES];
+    float out[WARPS][8 * NT][DIM + 4];
+    float top[WARPS][8 * NT], sum[WARPS][8 * NT];
+    int warp_sums[WARPS];
+    int32_t before[];
+};
+
+template <typename T, int DIM, int NT>
+__global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(AttendParams p) {
+    extern __shared__ __align__(16) unsigned char raw[];
+    Shared<DIM, NT> &sh = *(Shared<DIM, NT> *)raw;
+    constexpr int ROWS = 8 * NT, WORDS = DIM / 32, ROW_BYTES = DIM / 2, OT = DIM / 16;
+    enter_grid();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int total = sum_tiles(p, sh.before, sh.warp_sums);
+    const int64_t tiles = (int64_t)total * p.heads * p.row_groups;
+    const int64_t first = run_start(tiles, blockIdx.x, gridDim.x), last = run_start(tiles, blockIdx.x + 1, gridDim.x);
+    if (first >= last) return;
+    Place ahead = find(p, sh.before, first), at = ahead;
+    int64_t issued = first;
+
+    /* the copies' side: the row of this lane's token in the cache (page * heads * page rows), -1 for none */
+    auto lookup = [&](const Place &place) -> int64_t {
+        const int position = place.tile * TILE + warp * WARP_TOKENS + lane;
+        if (position >= place.length) return -1;
+        const int page = position / p.page;
+        const int64_t index = p.table[place.sequence * p.table_stride + page];
+        if (index < 0 || index >= p.pages) return -1;
+        return (index * p.heads + place.head) * p.page + (position - page * p.page);
+    };
+    int64_t row = lookup(ahead);
+    auto issue = [&](int stage) {
+        if (issued < last) {
+            Stage<DIM> &s = sh.ring[warp][stage];
+            constexpr int CHUNKS = ROW_BYTES / 16, PER = 32 / CHUNKS;
+#pragma unroll
+            for (int i = 0; i < CHUNKS; ++i) {
+                const int token = i * PER + lane / CHUNKS, byte = lane % CHUNKS * 16;
+                const int64_t from = __shfl_sync(~0u, row, token);
+                const uint32_t to = token * ROW_BYTES + swizzled<DIM>(token, byte);
+                const int64_t offset = (from < 0 ? 0 : from) * ROW_BYTES + byte;
+                copy16((uint32_t)__cvta_generic_to_shared(s.k) + to, p.k + offset, from >= 0);
+                copy16((uint32_t)__cvta_generic_to_shared(s.v) + to, p.v + offset, from >= 0);
+            }
+            const uint32_t held = __ballot_sync(~0u, row >= 0);
+            if (lane == 0) s.held = held;
+            copy4((uint32_t)__cvta_generic_to_shared(&s.k_meta[lane]), p.k_meta + (row < 0 ? 0 : row), row >= 0);
+            copy4((uint32_t)__cvta_generic_to_shared(&s.v_meta[lane]), p.v_meta + (row < 0 ? 0 : row), row >= 0);
+            if (++issued < last) {
+                advance(p, sh.before, ahead);
+                row = lookup(ahead);
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int s = 0; s < STAGES - 1; ++s) issue(s);
+
+    uint32_t qf[NT][2 * WORDS][2];
+    float o[NT][OT][4], least[NT][2], top[NT][2], sum[NT][2], by[NT][2], base[NT][2];
+    int sees[NT][2];
+    int v_exponent = 0;
+    int64_t segment_start = first;
+    int stage = 0;
+    for (int64_t t = first; t < last; ++t) {
+        if (t == first || at.tile == 0) {
+            /* a new (sequence, head, group of rows): its queries */
+            segment_start = t;
+            v_exponent = -16;
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+                const int own = at.row_group * ROWS + n * 8 + r, rows = p.tokens * p.group;
+                float v[8 * WORDS], largest = 0.0f, all = 0.0f;
+                const int token = own / p.group;
+                if (own < rows) {
+                    const T *q = (const T *)p.q + at.sequence * p.q_batch + token * p.q_token +
+                                 (int64_t)(at.head * p.group + own - token * p.group) * p.q_head + c * 8 * WORDS;
+#pragma unroll
+                    for (int i = 0; i < 8 * WORDS; ++i) v[i] = to_f32(q[i]);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8 * WORDS; ++i) v[i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < 8 * WORDS; ++i) largest = fmaxf(largest, fabsf(v[i])), all += v[i];
+#pragma unroll
+                for (int d = 1; d < 4; d <<= 1) {
+                    largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, d));
+                    all += __shfl_xor_sync(~0u, all, d);
+                }
+                const int exponent = max((int)(__float_as_uint(largest) >> 23) - 127, -100);
+                const float up = __uint_as_float((uint32_t)(127 + 13 - min(exponent, 127)) << 23);
+#pragma unroll
+                for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 8 * w + 2 * i;
+                        qf[n][2 * w + i][0] = packed(v[e] * up, v[e + 4] * up);
+                        qf[n][2 * w + i][1] = packed(v[e + 1] * up * 0x1p-4f, v[e + 5] * up * 0x1p-4f);
+                    }
+                /* of the rows that this thread has in the scores: 2 c and 2 c + 1 */
+                const float mine = p.scale_log2 / up, mine0 = p.scale_log2 * all;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    by[n][i] = __shfl_sync(~0u, mine, 4 * (2 * c + i));
+                    base[n][i] = __shfl_sync(~0u, mine0, 4 * (2 * c + i));
+                    const int row = at.row_group * ROWS + n * 8 + 2 * c + i;
+                    sees[n][i] = row < rows ? at.length - p.tokens + row / p.group + 1 : 0;
+                    top[n][i] = -INFINITY;
+                    sum[n][i] = least[n][i] = 0.0f;
+                }
+#pragma unroll
+                for (int i = 0; i < OT; ++i)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+            }
+        }
+        issue((stage + STAGES - 1) % STAGES);
+        asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        __syncwarp();
+        const Stage<DIM> &s = sh.ring[warp][stage];
+        /* S^T = K Q^T */
+        float score[2][NT][4];
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) score[m][n][j] = 0.0f;
+            const int t0 = 16 * m + token_of<DIM>(r), t1 = t0 + 8;
+            const Pack<uint32_t, WORDS> x0 =
+                *(const Pack<uint32_t, WORDS> *)(s.k + t0 * ROW_BYTES + swizzled<DIM>(t0, c * 4 * WORDS));
+            const Pack<uint32_t, WORDS> x1 =
+                *(const Pack<uint32_t, WORDS> *)(s.k + t1 * ROW_BYTES + swizzled<DIM>(t1, c * 4 * WORDS));
+#pragma unroll
+            for (int w = 0; w < WORDS; ++w)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const uint32_t a = x0.at[w] >> 8 * i, b = x1.at[w] >> 8 * i;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+                        mma(score[m][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0,
+                            qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+                }
+        }
+        /* logits to base 2, and the running maximum */
+        const int from = at.tile * TILE + warp * WARP_TOKENS;
+        const uint32_t held = s.held;
+        bool moved = false;
+        float next[NT][2], shrink[NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) next[n][i] = top[n][i];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int token = 16 * m + 8 * h + token_of<DIM>(r);
+                const float2 meta = __half22float2(s.k_meta[token]);
+                const int place = held >> token & 1 ? from + token : 0x7fffffff;
+                const float step = meta.x * 0x1p24f;
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float &x = score[m][n][2 * h + i];
+                        x = place < sees[n][i] ? fmaf(step, x * by[n][i], meta.y * base[n][i]) : -INFINITY;
+                        next[n][i] = fmaxf(next[n][i], x);
+                    }
+            }
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                for (int d = 4; d < 32; d <<= 1) next[n][i] = fmaxf(next[n][i], __shfl_xor_sync(~0u, next[n][i], d));
+                const float ref = next[n][i] == -INFINITY ? 0.0f : next[n][i];
+                shrink[n][i] = exp2_approx(top[n][i] - ref);
+                moved |= next[n][i] != top[n][i];
+                top[n][i] = next[n][i];
+            }
+        /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
+        const uint32_t step_bits = __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff;
+        const int exponent = (int)(__reduce_max_sync(~0u, step_bits) >> 10) - 15;
+        float rescale = 1.0f;
+        if (exponent > v_exponent) {
+            rescale = exp2_approx((float)(v_exponent - exponent));
+            v_exponent = exponent;
+            moved = true;
+        }
+        const float up = __uint_as_float((uint32_t)(127 + 14 - v_exponent) << 23);
+        if (__any_sync(~0u, moved)) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    sum[n][i] *= shrink[n][i];
+                    least[n][i] *= shrink[n][i];
+                }
+                const float f0 = shrink[n][0] * rescale, f1 = shrink[n][1] * rescale;
+#pragma unroll
+                for (int i = 0; i < OT; ++i)
+                    o[n][i][0] *= f0, o[n][i][1] *= f1, o[n][i][2] *= f0, o[n][i][3] *= f1;
+            }
+        }
+        uint32_t pf[2][NT][2];
+#pragma unroll
+        for (int m = 0; m < 2; ++m)
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const int token = 16 * m + 8 * h + token_of<DIM>(r);
+                const float2 meta = __half22float2(s.v_meta[token]);
+                const float step = meta.x * up;
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    float e[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const float ref = top[n][i] == -INFINITY ? 0.0f : top[n][i];
+                        e[i] = exp2_approx(score[m][n][2 * h + i] - ref);
+                        sum[n][i] += e[i];
+                        least[n][i] = fmaf(e[i], meta.y, least[n][i]);
+                    }
+                    pf[m][n][h] = transposed(packed(e[0] * step, e[1] * step));
+                }
+            }
+        /* O^T += V^T P^T */
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+            Pack<uint32_t, WORDS / 2> x[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int token = 16 * m + 8 * (i >> 1) + token_of<DIM>(2 * c + (i & 1));
+                x[i] = *(const Pack<uint32_t, WORDS / 2> *)(s.v + token * ROW_BYTES + swizzled<DIM>(token, r * 2 * WORDS));
+            }
+#pragma unroll
+            for (int w = 0; w < WORDS / 2; ++w)
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const uint32_t a = __byte_perm(x[0].at[w], x[1].at[w], half ? 0x7632 : 0x5410);
+                    const uint32_t b = __byte_perm(x[2].at[w], x[3].at[w], half ? 0x7632 : 0x5410);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t u = a >> 8 * i, v = b >> 8 * i;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma(o[n][4 * w + 2 * half + i], u & 0x000f000f, u & 0x00f000f0, v & 0x000f000f, v & 0x00f000f0,
+                                pf[m][n][0], pf[m][n][1]);
+                    }
+                }
+        }
+        __syncwarp();                   /* all lanes are done with the stage before it is filled again */
+        stage = (stage + 1) % STAGES;
+
+        if (at.tile + 1 == at.tiles || t + 1 == last) {
+            /* the four warps' sums joined */
+            const float down = __uint_as_float((uint32_t)(127 - 14 + v_exponent) << 23);
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+#pragma unroll
+                    for (int d = 4; d < 32; d <<= 1) {
+                        sum[n][i] += __shfl_xor_sync(~0u, sum[n][i], d);
+                        least[n][i] += __shfl_xor_sync(~0u, least[n][i], d);
+                    }
+                    if (r == 0) {
+                        sh.top[warp][8 * n + 2 * c + i] = top[n][i];
+                        sh.sum[warp][8 * n + 2 * c + i] = sum[n][i];
+                    }
+                    /* this thread's dims: 2 OT from 2 OT r on, of row 2 c + i */
+                    float *to = &sh.out[warp][8 * n + 2 * c + i][2 * OT * r];
+#pragma unroll
+                    for (int j = 0; j < OT; ++j) {
+                        to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, least[n][i]);
+                        to[2 * j + 1] = fmaf(o[n][j][2 + i] * 0x1p20f, down, least[n][i]);
+                    }
+                }
+            __syncthreads();
+            const bool whole = at.tile + 1 == at.tiles && t - segment_start + 1 == at.tiles;
+            const int rows = p.tokens * p.group;
+            const int64_t slot = (int64_t)blockIdx.x * 2 + (segment_start != first);
+            for (int i = threadIdx.x; i < ROWS * DIM / 4; i += WARPS * 32) {
+                const int n = i / (DIM / 4), e = i % (DIM / 4) * 4, own = at.row_group * ROWS + n;
+                float high = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) high = fmaxf(high, sh.top[w][n]);
+                const float ref = high == -INFINITY ? 0.0f : high;
+                float all = 0.0f;
+                float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+                for (int w = 0; w < WARPS; ++w) {
+                    const float f = exp2_approx(sh.top[w][n] - ref);
+                    const float4 x = *(const float4 *)&sh.out[w][n][e];
+                    all = fmaf(f, sh.sum[w][n], all);
+                    v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
+                }
+                if (whole) {
+                    if (own < rows) {
+                        const float inv = all > 0.0f || all != all ? 1.0f / all : 0.0f;
+                        const int token = own / p.group;
+                        T *out = (T *)p.out + at.sequence * p.out_batch + token * p.out_token +
+                                 (int64_t)(at.head * p.group + own - token * p.group) * p.out_head + e;
+                        out[0] = from_f32<T>(v.x * inv), out[1] = from_f32<T>(v.y * inv);
+                        out[2] = from_f32<T>(v.z * inv), out[3] = from_f32<T>(v.w * inv);
+                    }
+                } else {
+                    *(float4 *)(p.partial + (slot * ROWS + n) * DIM + e) = v;
+                    if (e == 0) {
+                        float *stat = p.partial + (int64_t)gridDim.x * 2 * ROWS * DIM + (slot * ROWS + n) * 2;
+                        stat[0] = high, stat[1] = all;
+                    }
+                }
+            }
+            __syncthreads();
+        }
+        if (t + 1 < last) advance(p, sh.before, at);
+    }
+    asm volatile("cp.async.wait_all;" ::: "memory");
+}
+
+/* joins the runs of a segment that several blocks of the first kernel shared, in their order */
+template <typename T, int DIM, int NT>
+__global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
+    constexpr int ROWS = 8 * NT;
+    __shared__ int sums[2][4];
+    enter_grid();
+    const int per = p.heads * p.row_groups, sequence = blockIdx.x / per, segment = blockIdx.x - sequence * per;
+    int before = 0, total = 0;
+    for (int b = threadIdx.x; b < p.batch; b += 128) {
+        const int n = sequence_tiles(sequence_length(p, b));
+        total += n;
+        if (b < sequence) before += n;
+    }
+    before = __reduce_add_sync(~0u, before);
+    total = __reduce_add_sync(~0u, total);
+    if ((threadIdx.x & 31) == 0) sums[0][threadIdx.x >> 5] = before, sums[1][threadIdx.x >> 5] = total;
+    __syncthreads();
+    before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
+    total = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
+    const int64_t tiles = (int64_t)total * per;
+    const int own_tiles = sequence_tiles(sequence_length(p, sequence));
+    const int64_t start = (int64_t)before * per + (int64_t)segment * own_tiles;
+    const int64_t a = run_of(tiles, start, blocks), z = run_of(tiles, start + own_tiles - 1, blocks);
+    if (a == z) return;
+    const float *stats = p.partial + (int64_t)blocks * 2 * ROWS * DIM;
+    const int head = segment / p.row_groups, row_group = segment - head * p.row_groups, rows = p.tokens * p.group;
+    for (int i = threadIdx.x; i < ROWS * DIM / 4; i += 128) {
+        const int n = i / (DIM / 4), e = i % (DIM / 4) * 4, own = row_group * ROWS + n;
+        if (own >= rows) continue;
+        float high = -INFINITY, all = 0.0f;
+        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+        for (int64_t block = a; block <= z; ++block) {
+            const int64_t t = run_start(tiles, block, blocks);
+            if (t == run_start(tiles, block + 1, blocks)) continue;       /* an empty run */
+            const int64_t slot = block * 2 + (t < start);
+            const float top = stats[(slot * ROWS + n) * 2], sum = stats[(slot * ROWS + n) * 2 + 1];
+            const float4 x = *(const float4 *)(p.partial + (slot * ROWS + n) * DIM + e);
+            const float next = fmaxf(high, top), ref = next == -INFINITY ? 0.0f : next;
+            const float f = exp2_approx(high - ref), g = exp2_approx(top - ref);
+            all = fmaf(g, sum, all * f);
+            v.x = fmaf(g, x.x, v.x * f), v.y = fmaf(g, x.y, v.y * f);
+            v.z = fmaf(g, x.z, v.z * f), v.w = fmaf(g, x.w, v.w * f);
+            high = next;
+        }
+        const float inv = all > 0.0f || all != all ? 1.0f / all : 0.0f;
+        const int token = own / p.group;
+        T *out = (T *)p.out + sequence * p.out_batch + token * p.out_token +
+                 (int64_t)(head * p.group + own - token * p.group) * p.out_head + e;
+        out[0] = from_f32<T>(v.x * inv), out[1] = from_f32<T>(v.y * inv);
+        out[2] = from_f32<T>(v.z * inv), out[3] = from_f32<T>(v.w * inv);
+    }
+}
+
+int sm_count(int device, int *out) {
+    static int counts[64];
+    if (device < 0 || device >= 64) return ops_fail(EMMY_RT_EINVAL, "device %d", device);
+    int n = __atomic_load_n(&counts[device], __ATOMIC_RELAXED);
+    if (!n) {
+        cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
+        if (e != cudaSuccess) return ops_cuda(e, "device attribute");
+        __atomic_store_n(&counts[device], n, __ATOMIC_RELAXED);
+    }
+    *out = n;
+    return 0;
+}
+
+template <typename T, int DIM, int NT> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
+    const size_t smem = sizeof(Shared<DIM, NT>) + 4 * ((size_t)p.batch + 1);
+    static uint64_t allowed;                 /* devices whose limit is raised */
+    if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
+        cudaError_t e = cudaFuncSetAttribute(cache4_attend<T, DIM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             (int)(sizeof(Shared<DIM, NT>) + 4 * (MAX_BATCH + 1)));
+        if (e != cudaSuccess) return ops_cuda(e, "shared memory of the attention");
+        __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
+    }
+    const int blocks = sms * BLOCKS_PER_SM<NT>;
+    cudaError_t e = launch(cache4_attend<T, DIM, NT>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
+    if (e != cudaSuccess) return ops_cuda(e, "attention over the 4-bit cache");
+    e = launch(cache4_join<T, DIM, NT>, dim3((unsigned)(p.batch * p.heads * p.row_groups)), dim3(128), 0, stream, p, blocks);
+    return ops_cuda(e, "joining the attention's parts");
+}
+
+uint64_t workspace(int sms, int dim) {
+    const int rows = 8 * (BLOCKS_PER_SM<1> > 2 * BLOCKS_PER_SM<2> ? BLOCKS_PER_SM<1> : 2 * BLOCKS_PER_SM<2>);
+    return (uint64_t)sms * rows * 2 * (dim + 2) * 4;
+}
+
+}  // namespace
+
+EMMY_EXPORT int emmy_ops_cache4_attend_workspace(int dim, int device, uint64_t *bytes) {
+    if (!bytes || (dim != 64 && dim != 128)) return ops_fail(EMMY_RT_EINVAL, "head dim %d is not 64 or 128", dim);
+    int sms;
+    if (int e = sm_count(device, &sms)) return e;
+    *bytes = workspace(sms, dim);
+    return 0;
+}
+
+EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int device, uint64_t stream) {
+    if (!a) return ops_fail(EMMY_RT_EINVAL, "no arguments");
+    if (int e = ops_check_cache4(a->cache)) return e;
+    if (a->dtype != EMMY_OPS_F16 && a->dtype != EMMY_OPS_BF16)
+        return ops_fail(EMMY_RT_EINVAL, "element type %d: queries are f16 or bf16", a->dtype);
+    if (a->batch < 0 || a->batch > MAX_BATCH) return ops_fail(EMMY_RT_EINVAL, "batch %d is not in 0 .. %d", a->batch, MAX_BATCH);
+    if (a->tokens < 0 || a->q_heads < 1 || a->q_heads % a->cache.heads)
+        return ops_fail(EMMY_RT_EINVAL, "%d tokens of %d heads over %d heads of the cache", a->tokens, a->q_heads, a->cache.heads);
+    const int group = a->q_heads / a->cache.heads;
+    if ((int64_t)a->tokens * group > (1 << 20)) return ops_fail(EMMY_RT_EINVAL, "%d tokens a sequence", a->tokens);
+    if (a->max_pages < 0 || (int64_t)a->max_pages * a->cache.page > 0x7fffff00LL)
+        return ops_fail(EMMY_RT_EINVAL, "%d pages of %d rows a sequence", a->max_pages, a->cache.page);
+    if (a->batch == 0 || a->tokens == 0) return 0;
+    if (!a->q || !a->out || !a->lengths || (a->max_pages && !a->table) || !a->workspace || !aligned(a->workspace, 16))
+        return ops_fail(EMMY_RT_EINVAL, "q, out, table, lengths and a workspace (on 16 bytes) are needed");
+    if (!aligned(a->q, 2) || !aligned(a->out, 2) || !aligned(a->table, 4) || !aligned(a->lengths, 4))
+        return ops_fail(EMMY_RT_EINVAL, "an operand is not aligned to its elements");
+    const int rows = a->tokens * group, nt = rows <= 8 ? 1 : 2;
+    AttendParams p = {};
+    p.k = (const char *)(uintptr_t)a->cache.k, p.v = (const char *)(uintptr_t)a->cache.v;
+    p.k_meta = (const __half2 *)(uintptr_t)a->cache.k_meta, p.v_meta = (const __half2 *)(uintptr_t)a->cache.v_meta;
+    p.q = (const char *)(uintptr_t)a->q, p.out = (char *)(uintptr_t)a->out;
+    p.table = (const int32_t *)(uintptr_t)a->table, p.lengths = (const int32_t *)(uintptr_t)a->lengths;
+    p.partial = (float *)(uintptr_t)a->workspace;
+    p.pages = a->cache.pages;
+    p.q_batch = a->q_batch, p.q_token = a->q_token, p.q_head = a->q_head;
+    p.out_batch = a->out_batch, p.out_token = a->out_token, p.out_head = a->out_head, p.table_stride = a->table_stride;
+    p.batch = a->batch, p.tokens = a->tokens, p.heads = a->cache.heads, p.group = group;
+    p.row_groups = (rows + 8 * nt - 1) / (8 * nt), p.page = a->cache.page;
+    p.max_positions = a->max_pages * a->cache.page;
+    p.scale_log2 = (float)(a->scale * 1.4426950408889634);
+    if ((int64_t)p.batch * p.heads * p.row_groups > 0x7fffffffLL ||
+        (int64_t)p.batch * ((int64_t)p.max_positions / TILE + 1) > 0x7fffffffLL)
+        return ops_fail(EMMY_RT_EINVAL, "%d sequences of %d positions are too many for one call", p.batch, p.max_positions);
+    int sms;
+    if (int e = sm_count(device, &sms)) return e;
+    if (a->workspace_bytes < workspace(sms, a->cache.dim))
+        return ops_fail(EMMY_RT_ESCRATCH, "a workspace of %llu bytes is too small", (unsigned long long)a->workspace_bytes);
+    DeviceScope scope(device);
+    if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
+    const bool f16 = a->dtype == EMMY_OPS_F16;
+    if (a->cache.dim == 64) {
+        if (nt == 1) return f16 ? go<__half, 64, 1>(p, sms, device, stream) : go<__nv_bfloat16, 64, 1>(p, sms, device, stream);
+        return f16 ? go<__half, 64, 2>(p, sms, device, stream) : go<__nv_bfloat16, 64, 2>(p, sms, device, stream);
+    }
+    if (nt == 1) return f16 ? go<__half, 128, 1>(p, sms, device, stream) : go<__nv_bfloat16, 128, 1>(p, sms, device, stream);
+    return f16 ? go<__half, 128, 2>(p, sms, device, stream) : go<__nv_bfloat16, 128, 2>(p, sms, device, stream);
+}

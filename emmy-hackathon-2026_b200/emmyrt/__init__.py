@@ -496,6 +496,14 @@ class Cache4AppendArgs(ctypes.Structure):
         [("slots_64", ctypes.c_int32), ("dtype", ctypes.c_int32)]
 
 
+class Cache4AttendArgs(ctypes.Structure):
+    """emmy_ops_cache4_attend_args"""
+    _fields_ = _CACHE4 + [(n, _u64) for n in ("q", "out", "table", "lengths", "workspace", "workspace_bytes")] + \
+        [(n, ctypes.c_int64) for n in ("q_batch", "q_token", "q_head", "out_batch", "out_token", "out_head",
+                                       "table_stride")] + \
+        [(n, ctypes.c_int32) for n in ("batch", "tokens", "q_heads", "max_pages", "dtype")] + [("scale", ctypes.c_float)]
+
+
 # every symbol declared in include/emmyrt_ops.h, with its ctypes signature
 OPS_SIGNATURES = {
     "emmy_ops_last_error": ([], ctypes.c_char_p),
@@ -503,6 +511,8 @@ OPS_SIGNATURES = {
     "emmy_ops_residual_norm": ([_P(NormArgs), _int, _u64], _int),
     "emmy_ops_rotary": ([_P(RotaryArgs), _int, _u64], _int),
     "emmy_ops_cache4_append": ([_P(Cache4AppendArgs), _int, _u64], _int),
+    "emmy_ops_cache4_attend_workspace": ([_int, _int, _P(_u64)], _int),
+    "emmy_ops_cache4_attend": ([_P(Cache4AttendArgs), _int, _u64], _int),
 }
 _ops_lib = None
 

@@ -1,4 +1,4 @@
-"""A paged key / value cache in 4 bits: appending tokens to it.
+"""A paged key / value cache in 4 bits: appending tokens to it, and attention over it.
 
 A token's vector of one head is held as levels 0 .. 15 with an f16 step and least value: an element
 stands for ``level * step + least``.  At head dim 128 that is 68 bytes instead of the 256 of bf16.
@@ -6,8 +6,11 @@ stands for ``level * step + least``.  At head dim 128 that is 68 bytes instead o
 
 from __future__ import annotations
 
-from . import Cache4AppendArgs, DeviceBuffer
-from .operands import CODE, FLOATS, INDICES, Array, Operator, Plan, apart, contiguous, operand, overlaps, shaped
+import ctypes
+import math
+
+from . import Cache4AppendArgs, Cache4AttendArgs, DeviceBuffer, EmmyRTError, ops_lib
+from .operands import CODE, FLOATS, INDICES, Array, Operator, Plan, apart, contiguous, operand, overlaps, shaped, written
 
 DIMS = (64, 128)
 
@@ -74,3 +77,57 @@ class Cache4(Operator):
         for part in held:
             checks += overlaps([part], ins + outs)
         return Plan("emmy_ops_cache4_append", a, self._FIELDS, checks)
+
+
+class Cache4Attention(Operator):
+    """Attention of ``q_heads`` query heads over a :class:`Cache4`; ``q_heads / cache.heads`` of them share a cached head.
+
+    The object owns the workspace of its calls: calls of one object must not overlap on the GPU (one stream, or events;
+    graphs that hold them likewise).  Make one for each stream that runs at the same time as others.
+    """
+
+    def __init__(self, cache: Cache4, q_heads: int):
+        super().__init__()
+        if cache.device != self.device:
+            raise ValueError(f"the cache is on GPU {cache.device}, the current one is {self.device}")
+        if q_heads < 1 or q_heads % cache.heads:
+            raise ValueError(f"{q_heads} query heads over {cache.heads} heads of the cache")
+        self.cache, self.q_heads = cache, int(q_heads)
+        need = ctypes.c_uint64()
+        status = ops_lib().emmy_ops_cache4_attend_workspace(cache.dim, self.device, ctypes.byref(need))
+        if status:
+            raise EmmyRTError(status, "attention workspace", ops_lib().emmy_ops_last_error().decode(errors="replace"))
+        self._workspace = DeviceBuffer(need.value)
+
+    def __call__(self, q, out, table, lengths, *, scale: float | None = None, stream: int = 0) -> None:
+        """``q`` and ``out`` are [batch, tokens, q_heads, dim] (f16 or bf16), ``lengths`` [batch] and ``table``
+        [batch, pages] int32: position p of sequence b is row ``p % page`` of the cache's page ``table[b, p // page]``.
+        Query i stands at position ``lengths[b] - tokens + i`` (its key is in the cache already) and sees the positions up
+        to its own; a query that sees nothing gives zeros.  Lengths beyond the table are cut there; pages that are none
+        are not seen.  ``scale`` is 1 / sqrt(dim) by default.  ``out`` may be ``q``."""
+        scale = self.cache.dim ** -0.5 if scale is None else float(scale)
+        self._call((q, out, table, lengths, *self.cache.arrays), scale, stream)
+
+    _FIELDS = ("q", "out", "table", "lengths", "cache_k", "cache_v", "cache_k_meta", "cache_v_meta")
+
+    def _plan(self, operands, scale) -> Plan:
+        q, out, table, lengths = operands[:4]
+        c, d = self.cache, self.device
+        if not math.isfinite(scale):
+            raise ValueError(f"scale {scale}")
+        q = operand(q, "q", ("f16", "bf16"), 4, d)
+        batch, tokens = q.shape[:2]
+        shaped(q, "q", (batch, tokens, self.q_heads, c.dim))
+        out = written(shaped(operand(out, "out", (q.dtype,), 4, d), "out", q.shape), "out")
+        table = operand(table, "table", ("i32",), 2, d)
+        if table.shape[0] != batch:
+            raise ValueError(f"table has {table.shape[0]} rows for {batch} sequences")
+        lengths = shaped(operand(lengths, "lengths", ("i32",), 1, d), "lengths", (batch,))
+        a = Cache4AttendArgs(cache_pages=c.pages, cache_heads=c.heads, cache_page=c.page, cache_dim=c.dim,
+                             workspace=self._workspace.ptr, workspace_bytes=self._workspace.nbytes, q_batch=q.strides[0],
+                             q_token=q.strides[1], q_head=q.strides[2], out_batch=out.strides[0], out_token=out.strides[1],
+                             out_head=out.strides[2], table_stride=table.strides[0], batch=batch, tokens=tokens,
+                             q_heads=self.q_heads, max_pages=table.shape[1], dtype=CODE[q.dtype], scale=scale)
+        others = [(0, q, "q"), (2, table, "table"), (3, lengths, "lengths")]
+        others += [(4 + i, part, "the cache") for i, part in enumerate(c.arrays)]
+        return Plan("emmy_ops_cache4_attend", a, self._FIELDS, overlaps([(1, out, "out")], others, same=((1, 0),)))

@@ -112,6 +112,24 @@ typedef struct {
 
 int emmy_ops_cache4_append(const emmy_ops_cache4_append_args *a, int device, uint64_t stream);
 
+/* Attention of `tokens` queries a sequence over its cached positions: query i of sequence b
+ * stands at position lengths[b] - tokens + i and sees the positions up to its own; one that
+ * sees nothing gives zeros.  q and out are (batch, tokens, q_heads, dim), the last one
+ * contiguous; q_heads / cache.heads query heads share a head of the cache.  Sequence b's
+ * positions lie in the pages table[b * table_stride ..] (max_pages of them); lengths beyond
+ * them are cut there, and nothing is seen of a page that is no page of the cache.  The workspace is emmy_ops_cache4_attend_workspace bytes; nothing in it is kept
+ * from call to call. */
+typedef struct {
+    emmy_ops_cache4 cache;
+    uint64_t q, out, table, lengths, workspace, workspace_bytes;   /* table, lengths: int32 */
+    int64_t q_batch, q_token, q_head, out_batch, out_token, out_head, table_stride;
+    int32_t batch, tokens, q_heads, max_pages, dtype;
+    float scale;
+} emmy_ops_cache4_attend_args;
+
+int emmy_ops_cache4_attend_workspace(int dim, int device, uint64_t *bytes);
+int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int device, uint64_t stream);
+
 #ifdef __cplusplus
 }
 #endif
