@@ -12,8 +12,8 @@
  *
  * The bytes of the cache bound it: a token is (dim / 2 + 4) * 2 bytes per head.  A level in
  * bits 0..3 of a 16-bit half IS an f16 number, level * 2^-24 (a subnormal one), and one in
- * bits 4..7 is level * 2^-20; the tensor cores multiply subnormal f16 exactly.  So unpacking is
- * one AND per two elements and one shift per eight, with no conversion; the powers of two
+ * bits 4..7 is level * 2^-20; the tensor cores multiply subnormal f16 exactly.  So unpacking a key
+ * is one AND per two elements and one shift per eight, with no conversion; the powers of two
  * are put into q's odd elements and into the results.  The queries are scaled by a power of
  * two per row so that their largest element is just below 2^14, which leaves f16 no less exact
  * than the 16-bit type they come in.
@@ -182,11 +182,15 @@ template <int DIM, int NT> struct Shared {
     int32_t before[];
 };
 
-template <typename T, int DIM, int NT>
+template <typename T, int DIM, int NT, bool PAGE32>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(AttendParams p) {
     extern __shared__ __align__(16) unsigned char raw[];
     Shared<DIM, NT> &sh = *(Shared<DIM, NT> *)raw;
     constexpr int ROWS = 8 * NT, WORDS = DIM / 32, ROW_BYTES = DIM / 2, OT = DIM / 16;
+    /* p s_v goes to f16, off by up to 2^-12 of itself.  Beside an f16 result that shows (3.2e-4 of the result's norm against
+     * 2.1e-4 from its own rounding), so there sum p and sum p z take the p that the rounded product stands for: what
+     * is left is 2^-12 of the values' distance from their mean.  A bf16 result's rounding hides it. */
+    constexpr bool EXACT = sizeof(T) == 2 && !__is_same(T, __nv_bfloat16);
     enter_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int total = sum_tiles(p, sh.before, sh.warp_sums);
@@ -196,9 +200,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     Place ahead = find(p, sh.before, first), at = ahead;
     int64_t issued = first;
 
-    /* the copies' side: the row of this lane's token in the cache (page * heads * page rows), -1 for none */
+    /* The copies' side.  `row`: this lane's token in the cache (rows of pages x heads x page), -1 for none.  With pages of
+     * a multiple of 32 rows a warp's tokens are consecutive rows of one page, so `row` is the first one's, the
+     * same for all lanes, and the copies take the page's rows behind a sequence's end along. */
     auto lookup = [&](const Place &place) -> int64_t {
-        const int position = place.tile * TILE + warp * WARP_TOKENS + lane;
+        const int position = place.tile * TILE + warp * WARP_TOKENS + (PAGE32 ? 0 : lane);
         if (position >= place.length) return -1;
         const int page = position / p.page;
         const int64_t index = p.table[place.sequence * p.table_stride + page];
@@ -210,19 +216,39 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         if (issued < last) {
             Stage<DIM> &s = sh.ring[warp][stage];
             constexpr int CHUNKS = ROW_BYTES / 16, PER = 32 / CHUNKS;
+            const uint32_t k_to = (uint32_t)__cvta_generic_to_shared(s.k), v_to = (uint32_t)__cvta_generic_to_shared(s.v);
+            const uint32_t meta_to = (uint32_t)__cvta_generic_to_shared(&s.k_meta[lane]);
+            uint32_t held;
+            if (PAGE32) {
+                const int left = ahead.length - ahead.tile * TILE - warp * WARP_TOKENS;
+                held = row < 0 ? 0 : left >= 32 ? ~0u : (1u << left) - 1;
+                if (row >= 0) {
+                    const int64_t offset = row * ROW_BYTES + lane * 16;
+                    const char *k = p.k + offset, *v = p.v + offset;
+                    const uint32_t to = lane / CHUNKS * ROW_BYTES + swizzled<DIM>(lane / CHUNKS, lane % CHUNKS * 16);
 #pragma unroll
-            for (int i = 0; i < CHUNKS; ++i) {
-                const int token = i * PER + lane / CHUNKS, byte = lane % CHUNKS * 16;
-                const int64_t from = __shfl_sync(~0u, row, token);
-                const uint32_t to = token * ROW_BYTES + swizzled<DIM>(token, byte);
-                const int64_t offset = (from < 0 ? 0 : from) * ROW_BYTES + byte;
-                copy16((uint32_t)__cvta_generic_to_shared(s.k) + to, p.k + offset, from >= 0);
-                copy16((uint32_t)__cvta_generic_to_shared(s.v) + to, p.v + offset, from >= 0);
+                    for (int i = 0; i < CHUNKS; ++i) {
+                        copy16(k_to + to + i * 512, k + i * 512, true);
+                        copy16(v_to + to + i * 512, v + i * 512, true);
+                    }
+                    copy4(meta_to, p.k_meta + row + lane, true);
+                    copy4(meta_to + sizeof s.k_meta, p.v_meta + row + lane, true);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < CHUNKS; ++i) {
+                    const int token = i * PER + lane / CHUNKS, byte = lane % CHUNKS * 16;
+                    const int64_t from = __shfl_sync(~0u, row, token);
+                    const uint32_t to = token * ROW_BYTES + swizzled<DIM>(token, byte);
+                    const int64_t offset = (from < 0 ? 0 : from) * ROW_BYTES + byte;
+                    copy16(k_to + to, p.k + offset, from >= 0);
+                    copy16(v_to + to, p.v + offset, from >= 0);
+                }
+                held = __ballot_sync(~0u, row >= 0);
+                copy4(meta_to, p.k_meta + (row < 0 ? 0 : row), row >= 0);
+                copy4(meta_to + sizeof s.k_meta, p.v_meta + (row < 0 ? 0 : row), row >= 0);
             }
-            const uint32_t held = __ballot_sync(~0u, row >= 0);
             if (lane == 0) s.held = held;
-            copy4((uint32_t)__cvta_generic_to_shared(&s.k_meta[lane]), p.k_meta + (row < 0 ? 0 : row), row >= 0);
-            copy4((uint32_t)__cvta_generic_to_shared(&s.v_meta[lane]), p.v_meta + (row < 0 ? 0 : row), row >= 0);
             if (++issued < last) {
                 advance(p, sh.before, ahead);
                 row = lookup(ahead);
@@ -235,7 +261,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     uint32_t qf[NT][2 * WORDS][2];
     float o[NT][OT][4], least[NT][2], top[NT][2], sum[NT][2], by[NT][2], base[NT][2];
     int sees[NT][2];
-    int v_exponent = 0;
+    int v_exponent = 0, all_see = 0;
     int64_t segment_start = first;
     int stage = 0;
     for (int64_t t = first; t < last; ++t) {
@@ -243,6 +269,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
             /* a new (sequence, head, group of rows): its queries */
             segment_start = t;
             v_exponent = -16;
+            all_see = at.length - p.tokens + 1;
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const int own = at.row_group * ROWS + n * 8 + r, rows = p.tokens * p.group;
@@ -322,8 +349,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         /* logits to base 2, and the running maximum */
         const int from = at.tile * TILE + warp * WARP_TOKENS;
         const uint32_t held = s.held;
+        const bool full = held == ~0u && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
         bool moved = false;
-        float next[NT][2], shrink[NT][2];
+        float next[NT][2], shrink[NT][2], v_step[2][2], v_least[2][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -333,17 +361,29 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int token = 16 * m + 8 * h + token_of<DIM>(r);
-                const float2 meta = __half22float2(s.k_meta[token]);
-                const int place = held >> token & 1 ? from + token : 0x7fffffff;
+                const float2 meta = __half22float2(s.k_meta[token]), v_meta = __half22float2(s.v_meta[token]);
                 const float step = meta.x * 0x1p24f;
+                v_step[m][h] = v_meta.x, v_least[m][h] = v_meta.y;
 #pragma unroll
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         float &x = score[m][n][2 * h + i];
-                        x = place < sees[n][i] ? fmaf(step, x * by[n][i], meta.y * base[n][i]) : -INFINITY;
-                        next[n][i] = fmaxf(next[n][i], x);
+                        x = fmaf(step, x * by[n][i], meta.y * base[n][i]);
                     }
+                if (!full) {
+                    const bool is_held = held >> token & 1;
+                    if (!is_held) v_step[m][h] = v_least[m][h] = 0.0f;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i)
+                            if (!is_held || from + token >= sees[n][i]) score[m][n][2 * h + i] = -INFINITY;
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) next[n][i] = fmaxf(next[n][i], score[m][n][2 * h + i]);
             }
 #pragma unroll
         for (int n = 0; n < NT; ++n)
@@ -357,7 +397,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 top[n][i] = next[n][i];
             }
         /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
-        const uint32_t step_bits = __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff;
+        const uint32_t step_bits = held >> lane & 1 ? __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff : 0;
         const int exponent = (int)(__reduce_max_sync(~0u, step_bits) >> 10) - 15;
         float rescale = 1.0f;
         if (exponent > v_exponent) {
@@ -385,9 +425,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         for (int m = 0; m < 2; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int token = 16 * m + 8 * h + token_of<DIM>(r);
-                const float2 meta = __half22float2(s.v_meta[token]);
-                const float step = meta.x * up;
+                const float step = v_step[m][h] * up, inverse = EXACT ? 1.0f / step : 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float e[2];
@@ -395,10 +433,19 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     for (int i = 0; i < 2; ++i) {
                         const float ref = top[n][i] == -INFINITY ? 0.0f : top[n][i];
                         e[i] = exp2_approx(score[m][n][2 * h + i] - ref);
-                        sum[n][i] += e[i];
-                        least[n][i] = fmaf(e[i], meta.y, least[n][i]);
                     }
-                    pf[m][n][h] = transposed(packed(e[0] * step, e[1] * step));
+                    const __half2 ps = __floats2half2_rn(e[0] * step, e[1] * step);
+                    pf[m][n][h] = transposed(*(const uint32_t *)&ps);
+                    if (EXACT) {
+                        const float2 rounded = __half22float2(ps);
+                        if (rounded.x >= 0x1p-14f) e[0] = rounded.x * inverse;
+                        if (rounded.y >= 0x1p-14f) e[1] = rounded.y * inverse;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        sum[n][i] += e[i];
+                        least[n][i] = fmaf(e[i], v_least[m][h], least[n][i]);
+                    }
                 }
             }
         /* O^T += V^T P^T */
@@ -416,13 +463,14 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 for (int half = 0; half < 2; ++half) {
                     const uint32_t a = __byte_perm(x[0].at[w], x[1].at[w], half ? 0x7632 : 0x5410);
                     const uint32_t b = __byte_perm(x[2].at[w], x[3].at[w], half ? 0x7632 : 0x5410);
+                    /* bytes 0 and 2, then 1 and 3; the even dim's level alone, and the whole byte,
+                     * 16 times the odd dim's level more: the even sum is taken out at the end */
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        const uint32_t u = a >> 8 * i, v = b >> 8 * i;
+                        const uint32_t u = __byte_perm(a, 0, i ? 0x4341 : 0x4240), v = __byte_perm(b, 0, i ? 0x4341 : 0x4240);
 #pragma unroll
                         for (int n = 0; n < NT; ++n)
-                            mma(o[n][4 * w + 2 * half + i], u & 0x000f000f, u & 0x00f000f0, v & 0x000f000f, v & 0x00f000f0,
-                                pf[m][n][0], pf[m][n][1]);
+                            mma(o[n][4 * w + 2 * half + i], u & 0x000f000f, u, v & 0x000f000f, v, pf[m][n][0], pf[m][n][1]);
                     }
                 }
         }
@@ -450,7 +498,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
                     for (int j = 0; j < OT; ++j) {
                         to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, least[n][i]);
-                        to[2 * j + 1] = fmaf(o[n][j][2 + i] * 0x1p20f, down, least[n][i]);
+                        to[2 * j + 1] = fmaf((o[n][j][2 + i] - o[n][j][i]) * 0x1p20f, down, least[n][i]);
                     }
                 }
             __syncthreads();
@@ -501,6 +549,7 @@ template <typename T, int DIM, int NT>
 __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
     constexpr int ROWS = 8 * NT;
     __shared__ int sums[2][4];
+    __shared__ float tops[4], totals[4], parts[4][DIM];
     enter_grid();
     const int per = p.heads * p.row_groups, sequence = blockIdx.x / per, segment = blockIdx.x - sequence * per;
     int before = 0, total = 0;
@@ -522,31 +571,47 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
     if (a == z) return;
     const float *stats = p.partial + (int64_t)blocks * 2 * ROWS * DIM;
     const int head = segment / p.row_groups, row_group = segment - head * p.row_groups, rows = p.tokens * p.group;
-    for (int i = threadIdx.x; i < ROWS * DIM / 4; i += 128) {
-        const int n = i / (DIM / 4), e = i % (DIM / 4) * 4, own = row_group * ROWS + n;
-        if (own >= rows) continue;
-        float high = -INFINITY, all = 0.0f;
-        float4 v = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-        for (int64_t block = a; block <= z; ++block) {
-            const int64_t t = run_start(tiles, block, blocks);
-            if (t == run_start(tiles, block + 1, blocks)) continue;       /* an empty run */
-            const int64_t slot = block * 2 + (t < start);
-            const float top = stats[(slot * ROWS + n) * 2], sum = stats[(slot * ROWS + n) * 2 + 1];
-            const float4 x = *(const float4 *)(p.partial + (slot * ROWS + n) * DIM + e);
-            const float next = fmaxf(high, top), ref = next == -INFINITY ? 0.0f : next;
-            const float f = exp2_approx(high - ref), g = exp2_approx(top - ref);
-            all = fmaf(g, sum, all * f);
-            v.x = fmaf(g, x.x, v.x * f), v.y = fmaf(g, x.y, v.y * f);
-            v.z = fmaf(g, x.z, v.z * f), v.w = fmaf(g, x.w, v.w * f);
-            high = next;
-        }
-        const float inv = all > 0.0f || all != all ? 1.0f / all : 0.0f;
-        const int token = own / p.group;
-        T *out = (T *)p.out + sequence * p.out_batch + token * p.out_token +
-                 (int64_t)(head * p.group + own - token * p.group) * p.out_head + e;
-        out[0] = from_f32<T>(v.x * inv), out[1] = from_f32<T>(v.y * inv);
-        out[2] = from_f32<T>(v.z * inv), out[3] = from_f32<T>(v.w * inv);
+    /* a row of the segment to each block of the grid's second dimension: its warps take every fourth run */
+    const int n = blockIdx.y, own = row_group * ROWS + n, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    if (own >= rows) return;
+    constexpr int PER = DIM / 32;
+    float high = -INFINITY, all = 0.0f, v[PER];
+#pragma unroll
+    for (int j = 0; j < PER; ++j) v[j] = 0.0f;
+#pragma unroll 4
+    for (int64_t block = a + warp; block <= z; block += 4) {
+        const int64_t t = run_start(tiles, block, blocks);
+        const bool empty = t == run_start(tiles, block + 1, blocks);
+        const int64_t slot = block * 2 + (t < start);
+        const float2 stat = *(const float2 *)(stats + (slot * ROWS + n) * 2);
+        const Pack<float, PER> x = *(const Pack<float, PER> *)(p.partial + (slot * ROWS + n) * DIM + lane * PER);
+        const float top = empty ? -INFINITY : stat.x, next = fmaxf(high, top), ref = next == -INFINITY ? 0.0f : next;
+        const float f = exp2_approx(high - ref), g = exp2_approx(top - ref);
+        all = fmaf(g, empty ? 0.0f : stat.y, all * f);
+#pragma unroll
+        for (int j = 0; j < PER; ++j) v[j] = fmaf(g, empty ? 0.0f : x.at[j], v[j] * f);
+        high = next;
     }
+    if (lane == 0) tops[warp] = high, totals[warp] = all;
+#pragma unroll
+    for (int j = 0; j < PER; ++j) parts[warp][lane * PER + j] = v[j];
+    __syncthreads();
+    float best = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) best = fmaxf(best, tops[w]);
+    const float ref = best == -INFINITY ? 0.0f : best;
+    float sum = 0.0f, out = 0.0f;
+    const int e = threadIdx.x;
+    if (e >= DIM) return;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float f = exp2_approx(tops[w] - ref);
+        sum = fmaf(f, totals[w], sum);
+        out = fmaf(f, parts[w][e], out);
+    }
+    const int token = own / p.group;
+    ((T *)p.out)[sequence * p.out_batch + token * p.out_token + (int64_t)(head * p.group + own - token * p.group) * p.out_head + e] =
+        from_f32<T>(sum > 0.0f || sum != sum ? out / sum : 0.0f);
 }
 
 int sm_count(int device, int *out) {
@@ -562,20 +627,26 @@ int sm_count(int device, int *out) {
     return 0;
 }
 
-template <typename T, int DIM, int NT> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
+template <typename T, int DIM, int NT, bool PAGE32> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
     const size_t smem = sizeof(Shared<DIM, NT>) + 4 * ((size_t)p.batch + 1);
     static uint64_t allowed;                 /* devices whose limit is raised */
     if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
-        cudaError_t e = cudaFuncSetAttribute(cache4_attend<T, DIM, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(cache4_attend<T, DIM, NT, PAGE32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)(sizeof(Shared<DIM, NT>) + 4 * (MAX_BATCH + 1)));
         if (e != cudaSuccess) return ops_cuda(e, "shared memory of the attention");
         __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
     }
     const int blocks = sms * BLOCKS_PER_SM<NT>;
-    cudaError_t e = launch(cache4_attend<T, DIM, NT>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
+    cudaError_t e = launch(cache4_attend<T, DIM, NT, PAGE32>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
     if (e != cudaSuccess) return ops_cuda(e, "attention over the 4-bit cache");
-    e = launch(cache4_join<T, DIM, NT>, dim3((unsigned)(p.batch * p.heads * p.row_groups)), dim3(128), 0, stream, p, blocks);
+    e = launch(cache4_join<T, DIM, NT>, dim3((unsigned)(p.batch * p.heads * p.row_groups), 8 * NT), dim3(128), 0, stream, p, blocks);
     return ops_cuda(e, "joining the attention's parts");
+}
+
+template <typename T, int DIM> int by_shape(const AttendParams &p, int nt, int sms, int device, uint64_t stream) {
+    if (p.page % WARP_TOKENS == 0)
+        return nt == 1 ? go<T, DIM, 1, true>(p, sms, device, stream) : go<T, DIM, 2, true>(p, sms, device, stream);
+    return nt == 1 ? go<T, DIM, 1, false>(p, sms, device, stream) : go<T, DIM, 2, false>(p, sms, device, stream);
 }
 
 uint64_t workspace(int sms, int dim) {
@@ -634,10 +705,7 @@ EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int
     DeviceScope scope(device);
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
     const bool f16 = a->dtype == EMMY_OPS_F16;
-    if (a->cache.dim == 64) {
-        if (nt == 1) return f16 ? go<__half, 64, 1>(p, sms, device, stream) : go<__nv_bfloat16, 64, 1>(p, sms, device, stream);
-        return f16 ? go<__half, 64, 2>(p, sms, device, stream) : go<__nv_bfloat16, 64, 2>(p, sms, device, stream);
-    }
-    if (nt == 1) return f16 ? go<__half, 128, 1>(p, sms, device, stream) : go<__nv_bfloat16, 128, 1>(p, sms, device, stream);
-    return f16 ? go<__half, 128, 2>(p, sms, device, stream) : go<__nv_bfloat16, 128, 2>(p, sms, device, stream);
+    if (a->cache.dim == 64)
+        return f16 ? by_shape<__half, 64>(p, nt, sms, device, stream) : by_shape<__nv_bfloat16, 64>(p, nt, sms, device, stream);
+    return f16 ? by_shape<__half, 128>(p, nt, sms, device, stream) : by_shape<__nv_bfloat16, 128>(p, nt, sms, device, stream);
 }

@@ -1,7 +1,8 @@
 """Attention over the 4-bit cache on the B200 against its definition in f64, and the decoder layer's operators in a row.
 
 Tolerances, for one output element with probabilities p, steps s, levels n and least values z of the values:
-half a step of the type; the rounding of p s to f16, 2^-11 of sum p s n, and of everything else 16 of 2^-24 of
+half a step of the type; the rounding of p s to f16, 2^-11 of sum p s n (where the result is f16, sum p and sum p z are taken
+of the rounded p: 2^-11 of sum p |v - out|), and of everything else 16 of 2^-24 of
 sum p (s n + |z|); and the logits: their f32 sums lose at most 2^-23 at each of the 8 products of 16 and in the
 scaling, 16 of 2^-23 of scale (s_k sum |q| n_k + |z_k| sum |q|), which moves every p by that much relative (twice: it is in
 the denominator too).
@@ -64,7 +65,12 @@ def reference(a, q, table, lengths, page, scale):
                             x.abs().sum(-1, keepdim=True) * zk.abs()[sees][..., 0].t()[:, None])
             moved = p * (2 * 16 * 2.0 ** -23) * size
             big = (nv * sv)[sees]
-            bound[b, t] = (torch.einsum("hgn,nhd->hgd", p, big) * 2.0 ** -11 +
+            if q.dtype == torch.float16:
+                away = (v[:, :, None] - out[b, t].view(1, heads, -1, dim)).abs()
+                rounding = torch.einsum("hgn,nhgd->hgd", p, away)
+            else:
+                rounding = torch.einsum("hgn,nhd->hgd", p, big)
+            bound[b, t] = (rounding * 2.0 ** -11 +
                            torch.einsum("hgn,nhd->hgd", moved + p * 16 * 2.0 ** -24, big + zv.abs()[sees]) +
                            moved.sum(-1, keepdim=True) * torch.einsum("hgn,nhd->hgd", p, big + zv.abs()[sees])).reshape(q_heads, dim)
     return out, bound
