@@ -25,7 +25,7 @@
  * chosen so that each thread's share of a token is consecutive bytes.
  *
  * Work is a list of tiles of 128 tokens over all (sequence, head, group of rows), cut into
- * equal runs, one for each block, whatever the lengths are.  A block's four warps take 32
+ * equal runs, one for each block, whatever the lengths are.  A block's two warps take 64
  * tokens of each tile with their own running maxima and sums and their own ring of
  * asynchronous copies, and join at the end of a sequence; a sequence that runs over several
  * blocks leaves 32-bit partial sums in the workspace, which a second kernel joins in order.
@@ -36,9 +36,9 @@ int ops_check_cache4(const emmy_ops_cache4 &c);
 
 namespace {
 
-constexpr int WARPS = 4, WARP_TOKENS = 32, TILE = WARPS * WARP_TOKENS, STAGES = 3;
+constexpr int WARPS = 2, WARP_TOKENS = 64, TILE = WARPS * WARP_TOKENS, STAGES = 2, MT = WARP_TOKENS / 16;
 /* what registers and shared memory let an SM hold of 8-row and of 16-row blocks */
-template <int NT> constexpr int BLOCKS_PER_SM = NT == 1 ? 3 : 2;
+template <int NT> constexpr int BLOCKS_PER_SM = NT == 1 ? 6 : 4;
 constexpr int MAX_BATCH = 4096;
 
 struct AttendParams {
@@ -50,18 +50,13 @@ struct AttendParams {
     float *partial;                     /* [blocks][2][rows][dim], then [blocks][2][rows][2] (max, sum) */
     int64_t pages, q_batch, q_token, q_head, out_batch, out_token, out_head, table_stride;
     int batch, tokens, heads, group, row_groups, page, max_positions;
+    uint32_t page_inverse, page_shift;  /* position / page without a division */
     float scale_log2;
 };
 
 /* where tile `t` of the list lies */
 struct Place {
     int sequence, head, row_group, tile, tiles, length;
-};
-
-/* the list of tiles: sequence b's part starts at before[b] * heads * row_groups */
-struct List {
-    int total;                          /* tiles of one (head, row group) over all sequences */
-    int64_t tiles;                      /* of all */
 };
 
 __device__ __forceinline__ int sequence_length(const AttendParams &p, int b) {
@@ -98,23 +93,30 @@ __device__ __forceinline__ int sum_tiles(const AttendParams &p, int32_t *before,
     return carry;
 }
 
-__device__ __forceinline__ int64_t run_start(int64_t tiles, int64_t block, int64_t blocks) { return tiles * block / blocks; }
-/* the last block whose run starts at or before tile t */
-__device__ __forceinline__ int64_t run_of(int64_t tiles, int64_t t, int64_t blocks) { return ((t + 1) * blocks - 1) / tiles; }
+/* The list's tiles in equal runs: block i's starts at i * each + min(i, more). */
+struct Runs {
+    int each, more;
+    __device__ Runs(int tiles, int blocks) : each(tiles / blocks), more(tiles - tiles / blocks * blocks) {}
+    __device__ int start(int block) const { return block * each + min(block, more); }
+    /* the block that has tile t */
+    __device__ int of(int t) const {
+        const int edge = more * (each + 1);
+        return t < edge ? t / (each + 1) : more + (t - edge) / max(each, 1);
+    }
+};
 
-__device__ __forceinline__ Place find(const AttendParams &p, const int32_t *before, int64_t t) {
+__device__ __forceinline__ Place find(const AttendParams &p, const int32_t *before, int t) {
     const int per = p.heads * p.row_groups;
     int lo = 0, hi = p.batch - 1;
     while (lo < hi) {                   /* the last sequence that starts at or before t */
         const int mid = (lo + hi + 1) / 2;
-        if ((int64_t)before[mid] * per <= t) lo = mid; else hi = mid - 1;
+        if (before[mid] * per <= t) lo = mid; else hi = mid - 1;
     }
     Place at;
     at.sequence = lo;
     at.tiles = before[lo + 1] - before[lo];
-    const int64_t r = t - (int64_t)before[lo] * per;
-    const int segment = (int)(r / at.tiles);
-    at.tile = (int)(r - (int64_t)segment * at.tiles);
+    const int r = t - before[lo] * per, segment = r / at.tiles;
+    at.tile = r - segment * at.tiles;
     at.head = segment / p.row_groups;
     at.row_group = segment - at.head * p.row_groups;
     at.length = sequence_length(p, lo);
@@ -171,22 +173,22 @@ template <int DIM> __device__ __forceinline__ int swizzled(int token, int byte) 
 template <int DIM> struct alignas(16) Stage {
     unsigned char k[WARP_TOKENS * DIM / 2], v[WARP_TOKENS * DIM / 2];
     __half2 k_meta[WARP_TOKENS], v_meta[WARP_TOKENS];
-    uint32_t held;                      /* bit t: token t is in the sequence, on a page of the cache */
+    uint64_t held;                      /* bit t: token t is in the sequence, on a page of the cache */
 };
 
 template <int DIM, int NT> struct Shared {
-    Stage<DIM> ring[WARPS][STAGES];
-    float out[WARPS][8 * NT][DIM + 4];
+    Stage<DIM> ring[WARPS][STAGES];     /* a warp's partial results lie in the stage that it used last */
     float top[WARPS][8 * NT], sum[WARPS][8 * NT];
     int warp_sums[WARPS];
     int32_t before[];
 };
 
-template <typename T, int DIM, int NT, bool PAGE32>
+template <typename T, int DIM, int NT, bool WHOLE>
 __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(AttendParams p) {
     extern __shared__ __align__(16) unsigned char raw[];
     Shared<DIM, NT> &sh = *(Shared<DIM, NT> *)raw;
-    constexpr int ROWS = 8 * NT, WORDS = DIM / 32, ROW_BYTES = DIM / 2, OT = DIM / 16;
+    constexpr int ROWS = 8 * NT, WORDS = DIM / 32, ROW_BYTES = DIM / 2, OT = DIM / 16, OUT_ROW = DIM + 4;
+    static_assert(ROWS * OUT_ROW * 4 <= (int)sizeof(Stage<DIM>), "a stage holds a warp's results");
     /* p s_v goes to f16, off by up to 2^-12 of itself.  Beside an f16 result that shows (3.2e-4 of the result's norm against
      * 2.1e-4 from its own rounding), so there sum p and sum p z take the p that the rounded product stands for: what
      * is left is 2^-12 of the values' distance from their mean.  A bf16 result's rounding hides it. */
@@ -194,64 +196,74 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     enter_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int total = sum_tiles(p, sh.before, sh.warp_sums);
-    const int64_t tiles = (int64_t)total * p.heads * p.row_groups;
-    const int64_t first = run_start(tiles, blockIdx.x, gridDim.x), last = run_start(tiles, blockIdx.x + 1, gridDim.x);
+    const Runs runs(total * p.heads * p.row_groups, gridDim.x);
+    const int first = runs.start(blockIdx.x), last = runs.start(blockIdx.x + 1);
     if (first >= last) return;
     Place ahead = find(p, sh.before, first), at = ahead;
-    int64_t issued = first;
+    int issued = first;
 
-    /* The copies' side.  `row`: this lane's token in the cache (rows of pages x heads x page), -1 for none.  With pages of
-     * a multiple of 32 rows a warp's tokens are consecutive rows of one page, so `row` is the first one's, the
-     * same for all lanes, and the copies take the page's rows behind a sequence's end along. */
-    auto lookup = [&](const Place &place) -> int64_t {
-        const int position = place.tile * TILE + warp * WARP_TOKENS + (PAGE32 ? 0 : lane);
+    /* The copies' side.  rows: where this lane's tokens (lane and lane + 32) lie in the cache (rows of pages x heads x
+     * page), -1 for nowhere.  WHOLE: pages are a multiple of a warp's tokens, which then are consecutive rows of
+     * one page: rows[0] is the first one's, the same for all lanes, and rows behind a sequence's end come along. */
+    auto lookup = [&](const Place &place, int i) -> int64_t {
+        const int position = place.tile * TILE + warp * WARP_TOKENS + (WHOLE ? 0 : lane + 32 * i);
         if (position >= place.length) return -1;
-        const int page = position / p.page;
+        const int page = p.page_inverse ? __umulhi(position, p.page_inverse) >> p.page_shift : position;
         const int64_t index = p.table[place.sequence * p.table_stride + page];
         if (index < 0 || index >= p.pages) return -1;
         return (index * p.heads + place.head) * p.page + (position - page * p.page);
     };
-    int64_t row = lookup(ahead);
+    int64_t rows[2];
+    auto look = [&] {
+        rows[0] = lookup(ahead, 0);
+        if (!WHOLE) rows[1] = lookup(ahead, 1);
+    };
+    look();
     auto issue = [&](int stage) {
         if (issued < last) {
             Stage<DIM> &s = sh.ring[warp][stage];
-            constexpr int CHUNKS = ROW_BYTES / 16, PER = 32 / CHUNKS;
+            constexpr int CHUNKS = ROW_BYTES / 16, PER = 32 / CHUNKS;     /* an access of the warp: PER tokens */
             const uint32_t k_to = (uint32_t)__cvta_generic_to_shared(s.k), v_to = (uint32_t)__cvta_generic_to_shared(s.v);
-            const uint32_t meta_to = (uint32_t)__cvta_generic_to_shared(&s.k_meta[lane]);
-            uint32_t held;
-            if (PAGE32) {
+            const uint32_t k_meta_to = (uint32_t)__cvta_generic_to_shared(&s.k_meta[lane]);
+            const uint32_t v_meta_to = (uint32_t)__cvta_generic_to_shared(&s.v_meta[lane]);
+            uint64_t held;
+            if (WHOLE) {
                 const int left = ahead.length - ahead.tile * TILE - warp * WARP_TOKENS;
-                held = row < 0 ? 0 : left >= 32 ? ~0u : (1u << left) - 1;
-                if (row >= 0) {
-                    const int64_t offset = row * ROW_BYTES + lane * 16;
+                held = rows[0] < 0 ? 0 : left >= 64 ? ~0ull : (1ull << left) - 1;
+                if (rows[0] >= 0) {
+                    const int64_t offset = rows[0] * ROW_BYTES + lane * 16;
                     const char *k = p.k + offset, *v = p.v + offset;
                     const uint32_t to = lane / CHUNKS * ROW_BYTES + swizzled<DIM>(lane / CHUNKS, lane % CHUNKS * 16);
 #pragma unroll
-                    for (int i = 0; i < CHUNKS; ++i) {
+                    for (int i = 0; i < WARP_TOKENS / PER; ++i) {
                         copy16(k_to + to + i * 512, k + i * 512, true);
                         copy16(v_to + to + i * 512, v + i * 512, true);
                     }
-                    copy4(meta_to, p.k_meta + row + lane, true);
-                    copy4(meta_to + sizeof s.k_meta, p.v_meta + row + lane, true);
+                    const __half2 *k_meta = p.k_meta + rows[0] + lane, *v_meta = p.v_meta + rows[0] + lane;
+                    copy4(k_meta_to, k_meta, true), copy4(k_meta_to + 128, k_meta + 32, true);
+                    copy4(v_meta_to, v_meta, true), copy4(v_meta_to + 128, v_meta + 32, true);
                 }
             } else {
 #pragma unroll
-                for (int i = 0; i < CHUNKS; ++i) {
+                for (int i = 0; i < WARP_TOKENS / PER; ++i) {
                     const int token = i * PER + lane / CHUNKS, byte = lane % CHUNKS * 16;
-                    const int64_t from = __shfl_sync(~0u, row, token);
+                    const int64_t from = __shfl_sync(~0u, rows[i * PER / 32], token & 31);
                     const uint32_t to = token * ROW_BYTES + swizzled<DIM>(token, byte);
                     const int64_t offset = (from < 0 ? 0 : from) * ROW_BYTES + byte;
                     copy16(k_to + to, p.k + offset, from >= 0);
                     copy16(v_to + to, p.v + offset, from >= 0);
                 }
-                held = __ballot_sync(~0u, row >= 0);
-                copy4(meta_to, p.k_meta + (row < 0 ? 0 : row), row >= 0);
-                copy4(meta_to + sizeof s.k_meta, p.v_meta + (row < 0 ? 0 : row), row >= 0);
+                held = __ballot_sync(~0u, rows[0] >= 0) | (uint64_t)__ballot_sync(~0u, rows[1] >= 0) << 32;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    copy4(k_meta_to + 128 * i, p.k_meta + (rows[i] < 0 ? 0 : rows[i]), rows[i] >= 0);
+                    copy4(v_meta_to + 128 * i, p.v_meta + (rows[i] < 0 ? 0 : rows[i]), rows[i] >= 0);
+                }
             }
             if (lane == 0) s.held = held;
             if (++issued < last) {
                 advance(p, sh.before, ahead);
-                row = lookup(ahead);
+                look();
             }
         }
         asm volatile("cp.async.commit_group;" ::: "memory");
@@ -262,9 +274,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     float o[NT][OT][4], least[NT][2], top[NT][2], sum[NT][2], by[NT][2], base[NT][2];
     int sees[NT][2];
     int v_exponent = 0, all_see = 0;
-    int64_t segment_start = first;
-    int stage = 0;
-    for (int64_t t = first; t < last; ++t) {
+    int segment_start = first, stage = 0;
+    for (int t = first; t < last; ++t) {
         if (t == first || at.tile == 0) {
             /* a new (sequence, head, group of rows): its queries */
             segment_start = t;
@@ -323,9 +334,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         __syncwarp();
         const Stage<DIM> &s = sh.ring[warp][stage];
         /* S^T = K Q^T */
-        float score[2][NT][4];
+        float score[MT][NT][4];
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < MT; ++m) {
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -348,16 +359,16 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         }
         /* logits to base 2, and the running maximum */
         const int from = at.tile * TILE + warp * WARP_TOKENS;
-        const uint32_t held = s.held;
-        const bool full = held == ~0u && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
+        const uint64_t held = s.held;
+        const bool full = held == ~0ull && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
         bool moved = false;
-        float next[NT][2], shrink[NT][2], v_step[2][2], v_least[2][2];
+        float next[NT][2], shrink[NT][2], v_step[MT][2], v_least[MT][2];
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
             for (int i = 0; i < 2; ++i) next[n][i] = top[n][i];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const int token = 16 * m + 8 * h + token_of<DIM>(r);
@@ -397,7 +408,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 top[n][i] = next[n][i];
             }
         /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
-        const uint32_t step_bits = held >> lane & 1 ? __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff : 0;
+        const uint32_t step_bits = max(held >> lane & 1 ? __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff : 0,
+                                       held >> (lane + 32) & 1 ? __half_as_ushort(__low2half(s.v_meta[lane + 32])) & 0x7fff : 0);
         const int exponent = (int)(__reduce_max_sync(~0u, step_bits) >> 10) - 15;
         float rescale = 1.0f;
         if (exponent > v_exponent) {
@@ -420,9 +432,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     o[n][i][0] *= f0, o[n][i][1] *= f1, o[n][i][2] *= f0, o[n][i][3] *= f1;
             }
         }
-        uint32_t pf[2][NT][2];
+        uint32_t pf[MT][NT][2];
 #pragma unroll
-        for (int m = 0; m < 2; ++m)
+        for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const float step = v_step[m][h] * up, inverse = EXACT ? 1.0f / step : 0.0f;
@@ -450,7 +462,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
             }
         /* O^T += V^T P^T */
 #pragma unroll
-        for (int m = 0; m < 2; ++m) {
+        for (int m = 0; m < MT; ++m) {
             Pack<uint32_t, WORDS / 2> x[4];
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -475,7 +487,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 }
         }
         __syncwarp();                   /* all lanes are done with the stage before it is filled again */
-        stage = (stage + 1) % STAGES;
 
         if (at.tile + 1 == at.tiles || t + 1 == last) {
             /* the four warps' sums joined */
@@ -494,7 +505,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                         sh.sum[warp][8 * n + 2 * c + i] = sum[n][i];
                     }
                     /* this thread's dims: 2 OT from 2 OT r on, of row 2 c + i */
-                    float *to = &sh.out[warp][8 * n + 2 * c + i][2 * OT * r];
+                    float *to = (float *)&sh.ring[warp][stage] + (8 * n + 2 * c + i) * OUT_ROW + 2 * OT * r;
 #pragma unroll
                     for (int j = 0; j < OT; ++j) {
                         to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, least[n][i]);
@@ -516,7 +527,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
                 for (int w = 0; w < WARPS; ++w) {
                     const float f = exp2_approx(sh.top[w][n] - ref);
-                    const float4 x = *(const float4 *)&sh.out[w][n][e];
+                    const float4 x = *(const float4 *)((const float *)&sh.ring[w][stage] + n * OUT_ROW + e);
                     all = fmaf(f, sh.sum[w][n], all);
                     v.x = fmaf(f, x.x, v.x), v.y = fmaf(f, x.y, v.y), v.z = fmaf(f, x.z, v.z), v.w = fmaf(f, x.w, v.w);
                 }
@@ -539,6 +550,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
             }
             __syncthreads();
         }
+        stage = (stage + 1) % STAGES;
         if (t + 1 < last) advance(p, sh.before, at);
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
@@ -564,10 +576,10 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
     __syncthreads();
     before = sums[0][0] + sums[0][1] + sums[0][2] + sums[0][3];
     total = sums[1][0] + sums[1][1] + sums[1][2] + sums[1][3];
-    const int64_t tiles = (int64_t)total * per;
+    const Runs runs(total * per, blocks);
     const int own_tiles = sequence_tiles(sequence_length(p, sequence));
-    const int64_t start = (int64_t)before * per + (int64_t)segment * own_tiles;
-    const int64_t a = run_of(tiles, start, blocks), z = run_of(tiles, start + own_tiles - 1, blocks);
+    const int start = before * per + segment * own_tiles;
+    const int a = runs.of(start), z = runs.of(start + own_tiles - 1);
     if (a == z) return;
     const float *stats = p.partial + (int64_t)blocks * 2 * ROWS * DIM;
     const int head = segment / p.row_groups, row_group = segment - head * p.row_groups, rows = p.tokens * p.group;
@@ -579,17 +591,15 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
 #pragma unroll
     for (int j = 0; j < PER; ++j) v[j] = 0.0f;
 #pragma unroll 4
-    for (int64_t block = a + warp; block <= z; block += 4) {
-        const int64_t t = run_start(tiles, block, blocks);
-        const bool empty = t == run_start(tiles, block + 1, blocks);
-        const int64_t slot = block * 2 + (t < start);
+    for (int block = a + warp; block <= z; block += 4) {
+        const int64_t slot = block * 2 + (runs.start(block) < start);
         const float2 stat = *(const float2 *)(stats + (slot * ROWS + n) * 2);
         const Pack<float, PER> x = *(const Pack<float, PER> *)(p.partial + (slot * ROWS + n) * DIM + lane * PER);
-        const float top = empty ? -INFINITY : stat.x, next = fmaxf(high, top), ref = next == -INFINITY ? 0.0f : next;
+        const float top = stat.x, next = fmaxf(high, top), ref = next == -INFINITY ? 0.0f : next;
         const float f = exp2_approx(high - ref), g = exp2_approx(top - ref);
-        all = fmaf(g, empty ? 0.0f : stat.y, all * f);
+        all = fmaf(g, stat.y, all * f);
 #pragma unroll
-        for (int j = 0; j < PER; ++j) v[j] = fmaf(g, empty ? 0.0f : x.at[j], v[j] * f);
+        for (int j = 0; j < PER; ++j) v[j] = fmaf(g, x.at[j], v[j] * f);
         high = next;
     }
     if (lane == 0) tops[warp] = high, totals[warp] = all;
@@ -627,17 +637,17 @@ int sm_count(int device, int *out) {
     return 0;
 }
 
-template <typename T, int DIM, int NT, bool PAGE32> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
+template <typename T, int DIM, int NT, bool WHOLE> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
     const size_t smem = sizeof(Shared<DIM, NT>) + 4 * ((size_t)p.batch + 1);
     static uint64_t allowed;                 /* devices whose limit is raised */
     if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
-        cudaError_t e = cudaFuncSetAttribute(cache4_attend<T, DIM, NT, PAGE32>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+        cudaError_t e = cudaFuncSetAttribute(cache4_attend<T, DIM, NT, WHOLE>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                              (int)(sizeof(Shared<DIM, NT>) + 4 * (MAX_BATCH + 1)));
         if (e != cudaSuccess) return ops_cuda(e, "shared memory of the attention");
         __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
     }
     const int blocks = sms * BLOCKS_PER_SM<NT>;
-    cudaError_t e = launch(cache4_attend<T, DIM, NT, PAGE32>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
+    cudaError_t e = launch(cache4_attend<T, DIM, NT, WHOLE>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
     if (e != cudaSuccess) return ops_cuda(e, "attention over the 4-bit cache");
     e = launch(cache4_join<T, DIM, NT>, dim3((unsigned)(p.batch * p.heads * p.row_groups), 8 * NT), dim3(128), 0, stream, p, blocks);
     return ops_cuda(e, "joining the attention's parts");
@@ -695,9 +705,14 @@ EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int
     p.row_groups = (rows + 8 * nt - 1) / (8 * nt), p.page = a->cache.page;
     p.max_positions = a->max_pages * a->cache.page;
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
-    if ((int64_t)p.batch * p.heads * p.row_groups > 0x7fffffffLL ||
-        (int64_t)p.batch * ((int64_t)p.max_positions / TILE + 1) > 0x7fffffffLL)
+    if ((int64_t)p.batch * p.heads * p.row_groups > 0x7fffffffLL / ((int64_t)p.max_positions / TILE + 1))
         return ops_fail(EMMY_RT_EINVAL, "%d sequences of %d positions are too many for one call", p.batch, p.max_positions);
+    if (p.page > 1) {                   /* ceil(2^(31 + s) / page), 2^s >= page: exact below 2^31 */
+        uint32_t shift = 1;
+        while ((1u << shift) < (uint32_t)p.page) ++shift;
+        p.page_inverse = (uint32_t)((((uint64_t)1 << (31 + shift)) + p.page - 1) / p.page);
+        p.page_shift = shift - 1;
+    }
     int sms;
     if (int e = sm_count(device, &sms)) return e;
     if (a->workspace_bytes < workspace(sms, a->cache.dim))
