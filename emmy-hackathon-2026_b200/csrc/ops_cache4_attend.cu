@@ -160,6 +160,33 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+/* pairs of f32 that one instruction works on: a row of the scores has two neighbours in a thread */
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+
 /* The token that row r (0 .. 7) of an eight-token group stands for.  A warp reads a token's keys by
  * r = lane / 4 and its values by the pairs r = 2 (lane % 4) + {0, 1}; these orders (with the
  * swizzle below at dim 128) put both into different banks. */
@@ -271,7 +298,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     for (int s = 0; s < STAGES - 1; ++s) issue(s);
 
     uint32_t qf[NT][2 * WORDS][2];
-    float o[NT][OT][4], least[NT][2], top[NT][2], sum[NT][2], by[NT][2], base[NT][2];
+    float o[NT][OT][4], top[NT][2];
+    Two least[NT], sum[NT], by[NT], base[NT];
     int sees[NT][2];
     int v_exponent = 0, all_see = 0;
     int segment_start = first, stage = 0;
@@ -302,6 +330,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     largest = fmaxf(largest, __shfl_xor_sync(~0u, largest, d));
                     all += __shfl_xor_sync(~0u, all, d);
                 }
+                const float sign = p.scale_log2 < 0.0f ? -1.0f : 1.0f;
                 const int exponent = max((int)(__float_as_uint(largest) >> 23) - 127, -100);
                 const float up = __uint_as_float((uint32_t)(127 + 13 - min(exponent, 127)) << 23);
 #pragma unroll
@@ -309,19 +338,20 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
                         const int e = 8 * w + 2 * i;
-                        qf[n][2 * w + i][0] = packed(v[e] * up, v[e + 4] * up);
-                        qf[n][2 * w + i][1] = packed(v[e + 1] * up * 0x1p-4f, v[e + 5] * up * 0x1p-4f);
+                        const float low = sign * up, high = low * 0x1p-4f;
+                        qf[n][2 * w + i][0] = packed(v[e] * low, v[e + 4] * low);
+                        qf[n][2 * w + i][1] = packed(v[e + 1] * high, v[e + 5] * high);
                     }
                 /* of the rows that this thread has in the scores: 2 c and 2 c + 1 */
-                const float mine = p.scale_log2 / up, mine0 = p.scale_log2 * all;
+                const float mine = fmaxf(fabsf(p.scale_log2) / up, 0x1p-126f), mine0 = sign * up * all;
+                by[n] = Two(__shfl_sync(~0u, mine, 8 * c), __shfl_sync(~0u, mine, 8 * c + 4));
+                base[n] = Two(__shfl_sync(~0u, mine0, 8 * c), __shfl_sync(~0u, mine0, 8 * c + 4));
+                sum[n] = least[n] = Two(0.0f, 0.0f);
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
-                    by[n][i] = __shfl_sync(~0u, mine, 4 * (2 * c + i));
-                    base[n][i] = __shfl_sync(~0u, mine0, 4 * (2 * c + i));
                     const int row = at.row_group * ROWS + n * 8 + 2 * c + i;
                     sees[n][i] = row < rows ? at.length - p.tokens + row / p.group + 1 : 0;
                     top[n][i] = -INFINITY;
-                    sum[n][i] = least[n][i] = 0.0f;
                 }
 #pragma unroll
                 for (int i = 0; i < OT; ++i)
@@ -333,31 +363,34 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         __syncwarp();
         const Stage<DIM> &s = sh.ring[warp][stage];
-        /* S^T = K Q^T */
+        /* S^T = K Q^T, in two independent chains of products at a time */
         float score[MT][NT][4];
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
+        for (int m = 0; m < MT; m += 2) {
+            Pack<uint32_t, WORDS> x[2][2];
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
-                for (int j = 0; j < 4; ++j) score[m][n][j] = 0.0f;
-            const int t0 = 16 * m + token_of<DIM>(r), t1 = t0 + 8;
-            const Pack<uint32_t, WORDS> x0 =
-                *(const Pack<uint32_t, WORDS> *)(s.k + t0 * ROW_BYTES + swizzled<DIM>(t0, c * 4 * WORDS));
-            const Pack<uint32_t, WORDS> x1 =
-                *(const Pack<uint32_t, WORDS> *)(s.k + t1 * ROW_BYTES + swizzled<DIM>(t1, c * 4 * WORDS));
+                for (int h = 0; h < 2; ++h) {
+                    const int token = 16 * (m + j) + 8 * h + token_of<DIM>(r);
+                    x[j][h] = *(const Pack<uint32_t, WORDS> *)(s.k + token * ROW_BYTES + swizzled<DIM>(token, c * 4 * WORDS));
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) score[m + j][n][2 * h] = score[m + j][n][2 * h + 1] = 0.0f;
+                }
 #pragma unroll
             for (int w = 0; w < WORDS; ++w)
 #pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    const uint32_t a = x0.at[w] >> 8 * i, b = x1.at[w] >> 8 * i;
+                for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int n = 0; n < NT; ++n)
-                        mma(score[m][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0,
-                            qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
-                }
+                    for (int j = 0; j < 2; ++j) {
+                        const uint32_t a = x[j][0].at[w] >> 8 * i, b = x[j][1].at[w] >> 8 * i;
+#pragma unroll
+                        for (int n = 0; n < NT; ++n)
+                            mma(score[m + j][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0,
+                                qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+                    }
         }
-        /* logits to base 2, and the running maximum */
+        /* logits to base 2, all but the factor `by` of their row, and the running maximum */
         const int from = at.tile * TILE + warp * WARP_TOKENS;
         const uint64_t held = s.held;
         const bool full = held == ~0ull && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
@@ -376,12 +409,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 const float step = meta.x * 0x1p24f;
                 v_step[m][h] = v_meta.x, v_least[m][h] = v_meta.y;
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        float &x = score[m][n][2 * h + i];
-                        x = fmaf(step, x * by[n][i], meta.y * base[n][i]);
-                    }
+                for (int n = 0; n < NT; ++n) {
+                    float *x = &score[m][n][2 * h];
+                    const float2 y = fma2(Two(step, step), Two(x[0], x[1]), Two(meta.y, meta.y) * base[n]).get();
+                    x[0] = y.x, x[1] = y.y;
+                }
                 if (!full) {
                     const bool is_held = held >> token & 1;
                     if (!is_held) v_step[m][h] = v_least[m][h] = 0.0f;
@@ -396,17 +428,22 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
                     for (int i = 0; i < 2; ++i) next[n][i] = fmaxf(next[n][i], score[m][n][2 * h + i]);
             }
+        Two minus[NT];                  /* less the maximum, in the exponent */
 #pragma unroll
-        for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n) {
+            const float2 f = by[n].get();
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
 #pragma unroll
                 for (int d = 4; d < 32; d <<= 1) next[n][i] = fmaxf(next[n][i], __shfl_xor_sync(~0u, next[n][i], d));
                 const float ref = next[n][i] == -INFINITY ? 0.0f : next[n][i];
-                shrink[n][i] = exp2_approx(top[n][i] - ref);
+                shrink[n][i] = exp2_approx((top[n][i] - ref) * (i ? f.y : f.x));
                 moved |= next[n][i] != top[n][i];
                 top[n][i] = next[n][i];
+                next[n][i] = -ref * (i ? f.y : f.x);
             }
+            minus[n] = Two(next[n][0], next[n][1]);
+        }
         /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
         const uint32_t step_bits = max(held >> lane & 1 ? __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff : 0,
                                        held >> (lane + 32) & 1 ? __half_as_ushort(__low2half(s.v_meta[lane + 32])) & 0x7fff : 0);
@@ -421,11 +458,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         if (__any_sync(~0u, moved)) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    sum[n][i] *= shrink[n][i];
-                    least[n][i] *= shrink[n][i];
-                }
+                const Two f(shrink[n][0], shrink[n][1]);
+                sum[n] = sum[n] * f;
+                least[n] = least[n] * f;
                 const float f0 = shrink[n][0] * rescale, f1 = shrink[n][1] * rescale;
 #pragma unroll
                 for (int i = 0; i < OT; ++i)
@@ -440,24 +475,19 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 const float step = v_step[m][h] * up, inverse = EXACT ? 1.0f / step : 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
-                    float e[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const float ref = top[n][i] == -INFINITY ? 0.0f : top[n][i];
-                        e[i] = exp2_approx(score[m][n][2 * h + i] - ref);
-                    }
-                    const __half2 ps = __floats2half2_rn(e[0] * step, e[1] * step);
+                    const float2 x = fma2(by[n], Two(score[m][n][2 * h], score[m][n][2 * h + 1]), minus[n]).get();
+                    float e[2] = {exp2_approx(x.x), exp2_approx(x.y)};
+                    const float2 y = (Two(e[0], e[1]) * Two(step, step)).get();
+                    const __half2 ps = __floats2half2_rn(y.x, y.y);
                     pf[m][n][h] = transposed(*(const uint32_t *)&ps);
                     if (EXACT) {
                         const float2 rounded = __half22float2(ps);
                         if (rounded.x >= 0x1p-14f) e[0] = rounded.x * inverse;
                         if (rounded.y >= 0x1p-14f) e[1] = rounded.y * inverse;
                     }
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        sum[n][i] += e[i];
-                        least[n][i] = fmaf(e[i], v_least[m][h], least[n][i]);
-                    }
+                    const Two e2(e[0], e[1]);
+                    sum[n] = sum[n] + e2;
+                    least[n] = fma2(e2, Two(v_least[m][h], v_least[m][h]), least[n]);
                 }
             }
         /* O^T += V^T P^T */
@@ -492,26 +522,29 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
             /* the four warps' sums joined */
             const float down = __uint_as_float((uint32_t)(127 - 14 + v_exponent) << 23);
 #pragma unroll
-            for (int n = 0; n < NT; ++n)
+            for (int n = 0; n < NT; ++n) {
+                float2 s2 = sum[n].get(), l2 = least[n].get(), f2 = by[n].get();
 #pragma unroll
                 for (int i = 0; i < 2; ++i) {
+                    float all = i ? s2.y : s2.x, bottom = i ? l2.y : l2.x;
 #pragma unroll
                     for (int d = 4; d < 32; d <<= 1) {
-                        sum[n][i] += __shfl_xor_sync(~0u, sum[n][i], d);
-                        least[n][i] += __shfl_xor_sync(~0u, least[n][i], d);
+                        all += __shfl_xor_sync(~0u, all, d);
+                        bottom += __shfl_xor_sync(~0u, bottom, d);
                     }
                     if (r == 0) {
-                        sh.top[warp][8 * n + 2 * c + i] = top[n][i];
-                        sh.sum[warp][8 * n + 2 * c + i] = sum[n][i];
+                        sh.top[warp][8 * n + 2 * c + i] = top[n][i] == -INFINITY ? -INFINITY : top[n][i] * (i ? f2.y : f2.x);
+                        sh.sum[warp][8 * n + 2 * c + i] = all;
                     }
                     /* this thread's dims: 2 OT from 2 OT r on, of row 2 c + i */
                     float *to = (float *)&sh.ring[warp][stage] + (8 * n + 2 * c + i) * OUT_ROW + 2 * OT * r;
 #pragma unroll
                     for (int j = 0; j < OT; ++j) {
-                        to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, least[n][i]);
-                        to[2 * j + 1] = fmaf((o[n][j][2 + i] - o[n][j][i]) * 0x1p20f, down, least[n][i]);
+                        to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, bottom);
+                        to[2 * j + 1] = fmaf((o[n][j][2 + i] - o[n][j][i]) * 0x1p20f, down, bottom);
                     }
                 }
+            }
             __syncthreads();
             const bool whole = at.tile + 1 == at.tiles && t - segment_start + 1 == at.tiles;
             const int rows = p.tokens * p.group;

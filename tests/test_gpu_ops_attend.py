@@ -61,7 +61,7 @@ def reference(a, q, table, lengths, page, scale):
             logit = torch.einsum("hgd,nhd->hgn", x, k) * scale
             p = torch.softmax(logit, -1)
             out[b, t] = torch.einsum("hgn,nhd->hgd", p, v).reshape(q_heads, dim)
-            size = scale * (torch.einsum("hgd,nhd->hgn", x.abs(), (nk * sk)[sees]) +
+            size = abs(scale) * (torch.einsum("hgd,nhd->hgn", x.abs(), (nk * sk)[sees]) +
                             x.abs().sum(-1, keepdim=True) * zk.abs()[sees][..., 0].t()[:, None])
             moved = p * (2 * 16 * 2.0 ** -23) * size
             big = (nv * sv)[sees]
@@ -131,6 +131,8 @@ def test_extreme_sizes(runtime):
     check("bf16", 128, 1, 4, 1, 16, [500, 3], scale=30.0)
     check("f16", 128, 1, 4, 1, 16, [500, 3], v_span=2.0 ** -12)
     check("f16", 128, 1, 4, 1, 16, [500, 3], v_span=40000.0 / 2)
+    check("bf16", 128, 1, 4, 1, 16, [500, 3], scale=0.0)
+    check("bf16", 128, 1, 4, 1, 16, [500, 3], scale=-0.3)
     check("bf16", 64, 1, 4, 1, 16, [500, 3], q_size=2.0 ** 40, scale=2.0 ** -43)
     check("bf16", 64, 1, 4, 1, 16, [500, 3], q_size=2.0 ** -60, scale=2.0 ** 57)
 
