@@ -51,6 +51,7 @@ struct AttendParams {
     int64_t pages, q_batch, q_token, q_head, out_batch, out_token, out_head, table_stride;
     int batch, tokens, heads, group, row_groups, page, max_positions;
     uint32_t page_inverse, page_shift;  /* position / page without a division */
+    int q_wide, out_wide;               /* rows allow accesses of 16 and of 8 bytes */
     float scale_log2;
 };
 
@@ -142,12 +143,18 @@ __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool live) 
     asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(live ? 4 : 0) : "memory");
 }
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+/* d = a b */
+__device__ __forceinline__ void mma_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+                 : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+                 : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.0f));
+}
 __device__ __forceinline__ uint32_t transposed(uint32_t v) {
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %0;" : "+r"(v));
     return v;
 }
 __device__ __forceinline__ uint32_t packed(float low, float high) {
@@ -164,6 +171,7 @@ __device__ __forceinline__ float exp2_approx(float x) {
 struct Two {
     uint64_t v;
     __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ explicit Two(uint64_t both) : v(both) {}
     __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
     __device__ __forceinline__ float2 get() const {
         float2 f;
@@ -203,6 +211,12 @@ template <int DIM> struct alignas(16) Stage {
     uint64_t held;                      /* bit t: token t is in the sequence, on a page of the cache */
 };
 
+/* a token's (step, step, least, least) in f32, for instructions that work on pairs */
+struct Doubled {
+    ulonglong2 k, v;
+};
+static_assert(sizeof(Doubled) * WARP_TOKENS <= sizeof(Stage<64>::k), "they take the place of keys that have been read");
+
 template <int DIM, int NT> struct Shared {
     Stage<DIM> ring[WARPS][STAGES];     /* a warp's partial results lie in the stage that it used last */
     float top[WARPS][8 * NT], sum[WARPS][8 * NT];
@@ -220,7 +234,9 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
      * 2.1e-4 from its own rounding), so there sum p and sum p z take the p that the rounded product stands for: what
      * is left is 2^-12 of the values' distance from their mean.  A bf16 result's rounding hides it. */
     constexpr bool EXACT = sizeof(T) == 2 && !__is_same(T, __nv_bfloat16);
-    enter_grid();
+    /* the join may start only when what this kernel waits for is there: it reads the lengths before it waits */
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
     const int total = sum_tiles(p, sh.before, sh.warp_sums);
     const Runs runs(total * p.heads * p.row_groups, gridDim.x);
@@ -317,8 +333,17 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 if (own < rows) {
                     const T *q = (const T *)p.q + at.sequence * p.q_batch + token * p.q_token +
                                  (int64_t)(at.head * p.group + own - token * p.group) * p.q_head + c * 8 * WORDS;
+                    if (p.q_wide) {
 #pragma unroll
-                    for (int i = 0; i < 8 * WORDS; ++i) v[i] = to_f32(q[i]);
+                        for (int w = 0; w < WORDS; ++w) {
+                            const Pack<T, 8> x = *(const Pack<T, 8> *)(q + 8 * w);
+#pragma unroll
+                            for (int i = 0; i < 8; ++i) v[8 * w + i] = to_f32(x.at[i]);
+                        }
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 8 * WORDS; ++i) v[i] = to_f32(q[i]);
+                    }
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8 * WORDS; ++i) v[i] = 0.0f;
@@ -362,7 +387,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         issue((stage + STAGES - 1) % STAGES);
         asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
         __syncwarp();
-        const Stage<DIM> &s = sh.ring[warp][stage];
+        Stage<DIM> &s = sh.ring[warp][stage];
         /* S^T = K Q^T, in two independent chains of products at a time */
         float score[MT][NT][4];
 #pragma unroll
@@ -374,8 +399,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 for (int h = 0; h < 2; ++h) {
                     const int token = 16 * (m + j) + 8 * h + token_of<DIM>(r);
                     x[j][h] = *(const Pack<uint32_t, WORDS> *)(s.k + token * ROW_BYTES + swizzled<DIM>(token, c * 4 * WORDS));
-#pragma unroll
-                    for (int n = 0; n < NT; ++n) score[m + j][n][2 * h] = score[m + j][n][2 * h + 1] = 0.0f;
                 }
 #pragma unroll
             for (int w = 0; w < WORDS; ++w)
@@ -385,48 +408,79 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     for (int j = 0; j < 2; ++j) {
                         const uint32_t a = x[j][0].at[w] >> 8 * i, b = x[j][1].at[w] >> 8 * i;
 #pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma(score[m + j][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0,
-                                qf[n][2 * w + i][0], qf[n][2 * w + i][1]);
+                        for (int n = 0; n < NT; ++n) {
+                            const uint32_t *q = qf[n][2 * w + i];
+                            if (w + i == 0)
+                                mma_first(score[m + j][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0, q[0], q[1]);
+                            else
+                                mma(score[m + j][n], a & 0x000f000f, b & 0x000f000f, a & 0x00f000f0, b & 0x00f000f0, q[0], q[1]);
+                        }
                     }
+        }
+        /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
+        float rescale = 1.0f;
+        Doubled *const doubled = (Doubled *)s.k;
+        __syncwarp();                   /* all lanes are done with the keys */
+        {
+            const bool lives[2] = {(s.held >> lane & 1) != 0, (s.held >> (lane + 32) & 1) != 0};
+            const __half2 vm[2] = {s.v_meta[lane], s.v_meta[lane + 32]}, zero = __halves2half2(__half(), __half());
+            const __half2 of_v[2] = {lives[0] ? vm[0] : zero, lives[1] ? vm[1] : zero};
+            const uint32_t bits = max(__half_as_ushort(__low2half(of_v[0])) & 0x7fff, __half_as_ushort(__low2half(of_v[1])) & 0x7fff);
+            const int exponent = (int)(__reduce_max_sync(~0u, bits) >> 10) - 15;
+            if (exponent > v_exponent) {
+                rescale = v_exponent < -15 ? 1.0f : exp2_approx((float)(v_exponent - exponent));
+                v_exponent = exponent;
+            }
+            const float up = __uint_as_float((uint32_t)(127 + 14 - v_exponent) << 23);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float2 k = __half22float2(s.k_meta[lane + 32 * i]), v = __half22float2(of_v[i]);
+                const float k_step = k.x * 0x1p24f, v_step = v.x * up;
+                Doubled &to = doubled[lane + 32 * i];
+                to.k = make_ulonglong2(Two(k_step, k_step).v, Two(k.y, k.y).v);
+                to.v = make_ulonglong2(Two(v_step, v_step).v, Two(v.y, v.y).v);
+            }
+            __syncwarp();
         }
         /* logits to base 2, all but the factor `by` of their row, and the running maximum */
         const int from = at.tile * TILE + warp * WARP_TOKENS;
         const uint64_t held = s.held;
         const bool full = held == ~0ull && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
         bool moved = false;
-        float next[NT][2], shrink[NT][2], v_step[MT][2], v_least[MT][2];
-#pragma unroll
-        for (int n = 0; n < NT; ++n)
-#pragma unroll
-            for (int i = 0; i < 2; ++i) next[n][i] = top[n][i];
+        float next[NT][2], shrink[NT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const int token = 16 * m + 8 * h + token_of<DIM>(r);
-                const float2 meta = __half22float2(s.k_meta[token]), v_meta = __half22float2(s.v_meta[token]);
-                const float step = meta.x * 0x1p24f;
-                v_step[m][h] = v_meta.x, v_least[m][h] = v_meta.y;
+                const ulonglong2 k = doubled[16 * m + 8 * h + token_of<DIM>(r)].k;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     float *x = &score[m][n][2 * h];
-                    const float2 y = fma2(Two(step, step), Two(x[0], x[1]), Two(meta.y, meta.y) * base[n]).get();
+                    const float2 y = fma2(Two(k.x), Two(x[0], x[1]), Two(k.y) * base[n]).get();
                     x[0] = y.x, x[1] = y.y;
                 }
-                if (!full) {
-                    const bool is_held = held >> token & 1;
-                    if (!is_held) v_step[m][h] = v_least[m][h] = 0.0f;
+            }
+        if (!full) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int token = 16 * m + 8 * h + token_of<DIM>(r);
+                    const int place = held >> token & 1 ? from + token : 0x7fffffff;
 #pragma unroll
                     for (int n = 0; n < NT; ++n)
 #pragma unroll
                         for (int i = 0; i < 2; ++i)
-                            if (!is_held || from + token >= sees[n][i]) score[m][n][2 * h + i] = -INFINITY;
+                            if (place >= sees[n][i]) score[m][n][2 * h + i] = -INFINITY;
                 }
+        }
 #pragma unroll
-                for (int n = 0; n < NT; ++n)
+        for (int n = 0; n < NT; ++n)
 #pragma unroll
-                    for (int i = 0; i < 2; ++i) next[n][i] = fmaxf(next[n][i], score[m][n][2 * h + i]);
+            for (int i = 0; i < 2; ++i) {
+                next[n][i] = top[n][i];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) next[n][i] = fmaxf(next[n][i], fmaxf(score[m][n][i], score[m][n][2 + i]));
             }
         Two minus[NT];                  /* less the maximum, in the exponent */
 #pragma unroll
@@ -444,18 +498,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
             }
             minus[n] = Two(next[n][0], next[n][1]);
         }
-        /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
-        const uint32_t step_bits = max(held >> lane & 1 ? __half_as_ushort(__low2half(s.v_meta[lane])) & 0x7fff : 0,
-                                       held >> (lane + 32) & 1 ? __half_as_ushort(__low2half(s.v_meta[lane + 32])) & 0x7fff : 0);
-        const int exponent = (int)(__reduce_max_sync(~0u, step_bits) >> 10) - 15;
-        float rescale = 1.0f;
-        if (exponent > v_exponent) {
-            rescale = exp2_approx((float)(v_exponent - exponent));
-            v_exponent = exponent;
-            moved = true;
-        }
-        const float up = __uint_as_float((uint32_t)(127 + 14 - v_exponent) << 23);
-        if (__any_sync(~0u, moved)) {
+        if (__any_sync(~0u, moved) || rescale != 1.0f) {
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
                 const Two f(shrink[n][0], shrink[n][1]);
@@ -472,12 +515,13 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         for (int m = 0; m < MT; ++m)
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
-                const float step = v_step[m][h] * up, inverse = EXACT ? 1.0f / step : 0.0f;
+                const ulonglong2 v = doubled[16 * m + 8 * h + token_of<DIM>(r)].v;
+                const float inverse = EXACT ? 1.0f / Two(v.x).get().x : 0.0f;
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float2 x = fma2(by[n], Two(score[m][n][2 * h], score[m][n][2 * h + 1]), minus[n]).get();
                     float e[2] = {exp2_approx(x.x), exp2_approx(x.y)};
-                    const float2 y = (Two(e[0], e[1]) * Two(step, step)).get();
+                    const float2 y = (Two(e[0], e[1]) * Two(v.x)).get();
                     const __half2 ps = __floats2half2_rn(y.x, y.y);
                     pf[m][n][h] = transposed(*(const uint32_t *)&ps);
                     if (EXACT) {
@@ -487,7 +531,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     }
                     const Two e2(e[0], e[1]);
                     sum[n] = sum[n] + e2;
-                    least[n] = fma2(e2, Two(v_least[m][h], v_least[m][h]), least[n]);
+                    least[n] = fma2(e2, Two(v.y), least[n]);
                 }
             }
         /* O^T += V^T P^T */
@@ -570,8 +614,12 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                         const int token = own / p.group;
                         T *out = (T *)p.out + at.sequence * p.out_batch + token * p.out_token +
                                  (int64_t)(at.head * p.group + own - token * p.group) * p.out_head + e;
-                        out[0] = from_f32<T>(v.x * inv), out[1] = from_f32<T>(v.y * inv);
-                        out[2] = from_f32<T>(v.z * inv), out[3] = from_f32<T>(v.w * inv);
+                        const Pack<T, 4> y = {from_f32<T>(v.x * inv), from_f32<T>(v.y * inv), from_f32<T>(v.z * inv),
+                                              from_f32<T>(v.w * inv)};
+                        if (p.out_wide)
+                            *(Pack<T, 4> *)out = y;
+                        else
+                            out[0] = y.at[0], out[1] = y.at[1], out[2] = y.at[2], out[3] = y.at[3];
                     }
                 } else {
                     *(float4 *)(p.partial + (slot * ROWS + n) * DIM + e) = v;
@@ -595,7 +643,7 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
     constexpr int ROWS = 8 * NT;
     __shared__ int sums[2][4];
     __shared__ float tops[4], totals[4], parts[4][DIM];
-    enter_grid();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     const int per = p.heads * p.row_groups, sequence = blockIdx.x / per, segment = blockIdx.x - sequence * per;
     int before = 0, total = 0;
     for (int b = threadIdx.x; b < p.batch; b += 128) {
@@ -613,6 +661,7 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
     const int own_tiles = sequence_tiles(sequence_length(p, sequence));
     const int start = before * per + segment * own_tiles;
     const int a = runs.of(start), z = runs.of(start + own_tiles - 1);
+    asm volatile("griddepcontrol.wait;" ::: "memory");     /* the parts are written */
     if (a == z) return;
     const float *stats = p.partial + (int64_t)blocks * 2 * ROWS * DIM;
     const int head = segment / p.row_groups, row_group = segment - head * p.row_groups, rows = p.tokens * p.group;
@@ -679,7 +728,8 @@ template <typename T, int DIM, int NT, bool WHOLE> int go(const AttendParams &p,
         if (e != cudaSuccess) return ops_cuda(e, "shared memory of the attention");
         __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
     }
-    const int blocks = sms * BLOCKS_PER_SM<NT>;
+    /* as many blocks as run at once: the list of a long batch takes shared memory too */
+    const int fit = (int)((228 * 1024) / (smem + 1024)), blocks = sms * (fit < BLOCKS_PER_SM<NT> ? fit : BLOCKS_PER_SM<NT>);
     cudaError_t e = launch(cache4_attend<T, DIM, NT, WHOLE>, dim3(blocks), dim3(WARPS * 32), smem, stream, p);
     if (e != cudaSuccess) return ops_cuda(e, "attention over the 4-bit cache");
     e = launch(cache4_join<T, DIM, NT>, dim3((unsigned)(p.batch * p.heads * p.row_groups), 8 * NT), dim3(128), 0, stream, p, blocks);
@@ -734,6 +784,8 @@ EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int
     p.pages = a->cache.pages;
     p.q_batch = a->q_batch, p.q_token = a->q_token, p.q_head = a->q_head;
     p.out_batch = a->out_batch, p.out_token = a->out_token, p.out_head = a->out_head, p.table_stride = a->table_stride;
+    p.q_wide = aligned(a->q, 16) && !((p.q_batch | p.q_token | p.q_head) & 7);
+    p.out_wide = aligned(a->out, 8) && !((p.out_batch | p.out_token | p.out_head) & 3);
     p.batch = a->batch, p.tokens = a->tokens, p.heads = a->cache.heads, p.group = group;
     p.row_groups = (rows + 8 * nt - 1) / (8 * nt), p.page = a->cache.page;
     p.max_positions = a->max_pages * a->cache.page;
