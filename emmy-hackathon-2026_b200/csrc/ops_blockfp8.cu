@@ -1,0 +1,633 @@
+/*
+ * FP8 (e4m3) products with a scale for each block of 128.
+ *
+ *     y[m, n] = sum_b sx[b, m] sw[n / 128, b] sum_{k in block b} xq[m, k] wq[n, k]
+ *
+ * x is quantised per row and 128 columns, W per 128 x 128 block:
+ *     s = amax / 448 (1 where that is 0),  q = e4m3(v / s), nearest even.
+ *
+ * Three kernels: the two quantisers (bound by their bytes), a tensor-core product for many
+ * rows of x, and one for few rows, which is bound by the bytes of W.
+ */
+#include "ops_common.cuh"
+
+namespace {
+
+constexpr int BLOCK = 128;
+constexpr float E4M3_MAX = 448.0f;
+
+__device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
+    uint16_t low, high;
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(low) : "f"(b), "f"(a));
+    asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(high) : "f"(d), "f"(c));
+    return low | (uint32_t)high << 16;
+}
+
+/* |v| as an ordered integer: a NaN is the largest */
+__device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ float scale_of(uint32_t largest) {
+    const float s = __fdiv_rn(__uint_as_float(largest), E4M3_MAX);
+    return s == 0.0f ? 1.0f : s;
+}
+
+template <typename T> __device__ __forceinline__ void load8(const T *x, int64_t e, int64_t end, bool wide, float (&v)[8]) {
+    if (wide && e + 8 <= end) {
+        constexpr int V = 16 / sizeof(T);
+#pragma unroll
+        for (int i = 0; i < 8; i += V) {
+            const Pack<T, V> q = *(const Pack<T, V> *)(x + e + i);
+#pragma unroll
+            for (int j = 0; j < V; ++j) v[i + j] = to_f32(q.at[j]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = e + i < end ? to_f32(x[e + i]) : 0.0f;
+    }
+}
+
+/* ---- quantisers ---------------------------------------------------------------------- */
+
+struct QuantRowsParams {
+    const char *x;
+    uint8_t *q;
+    float *s;
+    int64_t rows, cols, x_stride, q_stride, s_stride;
+    int wide;
+};
+
+/* 16 lanes a block of 128, eight elements each */
+template <typename T> __global__ void __launch_bounds__(256) quantize_rows(QuantRowsParams p) {
+    enter_grid();
+    const int64_t blocks = (p.cols + BLOCK - 1) / BLOCK, item = (int64_t)blockIdx.x * 16 + threadIdx.x / 16;
+    const int lane = threadIdx.x & 15;
+    const int64_t row = item / blocks, b = item - row * blocks;
+    const bool live = row < p.rows;
+    float v[8];
+    uint32_t largest = 0;
+    const int64_t e = b * BLOCK + lane * 8;
+    if (live) {
+        load8((const T *)p.x + row * p.x_stride, e, p.cols, p.wide, v);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) largest = max(largest, magnitude(v[i]));
+    }
+#pragma unroll
+    for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
+    if (!live) return;
+    const float s = scale_of(largest);
+    if (lane == 0) p.s[b * p.s_stride + row] = s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], s);
+    const uint2 q = make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
+    /* rows are a multiple of 16 bytes apart: columns past the end, up to there, become zero */
+    if (e < p.q_stride && e < ((p.cols + 15) & ~15ll)) *(uint2 *)(p.q + row * p.q_stride + e) = q;
+}
+
+struct QuantBlocksParams {
+    const char *w;
+    uint8_t *q;
+    float *s;
+    int64_t rows, cols, w_stride, q_stride, s_stride;
+    int wide;
+};
+
+/* a block of threads for each 128 x 128 block: 16 threads a row, 16 rows at a time, values kept in registers */
+template <typename T> __global__ void __launch_bounds__(256) quantize_blocks(QuantBlocksParams p) {
+    __shared__ uint32_t warps[8];
+    enter_grid();
+    const int64_t row0 = (int64_t)blockIdx.y * BLOCK + threadIdx.x / 16, e = (int64_t)blockIdx.x * BLOCK + (threadIdx.x & 15) * 8;
+    uint32_t largest = 0;
+    float v[8][8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t row = row0 + 16 * i;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        if (row < p.rows) load8((const T *)p.w + row * p.w_stride, e, p.cols, p.wide, v[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(v[i][j]));
+    }
+    largest = __reduce_max_sync(~0u, largest);
+    if ((threadIdx.x & 31) == 0) warps[threadIdx.x >> 5] = largest;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) largest = max(largest, warps[i]);
+    const float s = scale_of(largest);
+    if (threadIdx.x == 0) p.s[blockIdx.y * p.s_stride + blockIdx.x] = s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const int64_t row = row0 + 16 * i;
+        if (row >= p.rows) continue;
+        float u[8];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) u[j] = __fdiv_rn(v[i][j], s);
+        const uint2 q = make_uint2(e4m3x4(u[0], u[1], u[2], u[3]), e4m3x4(u[4], u[5], u[6], u[7]));
+        uint8_t *to = p.q + row * p.q_stride + e;
+        if (e + 8 <= p.cols) {
+            *(uint2 *)to = q;
+        } else {
+            for (int j = 0; j < 8 && e + j < p.cols; ++j) to[j] = (uint8_t)((j < 4 ? q.x : q.y) >> 8 * (j & 3));
+        }
+    }
+}
+
+/* ---- few rows of x -------------------------------------------------------------------- */
+
+struct FewParams {
+    const uint8_t *x, *w;
+    const float *sx, *sw;
+    char *y;
+    int64_t x_stride, w_stride, sx_stride, sw_stride, y_stride;
+    int m, n, k;
+};
+
+__device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k32.row.col.f32.e4m3.e4m3.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+
+/* 16 bytes of a row at byte k, zero from `end` on */
+__device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int end) {
+    if (k + 16 <= end) return *(const uint4 *)(row + k);
+    uint32_t v[4] = {0, 0, 0, 0};
+    for (int i = 0; k + i < end; ++i) v[i >> 2] |= (uint32_t)row[k + i] << 8 * (i & 3);
+    return make_uint4(v[0], v[1], v[2], v[3]);
+}
+
+/* 16 rows of W a block of threads; its 8 warps take every eighth block of 128 columns and join at the end.  A thread loads
+ * 16 consecutive bytes of a row; the order of the columns inside a product is the same for x and W, and free. */
+template <typename T, int NT> __global__ void __launch_bounds__(256) few_rows(FewParams p) {
+    constexpr int WARPS = 8;
+    __shared__ float parts[WARPS][16][8 * NT + 1];
+    enter_grid();
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
+    const int n0 = blockIdx.x * 16, blocks = (p.k + BLOCK - 1) / BLOCK;
+    const uint8_t *w0 = p.w + (int64_t)min(n0 + r, p.n - 1) * p.w_stride, *w1 = p.w + (int64_t)min(n0 + r + 8, p.n - 1) * p.w_stride;
+    float acc[NT][4];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[t][i] = 0.0f;
+#pragma unroll 2
+    for (int b = warp; b < blocks; b += WARPS) {
+        const int k = b * BLOCK + 16 * c;
+        const uint4 a0 = row16(w0, k, p.k), a1 = row16(w1, k, p.k), a2 = row16(w0, k + 64, p.k), a3 = row16(w1, k + 64, p.k);
+        const float sw = p.sw[(n0 / BLOCK) * p.sw_stride + b];
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const int row = 8 * t + r;
+            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
+            if (row < p.m) {
+                const uint8_t *x = p.x + row * p.x_stride;
+                if (k < p.k) x0 = *(const uint4 *)(x + k);
+                if (k + 64 < p.k) x1 = *(const uint4 *)(x + k + 64);
+            }
+            float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+            mma_e4m3(d, a0.x, a1.x, a0.y, a1.y, x0.x, x0.y);
+            mma_e4m3(d, a0.z, a1.z, a0.w, a1.w, x0.z, x0.w);
+            mma_e4m3(d, a2.x, a3.x, a2.y, a3.y, x1.x, x1.y);
+            mma_e4m3(d, a2.z, a3.z, a2.w, a3.w, x1.z, x1.w);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const int own = 8 * t + 2 * c + i;
+                const float s = own < p.m ? sw * p.sx[b * p.sx_stride + own] : 0.0f;
+                acc[t][i] = fmaf(s, d[i], acc[t][i]);
+                acc[t][2 + i] = fmaf(s, d[2 + i], acc[t][2 + i]);
+            }
+        }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) parts[warp][r + 8 * (i >> 1)][8 * t + 2 * c + (i & 1)] = acc[t][i];
+    __syncthreads();
+    for (int i = threadIdx.x; i < 16 * 8 * NT; i += 256) {
+        const int n = i & 15, m = i >> 4;
+        if (m >= p.m || n0 + n >= p.n) continue;
+        float s = 0.0f;
+#pragma unroll
+        for (int v = 0; v < WARPS; ++v) s += parts[v][n][m];
+        ((T *)p.y)[m * p.y_stride + n0 + n] = from_f32<T>(s);
+    }
+}
+
+/* ---- many rows of x: tcgen05 ------------------------------------------------------------ */
+
+/* A tile of 128 rows of x (256 on a pair of SMs) by BN columns of y.  Warp 0 copies, warp 1 multiplies, warps 4 and on scale:
+ * the tensor core sums a block of 128 columns into tensor memory, and the scaling warps add scale times that to the
+ * tile's sums in registers while the next block's product runs (tensor memory holds 512 / BN blocks).  Operands
+ * arrive by TMA in 128-byte rows with the 128-byte swizzle; every wait gives up after 2 s. */
+constexpr uint64_t TIMEOUT_NS = 2000000000ull;
+
+struct ManyParams {
+    const float *sx, *sw;
+    char *y;
+    unsigned *status;
+    int64_t sx_stride, sw_stride, y_stride;
+    int m, n, k_blocks, m_tiles, n_tiles, wide;
+};
+
+__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
+
+__device__ __forceinline__ bool try_wait(uint32_t barrier, uint32_t parity) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\nselp.u32 %0, 1, 0, q;\n}"
+                 : "=r"(ok) : "r"(barrier), "r"(parity) : "memory");
+    return ok;
+}
+__device__ __forceinline__ uint64_t now_ns() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return t;
+}
+/* false when the wait gave up, here or in another role */
+__device__ __forceinline__ bool wait_slowly(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
+    const uint64_t start = now_ns();
+    while (!try_wait(barrier, parity)) {
+        if (*abort) return false;
+        if (now_ns() - start > TIMEOUT_NS) {
+            *abort = 1;
+            atomicOr(status, role);
+            return false;
+        }
+    }
+    return true;
+}
+__device__ __forceinline__ bool wait_for(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
+    if (try_wait(barrier, parity)) return true;
+    return wait_slowly(barrier, parity, abort, status, role);
+}
+
+struct TensorMap {
+    alignas(64) unsigned char bytes[128];
+};
+
+template <bool PAIR>
+__device__ __forceinline__ void tma_load(uint32_t to, const TensorMap *map, int x, int y, uint32_t barrier) {
+    if (PAIR)
+        asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(barrier) : "memory");
+    else
+        asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                     ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(barrier) : "memory");
+}
+template <bool PAIR>
+__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+    if (PAIR)
+        asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, q;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+    else
+        asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, q;\n}"
+                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+}
+template <bool PAIR> __device__ __forceinline__ void commit(uint32_t barrier) {
+    if (PAIR)
+        asm volatile("{\n.reg .b16 m;\nmov.b16 m, 3;\n"
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], m;\n}"
+                     ::"r"(barrier) : "memory");
+    else
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+}
+/* K-major rows of 128 bytes, 128-byte swizzle, eight rows 1024 bytes apart */
+__device__ __forceinline__ uint64_t operand(uint32_t address) {
+    return (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | (1u << 16) | ((address & 0x3ffff) >> 4);
+}
+__device__ __forceinline__ void tensor_load(uint32_t address, float (&v)[32]) {
+    uint32_t *u = (uint32_t *)v;
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+                   "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
+                   "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
+                   "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
+                 : "r"(address));
+}
+
+template <int BN, bool PAIR> struct ManyShape {
+    static constexpr int ROWS = PAIR ? 256 : 128;                     /* of a tile */
+    static constexpr int B_ROWS = PAIR ? BN / 2 : BN;                 /* rows of W that one SM copies */
+    static constexpr int A_BYTES = 128 * BLOCK, B_BYTES = B_ROWS * BLOCK, STAGE = A_BYTES + B_BYTES;
+    static constexpr int STAGES = STAGE > 40960 ? 4 : STAGE >= 32768 ? 6 : 8;
+    static constexpr int BUFFERS = 512 / BN > 4 ? 4 : 512 / BN;
+    static constexpr int COLUMNS = BN * BUFFERS < 32 ? 32 : BN * BUFFERS;
+    static constexpr int SCALE_WARPS = BN >= 128 ? 8 : 4;
+    static constexpr int PER = BN / (SCALE_WARPS / 4);                /* columns a scaling thread */
+    static constexpr int THREADS = 128 + 32 * SCALE_WARPS;
+    static constexpr bool SPLIT = PER == 128;     /* the scaling warps need more registers than an even share */
+    static constexpr int SMEM = STAGES * STAGE + 1024;
+};
+
+template <typename T, int BN, bool PAIR>
+__global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
+    many_rows(const __grid_constant__ TensorMap x_map, const __grid_constant__ TensorMap w_map, ManyParams p) {
+    using S = ManyShape<BN, PAIR>;
+    extern __shared__ unsigned char raw[];
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS];
+    __shared__ uint32_t tensor_base;
+    __shared__ volatile unsigned abort;
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t ring = (shared_address(raw) + 1023) & ~1023u;
+    uint32_t rank = 0;
+    if (PAIR) asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&full[i])));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&empty[i])));
+        }
+        for (int i = 0; i < S::BUFFERS; ++i) {
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&summed[i])));
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&read[i])), "r"(S::SCALE_WARPS * (PAIR ? 2 : 1)));
+        }
+        abort = 0;
+        asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
+    }
+    if (PAIR) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    if (warp == 1) {
+        const uint32_t to = shared_address(&tensor_base);
+        if (PAIR)
+            asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                         "tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::"r"(to), "n"(S::COLUMNS) : "memory");
+        else
+            asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;\n"
+                         "tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::"r"(to), "n"(S::COLUMNS) : "memory");
+    }
+    enter_grid();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    const uint32_t base = tensor_base;
+    const int worker = PAIR ? blockIdx.x / 2 : blockIdx.x, workers = PAIR ? gridDim.x / 2 : gridDim.x;
+    const int tiles = p.m_tiles * p.n_tiles;
+
+    /* tiles that run together share rows and columns: groups of 16 row tiles, column by column */
+    auto place = [&](int t, int &m0, int &n0) {
+        const int group = t / (16 * p.n_tiles), first = group * 16, rows = min(16, p.m_tiles - first);
+        const int r = t - first * p.n_tiles;
+        n0 = r / rows * BN;
+        m0 = (first + r % rows) * S::ROWS;
+    };
+
+    if (warp < 4 && S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp == 0) {
+        if (lane == 0) {
+            uint32_t leader = shared_address(&full[0]);
+            if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(leader));
+            int stage = 0;
+            uint32_t phase = 0;
+            bool ok = true;
+            for (int t = worker; t < tiles && ok; t += workers) {
+                int m0, n0;
+                place(t, m0, n0);
+                if (PAIR) m0 += 128 * rank, n0 += S::B_ROWS * rank;
+                for (int b = 0; b < p.k_blocks; ++b) {
+                    if (!(ok = wait_for(shared_address(&empty[stage]), phase ^ 1, &abort, p.status, 1))) break;
+                    if (rank == 0)      /* both copies of a pair complete on the leader's barrier */
+                        asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
+                                     ::"r"(shared_address(&full[stage])), "r"(S::STAGE * (PAIR ? 2 : 1)) : "memory");
+                    const uint32_t to = ring + stage * S::STAGE, barrier = leader + 8 * stage;
+                    tma_load<PAIR>(to, &x_map, b * BLOCK, m0, barrier);
+                    tma_load<PAIR>(to + S::A_BYTES, &w_map, b * BLOCK, n0, barrier);
+                    if (++stage == S::STAGES) stage = 0, phase ^= 1;
+                }
+            }
+        }
+    } else if (warp == 1) {
+        if (lane == 0 && rank == 0) {
+            constexpr uint32_t idesc = 1u << 4 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(S::ROWS >> 4) << 24;
+            int stage = 0, buffer = 0;
+            uint32_t phase = 0, buffer_phase = 0;
+            bool ok = true;
+            for (int t = worker; t < tiles && ok; t += workers)
+                for (int b = 0; b < p.k_blocks; ++b) {
+                    if (!(ok = wait_for(shared_address(&read[buffer]), buffer_phase ^ 1, &abort, p.status, 2))) break;
+                    if (!(ok = wait_for(shared_address(&full[stage]), phase, &abort, p.status, 2))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    const uint32_t a = ring + stage * S::STAGE;
+#pragma unroll
+                    for (int i = 0; i < BLOCK / 32; ++i)
+                        multiply<PAIR>(base + buffer * BN, operand(a + 32 * i), operand(a + S::A_BYTES + 32 * i), idesc, i > 0);
+                    commit<PAIR>(shared_address(&empty[stage]));
+                    commit<PAIR>(shared_address(&summed[buffer]));
+                    if (++stage == S::STAGES) stage = 0, phase ^= 1;
+                    if (++buffer == S::BUFFERS) buffer = 0, buffer_phase ^= 1;
+                }
+        }
+    } else if (warp >= 4) {
+        if (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");      /* 256 of them, and 128 with 56: 384 of 168 */
+        const int quarter = warp & 3, half = (warp - 4) >> 2;
+        const uint32_t mine = base + (uint32_t)(quarter * 32) * 65536 + half * S::PER;
+        uint32_t leader = shared_address(&read[0]);
+        if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(leader));
+        int buffer = 0;
+        uint32_t phase = 0;
+        bool ok = true;
+        for (int t = worker; t < tiles && ok; t += workers) {
+            int m0, n0;
+            place(t, m0, n0);
+            const int row = m0 + 128 * rank + 32 * quarter + lane, col = n0 + half * S::PER;
+            const float *sx = p.sx + row, *sw = p.sw + (int64_t)(min(col, p.n - 1) / BLOCK) * p.sw_stride;
+            const bool live = row < p.m;
+            float sum[S::PER];
+#pragma unroll
+            for (int i = 0; i < S::PER; ++i) sum[i] = 0.0f;
+            float next = live ? *sx * *sw : 0.0f;
+            for (int b = 0; b < p.k_blocks; ++b) {
+                const float s = next;
+                if (b + 1 < p.k_blocks && live) next = sx[(b + 1) * p.sx_stride] * sw[b + 1];
+                if (!(ok = wait_for(shared_address(&summed[buffer]), phase, &abort, p.status, 4))) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+#pragma unroll
+                for (int c = 0; c < S::PER; c += 32) {
+                    float v[32];
+                    tensor_load(mine + buffer * BN + c, v);
+                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
+                    if (c + 32 >= S::PER) {     /* all of it is in registers */
+                        asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+                        __syncwarp();
+                        if (lane == 0) {
+                            if (PAIR)
+                                asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(leader + 8 * buffer) : "memory");
+                            else
+                                asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(leader + 8 * buffer) : "memory");
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) sum[c + i] = fmaf(s, v[i], sum[c + i]);
+                }
+                if (++buffer == S::BUFFERS) buffer = 0, phase ^= 1;
+            }
+            if (!live || !ok) continue;
+            T *y = (T *)p.y + row * p.y_stride + col;
+            constexpr int V = 16 / sizeof(T);
+#pragma unroll
+            for (int i = 0; i < S::PER; i += V) {
+                if (p.wide && col + i + V <= p.n) {
+                    Pack<T, V> q;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) q.at[j] = from_f32<T>(sum[i + j]);
+                    *(Pack<T, V> *)(y + i) = q;
+                } else {
+#pragma unroll
+                    for (int j = 0; j < V; ++j)
+                        if (col + i + j < p.n) y[i + j] = from_f32<T>(sum[i + j]);
+                }
+            }
+        }
+    }
+    __syncwarp();
+    asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
+    __syncthreads();
+    if (PAIR) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
+    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+    if (warp == 1) {
+        if (PAIR)
+            asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(S::COLUMNS));
+        else
+            asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(S::COLUMNS));
+    }
+}
+
+int encode(TensorMap *map, uint64_t at, int64_t cols, int64_t rows, int64_t stride, int box_rows) {
+    const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)stride};
+    const unsigned box[2] = {BLOCK, (unsigned)box_rows}, steps[2] = {1, 1};
+    /* bytes, no interleave, 128-byte swizzle, 256-byte L2 promotion, zeros outside */
+    if (int e = emmy_rt_tensor_map_encode_tiled(map, 0, 2, at, dims, strides, box, steps, 0, 3, 3, 0))
+        return ops_fail(e, "tensor map: %s", emmy_rt_last_error());
+    return 0;
+}
+
+template <typename T, int BN, bool PAIR> int go_many(const emmy_ops_blockfp8_args *a, ManyParams p, int device, uint64_t stream) {
+    using S = ManyShape<BN, PAIR>;
+    static uint64_t allowed;
+    if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
+        cudaError_t e = cudaFuncSetAttribute(many_rows<T, BN, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, S::SMEM);
+        if (e != cudaSuccess) return ops_cuda(e, "shared memory of the FP8 product");
+        __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
+    }
+    TensorMap x, w;
+    if (int e = encode(&x, a->xq, a->k, a->m, a->xq_stride, 128)) return e;
+    if (int e = encode(&w, a->wq, a->k, a->n, a->wq_stride, S::B_ROWS)) return e;
+    int sms;
+    if (int e = ops_sm_count(device, &sms)) return e;
+    p.m_tiles = (int)((a->m + S::ROWS - 1) / S::ROWS);
+    p.n_tiles = (int)((a->n + BN - 1) / BN);
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const int workers = PAIR ? sms / 2 : sms, blocks = (int)(tiles < workers ? tiles : workers) * (PAIR ? 2 : 1);
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(S::THREADS), cfg.dynamicSmemBytes = S::SMEM;
+    cfg.stream = (cudaStream_t)(uintptr_t)stream;
+    cudaLaunchAttribute attributes[2] = {};
+    attributes[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attributes[0].val.programmaticStreamSerializationAllowed = 1;
+    attributes[1].id = cudaLaunchAttributeClusterDimension;
+    attributes[1].val.clusterDim.x = PAIR ? 2 : 1, attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
+    cfg.attrs = attributes, cfg.numAttrs = 2;
+    return ops_cuda(cudaLaunchKernelEx(&cfg, many_rows<T, BN, PAIR>, x, w, p), "FP8 product");
+}
+
+template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, uint64_t stream) {
+    if (a->m <= 32) {
+        FewParams p = {(const uint8_t *)(uintptr_t)a->xq, (const uint8_t *)(uintptr_t)a->wq, (const float *)(uintptr_t)a->xs,
+                       (const float *)(uintptr_t)a->ws, (char *)(uintptr_t)a->y, a->xq_stride, a->wq_stride, a->xs_stride,
+                       a->ws_stride, a->y_stride, (int)a->m, (int)a->n, (int)a->k};
+        const dim3 grid((unsigned)((a->n + 15) / 16));
+        cudaError_t e = a->m <= 8    ? launch(few_rows<T, 1>, grid, dim3(256), 0, stream, p)
+                        : a->m <= 16 ? launch(few_rows<T, 2>, grid, dim3(256), 0, stream, p)
+                                     : launch(few_rows<T, 4>, grid, dim3(256), 0, stream, p);
+        return ops_cuda(e, "FP8 product of few rows");
+    }
+    ManyParams p = {};
+    p.sx = (const float *)(uintptr_t)a->xs, p.sw = (const float *)(uintptr_t)a->ws, p.y = (char *)(uintptr_t)a->y;
+    p.status = (unsigned *)(uintptr_t)a->status;
+    p.sx_stride = a->xs_stride, p.sw_stride = a->ws_stride, p.y_stride = a->y_stride;
+    p.m = (int)a->m, p.n = (int)a->n, p.k_blocks = (int)((a->k + BLOCK - 1) / BLOCK);
+    p.wide = aligned(a->y, 16) && a->y_stride * sizeof(T) % 16 == 0;
+    int sms;
+    if (int e = ops_sm_count(device, &sms)) return e;
+    /* the widest tiles that still give every SM one */
+    const int64_t rows = (a->m + 127) / 128;
+    if (a->m > 128 && ((a->m + 255) / 256) * ((a->n + 255) / 256) * 2 >= sms) return go_many<T, 256, true>(a, p, device, stream);
+    if (rows * ((a->n + 127) / 128) >= sms) return go_many<T, 128, false>(a, p, device, stream);
+    if (rows * ((a->n + 63) / 64) >= sms) return go_many<T, 64, false>(a, p, device, stream);
+    return go_many<T, 32, false>(a, p, device, stream);
+}
+
+int check_matrix(const char *name, uint64_t at, int64_t rows, int64_t cols, int64_t stride, int size, int multiple) {
+    if (rows < 0 || cols < 1 || rows > 0x7fffff00LL || cols > 0x7fffff00LL)
+        return ops_fail(EMMY_RT_EINVAL, "%s of %lld x %lld", name, (long long)rows, (long long)cols);
+    if (rows > 1 && stride < cols) return ops_fail(EMMY_RT_EINVAL, "%s: rows overlap: stride %lld", name, (long long)stride);
+    if (!at || !aligned(at, size * multiple)) return ops_fail(EMMY_RT_EINVAL, "%s is needed, on %d bytes", name, size * multiple);
+    if (stride % multiple) return ops_fail(EMMY_RT_EINVAL, "%s: rows are not a multiple of %d elements apart", name, multiple);
+    return 0;
+}
+
+}  // namespace
+
+EMMY_EXPORT int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args *a, int device, uint64_t stream) {
+    if (!a) return ops_fail(EMMY_RT_EINVAL, "no arguments");
+    if (!known_dtype(a->dtype)) return ops_fail(EMMY_RT_EINVAL, "element type %d", a->dtype);
+    const int es = elem_size(a->dtype);
+    const int64_t row_blocks = a->square ? (a->rows + BLOCK - 1) / BLOCK : a->rows, col_blocks = (a->cols + BLOCK - 1) / BLOCK;
+    if (int e = check_matrix("x", a->rows ? a->x : 16, a->rows, a->cols, a->x_stride, es, 1)) return e;
+    if (int e = check_matrix("q", a->rows ? a->q : 16, a->rows, a->cols, a->q_stride, 1, 16)) return e;
+    if (a->q_stride < (a->cols + 15) / 16 * 16) return ops_fail(EMMY_RT_EINVAL, "rows of q are not padded to 16 bytes");
+    if (int e = check_matrix("s", a->rows ? a->s : 16, a->square ? row_blocks : col_blocks, a->square ? col_blocks : a->rows > 0 ? a->rows : 1,
+                             a->s_stride, 4, 1))
+        return e;
+    if (a->rows == 0) return 0;
+    DeviceScope scope(device);
+    if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
+    const int wide = aligned(a->x, 16) && a->x_stride * es % 16 == 0;
+    cudaError_t e;
+    if (a->square) {
+        if (row_blocks > 65535) return ops_fail(EMMY_RT_EINVAL, "%lld rows of a weight", (long long)a->rows);
+        QuantBlocksParams p = {(const char *)(uintptr_t)a->x, (uint8_t *)(uintptr_t)a->q, (float *)(uintptr_t)a->s, a->rows, a->cols,
+                               a->x_stride, a->q_stride, a->s_stride, wide};
+        const dim3 grid((unsigned)col_blocks, (unsigned)row_blocks);
+        e = a->dtype == EMMY_OPS_F32   ? launch(quantize_blocks<float>, grid, dim3(256), 0, stream, p)
+            : a->dtype == EMMY_OPS_F16 ? launch(quantize_blocks<__half>, grid, dim3(256), 0, stream, p)
+                                       : launch(quantize_blocks<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
+    } else {
+        if (a->rows * col_blocks > 0x7fffffffLL * 16) return ops_fail(EMMY_RT_EINVAL, "x of %lld x %lld", (long long)a->rows, (long long)a->cols);
+        QuantRowsParams p = {(const char *)(uintptr_t)a->x, (uint8_t *)(uintptr_t)a->q, (float *)(uintptr_t)a->s, a->rows, a->cols,
+                             a->x_stride, a->q_stride, a->s_stride, wide};
+        const dim3 grid((unsigned)((a->rows * col_blocks + 15) / 16));
+        e = a->dtype == EMMY_OPS_F32   ? launch(quantize_rows<float>, grid, dim3(256), 0, stream, p)
+            : a->dtype == EMMY_OPS_F16 ? launch(quantize_rows<__half>, grid, dim3(256), 0, stream, p)
+                                       : launch(quantize_rows<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
+    }
+    return ops_cuda(e, "FP8 quantisation");
+}
+
+EMMY_EXPORT int emmy_ops_blockfp8_product(const emmy_ops_blockfp8_args *a, int device, uint64_t stream) {
+    if (!a) return ops_fail(EMMY_RT_EINVAL, "no arguments");
+    if (!known_dtype(a->dtype)) return ops_fail(EMMY_RT_EINVAL, "element type %d", a->dtype);
+    const int es = elem_size(a->dtype);
+    const int64_t k_blocks = (a->k + BLOCK - 1) / BLOCK, n_blocks = (a->n + BLOCK - 1) / BLOCK;
+    if (a->n < 1) return ops_fail(EMMY_RT_EINVAL, "n %lld", (long long)a->n);
+    if (int e = check_matrix("xq", a->m ? a->xq : 16, a->m, a->k, a->xq_stride, 1, 16)) return e;
+    if (int e = check_matrix("wq", a->wq, a->n, a->k, a->wq_stride, 1, 16)) return e;
+    if (a->xq_stride < (a->k + 15) / 16 * 16 || a->wq_stride < (a->k + 15) / 16 * 16)
+        return ops_fail(EMMY_RT_EINVAL, "rows of xq and wq are not padded to 16 bytes");
+    if (int e = check_matrix("xs", a->m ? a->xs : 16, k_blocks, a->m > 0 ? a->m : 1, a->xs_stride, 4, 1)) return e;
+    if (int e = check_matrix("ws", a->ws, n_blocks, k_blocks, a->ws_stride, 4, 1)) return e;
+    if (int e = check_matrix("y", a->m ? a->y : 16, a->m, a->n, a->y_stride, es, 1)) return e;
+    if (!a->status || !aligned(a->status, 4)) return ops_fail(EMMY_RT_EINVAL, "a status word is needed");
+    if (((a->m + 127) / 128) * ((a->n + 31) / 32) > 0x7fffffffLL)
+        return ops_fail(EMMY_RT_EINVAL, "y of %lld x %lld", (long long)a->m, (long long)a->n);
+    if (a->m == 0) return 0;
+    DeviceScope scope(device);
+    if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
+    return a->dtype == EMMY_OPS_F32   ? product<float>(a, device, stream)
+           : a->dtype == EMMY_OPS_F16 ? product<__half>(a, device, stream)
+                                      : product<__nv_bfloat16>(a, device, stream);
+}
+
+EMMY_EXPORT int emmy_ops_blockfp8_linear(const emmy_ops_blockfp8_linear_args *a, int device, uint64_t stream) {
+    if (!a) return ops_fail(EMMY_RT_EINVAL, "no arguments");
+    const emmy_ops_blockfp8_args &q = a->product;
+    if (q.m == 0) return 0;
+    const emmy_ops_blockfp8_quantize_args x = {a->x, q.xq, q.xs, a->x_stride, q.xq_stride, q.xs_stride, q.m, q.k, a->x_dtype, 0};
+    if (int e = emmy_ops_blockfp8_quantize(&x, device, stream)) return e;
+    return emmy_ops_blockfp8_product(&q, device, stream);
+}

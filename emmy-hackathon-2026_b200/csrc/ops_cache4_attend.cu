@@ -706,19 +706,6 @@ __global__ void __launch_bounds__(128) cache4_join(AttendParams p, int blocks) {
         from_f32<T>(sum > 0.0f || sum != sum ? out / sum : 0.0f);
 }
 
-int sm_count(int device, int *out) {
-    static int counts[64];
-    if (device < 0 || device >= 64) return ops_fail(EMMY_RT_EINVAL, "device %d", device);
-    int n = __atomic_load_n(&counts[device], __ATOMIC_RELAXED);
-    if (!n) {
-        cudaError_t e = cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device);
-        if (e != cudaSuccess) return ops_cuda(e, "device attribute");
-        __atomic_store_n(&counts[device], n, __ATOMIC_RELAXED);
-    }
-    *out = n;
-    return 0;
-}
-
 template <typename T, int DIM, int NT, bool WHOLE> int go(const AttendParams &p, int sms, int device, uint64_t stream) {
     const size_t smem = sizeof(Shared<DIM, NT>) + 4 * ((size_t)p.batch + 1);
     static uint64_t allowed;                 /* devices whose limit is raised */
@@ -752,7 +739,7 @@ uint64_t workspace(int sms, int dim) {
 EMMY_EXPORT int emmy_ops_cache4_attend_workspace(int dim, int device, uint64_t *bytes) {
     if (!bytes || (dim != 64 && dim != 128)) return ops_fail(EMMY_RT_EINVAL, "head dim %d is not 64 or 128", dim);
     int sms;
-    if (int e = sm_count(device, &sms)) return e;
+    if (int e = ops_sm_count(device, &sms)) return e;
     *bytes = workspace(sms, dim);
     return 0;
 }
@@ -799,7 +786,7 @@ EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int
         p.page_shift = shift - 1;
     }
     int sms;
-    if (int e = sm_count(device, &sms)) return e;
+    if (int e = ops_sm_count(device, &sms)) return e;
     if (a->workspace_bytes < workspace(sms, a->cache.dim))
         return ops_fail(EMMY_RT_ESCRATCH, "a workspace of %llu bytes is too small", (unsigned long long)a->workspace_bytes);
     DeviceScope scope(device);

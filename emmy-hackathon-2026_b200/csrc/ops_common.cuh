@@ -15,6 +15,7 @@
 /* records the text of a failure and returns its status */
 int ops_fail(int status, const char *format, ...);
 int ops_cuda(cudaError_t e, const char *what);
+int ops_sm_count(int device, int *out);
 
 /* makes `device` current for the lifetime of the object */
 struct DeviceScope {

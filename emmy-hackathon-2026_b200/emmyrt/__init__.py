@@ -504,12 +504,35 @@ class Cache4AttendArgs(ctypes.Structure):
         [(n, ctypes.c_int32) for n in ("batch", "tokens", "q_heads", "max_pages", "dtype")] + [("scale", ctypes.c_float)]
 
 
+class BlockFp8QuantizeArgs(ctypes.Structure):
+    """emmy_ops_blockfp8_quantize_args"""
+    _fields_ = [(n, _u64) for n in ("x", "q", "s")] + \
+        [(n, ctypes.c_int64) for n in ("x_stride", "q_stride", "s_stride", "rows", "cols")] + \
+        [("dtype", ctypes.c_int32), ("square", ctypes.c_int32)]
+
+
+class BlockFp8Args(ctypes.Structure):
+    """emmy_ops_blockfp8_args"""
+    _fields_ = [(n, _u64) for n in ("xq", "xs", "wq", "ws", "y", "status")] + \
+        [(n, ctypes.c_int64) for n in ("xq_stride", "xs_stride", "wq_stride", "ws_stride", "y_stride", "m", "n", "k")] + \
+        [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
+class BlockFp8LinearArgs(ctypes.Structure):
+    """emmy_ops_blockfp8_linear_args"""
+    _fields_ = BlockFp8Args._fields_ + [("x", _u64), ("x_stride", ctypes.c_int64), ("x_dtype", ctypes.c_int32),
+                                        ("reserved2", ctypes.c_int32)]
+
+
 # every symbol declared in include/emmyrt_ops.h, with its ctypes signature
 OPS_SIGNATURES = {
     "emmy_ops_last_error": ([], ctypes.c_char_p),
     "emmy_ops_current_device": ([_P(_int)], _int),
     "emmy_ops_residual_norm": ([_P(NormArgs), _int, _u64], _int),
     "emmy_ops_rotary": ([_P(RotaryArgs), _int, _u64], _int),
+    "emmy_ops_blockfp8_quantize": ([_P(BlockFp8QuantizeArgs), _int, _u64], _int),
+    "emmy_ops_blockfp8_product": ([_P(BlockFp8Args), _int, _u64], _int),
+    "emmy_ops_blockfp8_linear": ([_P(BlockFp8LinearArgs), _int, _u64], _int),
     "emmy_ops_cache4_append": ([_P(Cache4AppendArgs), _int, _u64], _int),
     "emmy_ops_cache4_attend_workspace": ([_int, _int, _P(_u64)], _int),
     "emmy_ops_cache4_attend": ([_P(Cache4AttendArgs), _int, _u64], _int),

@@ -88,6 +88,42 @@ typedef struct {
 
 int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint64_t stream);
 
+/* ---- FP8 (e4m3) products with a scale for each block of 128 --------------------------------- */
+
+/* q = e4m3(x / s), s = amax / 448 (1 where that is 0), over 128 columns of a row (square 0:
+ * s is [blocks of columns][rows]) or over 128 x 128 (square 1: s is [blocks of rows][blocks of
+ * columns]).  Rows of q are a multiple of 16 bytes apart; without square, columns up to the
+ * next multiple of 16 become zero. */
+typedef struct {
+    uint64_t x, q, s;
+    int64_t x_stride, q_stride, s_stride, rows, cols;
+    int32_t dtype, square;                    /* dtype of x */
+} emmy_ops_blockfp8_quantize_args;
+
+int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args *a, int device, uint64_t stream);
+
+/* y[m, n] = sum over blocks b of xs[b, m] ws[n / 128, b] sum over k in b of xq[m, k] wq[n, k], in
+ * f32, as quantised above (xq without square, its padding zero; wq with).  *status (a word of
+ * device memory, zeroed by the caller once) gets a bit when a wait inside the kernel gave
+ * up after 2 s; y is then not valid. */
+typedef struct {
+    uint64_t xq, xs, wq, ws, y, status;
+    int64_t xq_stride, xs_stride, wq_stride, ws_stride, y_stride, m, n, k;
+    int32_t dtype, reserved;                  /* dtype of y */
+} emmy_ops_blockfp8_args;
+
+int emmy_ops_blockfp8_product(const emmy_ops_blockfp8_args *a, int device, uint64_t stream);
+
+/* Both in a row: x (m x k, of x_dtype) quantised into product.xq and product.xs, then the product. */
+typedef struct {
+    emmy_ops_blockfp8_args product;
+    uint64_t x;
+    int64_t x_stride;
+    int32_t x_dtype, reserved;
+} emmy_ops_blockfp8_linear_args;
+
+int emmy_ops_blockfp8_linear(const emmy_ops_blockfp8_linear_args *a, int device, uint64_t stream);
+
 /* ---- a paged key / value cache in 4 bits -------------------------------------------------- */
 
 /* Levels [pages, heads, page, dim / 2] bytes (element 2 i in the low half of byte i) and

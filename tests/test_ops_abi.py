@@ -9,7 +9,9 @@ import pytest
 from conftest import ROOT
 
 STRUCTS = {"emmy_ops_norm_args": "NormArgs", "emmy_ops_rotary_args": "RotaryArgs",
-           "emmy_ops_cache4_append_args": "Cache4AppendArgs"}
+           "emmy_ops_cache4_append_args": "Cache4AppendArgs", "emmy_ops_cache4_attend_args": "Cache4AttendArgs",
+           "emmy_ops_blockfp8_quantize_args": "BlockFp8QuantizeArgs", "emmy_ops_blockfp8_args": "BlockFp8Args",
+           "emmy_ops_blockfp8_linear_args": "BlockFp8LinearArgs"}
 
 
 def test_exports_match_header():
@@ -22,6 +24,9 @@ def test_exports_match_header():
 
 
 def c_name(field: str, struct: str) -> str:
+    if struct == "emmy_ops_blockfp8_linear_args":
+        own = {"x": "x", "x_stride": "x_stride", "x_dtype": "x_dtype", "reserved2": "reserved"}
+        return own.get(field, "product." + field)
     if field.startswith("cache_"):
         return "cache." + field[6:]
     if struct == "emmy_ops_rotary_args" and field[-1] in "01":
