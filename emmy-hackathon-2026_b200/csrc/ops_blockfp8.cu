@@ -318,15 +318,47 @@ template <bool PAIR> __device__ __forceinline__ void commit(uint32_t barrier) {
 __device__ __forceinline__ uint64_t operand(uint32_t address) {
     return (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | (1u << 16) | ((address & 0x3ffff) >> 4);
 }
-__device__ __forceinline__ void tensor_load(uint32_t address, float (&v)[32]) {
-    uint32_t *u = (uint32_t *)v;
-    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-                 "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+__device__ __forceinline__ void tensor_load(uint32_t address, uint32_t (&u)[32]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
                  : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
                    "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15]), "=r"(u[16]),
                    "=r"(u[17]), "=r"(u[18]), "=r"(u[19]), "=r"(u[20]), "=r"(u[21]), "=r"(u[22]), "=r"(u[23]), "=r"(u[24]),
                    "=r"(u[25]), "=r"(u[26]), "=r"(u[27]), "=r"(u[28]), "=r"(u[29]), "=r"(u[30]), "=r"(u[31])
                  : "r"(address));
+}
+/* the loads before it are done; `u` passes through, so that no use of it moves ahead of the wait */
+__device__ __forceinline__ void tensor_wait(uint32_t (&u)[32]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]),
+                   "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15]), "+r"(u[16]),
+                   "+r"(u[17]), "+r"(u[18]), "+r"(u[19]), "+r"(u[20]), "+r"(u[21]), "+r"(u[22]), "+r"(u[23]), "+r"(u[24]),
+                   "+r"(u[25]), "+r"(u[26]), "+r"(u[27]), "+r"(u[28]), "+r"(u[29]), "+r"(u[30]), "+r"(u[31])::"memory");
+}
+__device__ __forceinline__ void tensor_load(uint32_t address, uint32_t (&u)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+                 "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(u[0]), "=r"(u[1]), "=r"(u[2]), "=r"(u[3]), "=r"(u[4]), "=r"(u[5]), "=r"(u[6]), "=r"(u[7]), "=r"(u[8]),
+                   "=r"(u[9]), "=r"(u[10]), "=r"(u[11]), "=r"(u[12]), "=r"(u[13]), "=r"(u[14]), "=r"(u[15])
+                 : "r"(address));
+}
+/* the loads before it are done; `u` passes through, so that no use of it moves ahead of the wait */
+__device__ __forceinline__ void tensor_wait(uint32_t (&u)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(u[0]), "+r"(u[1]), "+r"(u[2]), "+r"(u[3]), "+r"(u[4]), "+r"(u[5]), "+r"(u[6]), "+r"(u[7]), "+r"(u[8]),
+                   "+r"(u[9]), "+r"(u[10]), "+r"(u[11]), "+r"(u[12]), "+r"(u[13]), "+r"(u[14]), "+r"(u[15])::"memory");
+}
+/* a pair of f32 sums: sum += s v */
+__device__ __forceinline__ void add_scaled(uint64_t &sum, uint64_t s, uint32_t v0, uint32_t v1) {
+    uint64_t v;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "r"(v0), "r"(v1));
+    asm("fma.rn.f32x2 %0, %1, %2, %0;" : "+l"(sum) : "l"(s), "l"(v));
+}
+
+__device__ __forceinline__ float half_of(uint64_t v, int high) {
+    float a, b;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v));
+    return high ? b : a;
 }
 
 template <int BN, bool PAIR> struct ManyShape {
@@ -338,6 +370,7 @@ template <int BN, bool PAIR> struct ManyShape {
     static constexpr int COLUMNS = BN * BUFFERS < 32 ? 32 : BN * BUFFERS;
     static constexpr int SCALE_WARPS = BN >= 128 ? 8 : 4;
     static constexpr int PER = BN / (SCALE_WARPS / 4);                /* columns a scaling thread */
+    static constexpr int CHUNK = PER >= 64 ? 32 : 16, CHUNKS = PER / CHUNK;   /* columns a load of tensor memory */
     static constexpr int THREADS = 128 + 32 * SCALE_WARPS;
     static constexpr bool SPLIT = PER == 128;     /* the scaling warps need more registers than an even share */
     static constexpr int SMEM = STAGES * STAGE + 1024;
@@ -393,7 +426,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         m0 = (first + r % rows) * S::ROWS;
     };
 
-    if (warp < 4 && S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 56;");
+    if (warp < 4 && S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 0) {
         if (lane == 0) {
             uint32_t leader = shared_address(&full[0]);
@@ -439,7 +472,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                 }
         }
     } else if (warp >= 4) {
-        if (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 224;");      /* 256 of them, and 128 with 56: 384 of 168 */
+        if (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");      /* 256 of them, and 128 with 40: 384 of 168 */
         const int quarter = warp & 3, half = (warp - 4) >> 2;
         const uint32_t mine = base + (uint32_t)(quarter * 32) * 65536 + half * S::PER;
         uint32_t leader = shared_address(&read[0]);
@@ -453,29 +486,41 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             const int row = m0 + 128 * rank + 32 * quarter + lane, col = n0 + half * S::PER;
             const float *sx = p.sx + row, *sw = p.sw + (int64_t)(min(col, p.n - 1) / BLOCK) * p.sw_stride;
             const bool live = row < p.m;
-            float sum[S::PER];
+            uint64_t sum[S::PER / 2];
 #pragma unroll
-            for (int i = 0; i < S::PER; ++i) sum[i] = 0.0f;
+            for (int i = 0; i < S::PER / 2; ++i) sum[i] = 0;
             /* scales are fetched four blocks ahead of their use, which hides their way from L2 */
-            float ahead[4];
+            float ahead[4], now[4];
             auto fetch = [&](int b, int i) { ahead[i] = live && b + i < p.k_blocks ? sx[(b + i) * p.sx_stride] * sw[b + i] : 0.0f; };
 #pragma unroll
             for (int i = 0; i < 4; ++i) fetch(0, i);
-            for (int b0 = 0; b0 < p.k_blocks && ok; b0 += 4) {
-                const float now[4] = {ahead[0], ahead[1], ahead[2], ahead[3]};
-#pragma unroll
-                for (int i = 0; i < 4; ++i) fetch(b0 + 4, i);
-#pragma unroll 1
-                for (int i = 0; i < 4 && b0 + i < p.k_blocks; ++i) {
-                const float s = i == 0 ? now[0] : i == 1 ? now[1] : i == 2 ? now[2] : now[3];
-                if (!(ok = wait_for(shared_address(&summed[buffer]), phase, &abort, p.status, 4))) break;
+            /* a load of tensor memory is under way while the one before it is added, from block to block too */
+            uint32_t v[2][S::CHUNK];
+            auto begin = [&] {
+                if (!wait_for(shared_address(&summed[buffer]), phase, &abort, p.status, 4)) return false;
                 asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                tensor_load(mine + buffer * BN, v[0]);
+                return true;
+            };
+            if (!(ok = begin())) continue;
+#pragma unroll 1
+            for (int b = 0; b < p.k_blocks; ++b) {
+                if ((b & 3) == 0) {
 #pragma unroll
-                for (int c = 0; c < S::PER; c += 32) {
-                    float v[32];
-                    tensor_load(mine + buffer * BN + c, v);
-                    asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory");
-                    if (c + 32 >= S::PER) {     /* all of it is in registers */
+                    for (int i = 0; i < 4; ++i) now[i] = ahead[i];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) fetch(b + 4, i);
+                }
+                const float one = (b & 2) ? ((b & 1) ? now[3] : now[2]) : ((b & 1) ? now[1] : now[0]);
+                uint64_t s;
+                asm("mov.b64 %0, {%1, %1};" : "=l"(s) : "f"(one));
+#pragma unroll
+                for (int c = 0; c < S::CHUNKS; ++c) {
+                    tensor_wait(v[c & 1]);
+                    if (c + 1 < S::CHUNKS) {
+                        tensor_load(mine + buffer * BN + (c + 1) * S::CHUNK, v[(c + 1) & 1]);
+                    } else {
+                        /* all of the block is in registers */
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
@@ -484,12 +529,14 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                             else
                                 asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(leader + 8 * buffer) : "memory");
                         }
+                        if (++buffer == S::BUFFERS) buffer = 0, phase ^= 1;
+                        if (b + 1 < p.k_blocks) ok = begin();
                     }
 #pragma unroll
-                    for (int i = 0; i < 32; ++i) sum[c + i] = fmaf(s, v[i], sum[c + i]);
+                    for (int i = 0; i < S::CHUNK; i += 2)
+                        add_scaled(sum[(c * S::CHUNK + i) / 2], s, v[c & 1][i], v[c & 1][i + 1]);
                 }
-                if (++buffer == S::BUFFERS) buffer = 0, phase ^= 1;
-                }
+                if (!ok) break;
             }
             if (!live || !ok) continue;
             T *y = (T *)p.y + row * p.y_stride + col;
@@ -499,12 +546,12 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                 if (p.wide && col + i + V <= p.n) {
                     Pack<T, V> q;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) q.at[j] = from_f32<T>(sum[i + j]);
+                    for (int j = 0; j < V; ++j) q.at[j] = from_f32<T>(half_of(sum[(i + j) / 2], j & 1));
                     *(Pack<T, V> *)(y + i) = q;
                 } else {
 #pragma unroll
                     for (int j = 0; j < V; ++j)
-                        if (col + i + j < p.n) y[i + j] = from_f32<T>(sum[i + j]);
+                        if (col + i + j < p.n) y[i + j] = from_f32<T>(half_of(sum[(i + j) / 2], j & 1));
                 }
             }
         }
