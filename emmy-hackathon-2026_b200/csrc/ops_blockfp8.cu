@@ -75,38 +75,53 @@ struct QuantRowsParams {
 };
 
 /* 16 lanes a block of 128, eight elements each; 1 << across blocks of a row side by side in a block of threads, which
- * takes QUANT_ROWS rows for each of its 16 groups of lanes */
-constexpr int QUANT_ROWS = 2;
-template <typename T> __global__ void __launch_bounds__(256) quantize_rows(QuantRowsParams p) {
+ * takes QUANT_ROWS rows for each of its 16 groups of lanes, all loads before the first use.  WHOLE: every lane's eight
+ * elements are in the row or past it, and allow 16-byte accesses. */
+constexpr int QUANT_ROWS = 4;
+template <typename T, bool WHOLE> __global__ void __launch_bounds__(256) quantize_rows(QuantRowsParams p) {
     enter_grid();
     const int group = threadIdx.x / 16, lane = threadIdx.x & 15, down = 16 >> p.across;
     const int64_t b = ((int64_t)blockIdx.y << p.across) + (group & ((1 << p.across) - 1)), e = b * BLOCK + lane * 8;
     const int64_t first = (int64_t)blockIdx.x * (down * QUANT_ROWS) + (group >> p.across);
-    float v[QUANT_ROWS][8];
+    const int left = (int)min((int64_t)(QUANT_ROWS * 16), p.rows - first);       /* rows from `first` on */
+    const bool in = e < p.cols;
+    constexpr int V = 16 / sizeof(T);
+    Pack<T, V> x[QUANT_ROWS][8 / V];
+    const T *from = (const T *)p.x + first * p.x_stride + e;
 #pragma unroll
-    for (int i = 0; i < QUANT_ROWS; ++i) {
-        const int64_t row = first + i * down;
-        if (row < p.rows)
-            load8((const T *)p.x + row * p.x_stride, e, p.cols, p.wide, v[i]);
-        else
+    for (int i = 0; i < QUANT_ROWS; ++i, from += down * p.x_stride) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) v[i][j] = 0.0f;
+        for (int j = 0; j < 8; ++j) x[i][j / V].at[j % V] = from_f32<T>(0.0f);
+        if (i * down >= left) continue;
+        if (WHOLE) {
+            if (in)
+#pragma unroll
+                for (int j = 0; j < 8 / V; ++j) x[i][j] = *(const Pack<T, V> *)(from + j * V);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+                if (e + j < p.cols) x[i][j / V].at[j % V] = from[j];
+        }
     }
+    float *scale = p.s + b * p.s_stride + first;
+    uint8_t *to = p.q + first * p.q_stride + e;
+    const bool stores = e < ((p.cols + 15) & ~15ll);    /* columns past the end, up to a multiple of 16, become zero */
 #pragma unroll
-    for (int i = 0; i < QUANT_ROWS; ++i) {
-        const int64_t row = first + i * down;
+    for (int i = 0; i < QUANT_ROWS; ++i, to += down * p.q_stride) {
+        float v[8];
         uint32_t largest = 0;
 #pragma unroll
-        for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(v[i][j]));
+        for (int j = 0; j < 8; ++j) {
+            v[j] = to_f32(x[i][j / V].at[j % V]);
+            largest = max(largest, magnitude(v[j]));
+        }
 #pragma unroll
         for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
-        if (row >= p.rows || b * BLOCK >= p.cols) continue;
+        if (i * down >= left || b * BLOCK >= p.cols) continue;
         const float s = scale_of(largest);
-        if (lane == 0) p.s[b * p.s_stride + row] = s;
-        divide8(v[i], s);
-        const uint2 q = make_uint2(e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]), e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7]));
-        /* rows are a multiple of 16 bytes apart: columns past the end, up to there, become zero */
-        if (e < ((p.cols + 15) & ~15ll)) *(uint2 *)(p.q + row * p.q_stride + e) = q;
+        if (lane == 0) scale[i * down] = s;
+        divide8(v, s);
+        if (stores) *(uint2 *)to = make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
     }
 }
 
@@ -266,12 +281,16 @@ __device__ __forceinline__ uint64_t now_ns() {
     asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
     return t;
 }
-/* false when the wait gave up, here or in another role */
-__device__ __forceinline__ bool wait_slowly(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
-    const uint64_t start = now_ns();
-    while (!try_wait(barrier, parity)) {
+/* False when the wait gave up, here or in another role.  The timer is looked at in every 64th try only: most waits here
+ * are for one block's product, and reading it is slow. */
+__device__ __forceinline__ bool wait_for(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
+    uint64_t start = 0;
+    for (unsigned tries = 0; !try_wait(barrier, parity); ++tries) {
+        if ((tries & 63) != 63) continue;
         if (*abort) return false;
-        if (now_ns() - start > TIMEOUT_NS) {
+        const uint64_t now = now_ns();
+        if (!start) start = now;
+        if (now - start > TIMEOUT_NS) {
             *abort = 1;
             atomicOr(status, role);
             return false;
@@ -279,9 +298,17 @@ __device__ __forceinline__ bool wait_slowly(uint32_t barrier, uint32_t parity, v
     }
     return true;
 }
-__device__ __forceinline__ bool wait_for(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
-    if (try_wait(barrier, parity)) return true;
-    return wait_slowly(barrier, parity, abort, status, role);
+
+/* both barriers, tried together first: a try takes tens of cycles, and one thread issues all products */
+__device__ __forceinline__ bool wait_for_both(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, volatile unsigned *abort,
+                                              unsigned *status, unsigned role) {
+    uint32_t ok;
+    asm volatile("{\n.reg .pred p, q;\n"
+                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
+                 "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n"
+                 "and.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}"
+                 : "=r"(ok) : "r"(a), "r"(a_parity), "r"(b), "r"(b_parity) : "memory");
+    return ok || (wait_for(a, a_parity, abort, status, role) && wait_for(b, b_parity, abort, status, role));
 }
 
 struct TensorMap {
@@ -297,14 +324,27 @@ __device__ __forceinline__ void tma_load(uint32_t to, const TensorMap *map, int 
         asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
                      ::"r"(to), "l"(map), "r"(x), "r"(y), "r"(barrier) : "memory");
 }
-template <bool PAIR>
-__device__ __forceinline__ void multiply(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool add) {
+/* A block's product: four steps of 32 bytes along the rows.  Operands are K-major rows of 128 bytes with the 128-byte
+ * swizzle, eight rows 1024 bytes apart: the descriptors differ in the low words (address / 16) alone. */
+template <bool PAIR> __device__ __forceinline__ void multiply_block(uint32_t d, uint32_t a, uint32_t b, uint32_t idesc) {
+    constexpr uint32_t HIGH = (1024u >> 4) | (1u << 14) | (2u << 29);
+#define EMMY_STEPS(CG)                                                                                                  \
+    asm volatile("{\n.reg .pred first, later;\n.reg .b32 x, y;\n.reg .b64 u, v;\n"                                        \
+                 "setp.ne.u32 first, %3, %3;\nsetp.eq.u32 later, %3, %3;\n"                                              \
+                 "mov.b64 u, {%1, %4};\nmov.b64 v, {%2, %4};\n"                                                           \
+                 "tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%0], u, v, %3, first;\n"                                    \
+                 "add.u32 x, %1, 2;\nadd.u32 y, %2, 2;\nmov.b64 u, {x, %4};\nmov.b64 v, {y, %4};\n"                       \
+                 "tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%0], u, v, %3, later;\n"                                    \
+                 "add.u32 x, %1, 4;\nadd.u32 y, %2, 4;\nmov.b64 u, {x, %4};\nmov.b64 v, {y, %4};\n"                       \
+                 "tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%0], u, v, %3, later;\n"                                    \
+                 "add.u32 x, %1, 6;\nadd.u32 y, %2, 6;\nmov.b64 u, {x, %4};\nmov.b64 v, {y, %4};\n"                       \
+                 "tcgen05.mma.cta_group::" CG ".kind::f8f6f4 [%0], u, v, %3, later;\n}"                                   \
+                 ::"r"(d), "r"(a), "r"(b), "r"(idesc), "r"(HIGH) : "memory")
     if (PAIR)
-        asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::2.kind::f8f6f4 [%0], %1, %2, %3, q;\n}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+        EMMY_STEPS("2");
     else
-        asm volatile("{\n.reg .pred q;\nsetp.ne.u32 q, %4, 0;\ntcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, q;\n}"
-                     ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"((uint32_t)add) : "memory");
+        EMMY_STEPS("1");
+#undef EMMY_STEPS
 }
 template <bool PAIR> __device__ __forceinline__ void commit(uint32_t barrier) {
     if (PAIR)
@@ -313,10 +353,6 @@ template <bool PAIR> __device__ __forceinline__ void commit(uint32_t barrier) {
                      ::"r"(barrier) : "memory");
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
-}
-/* K-major rows of 128 bytes, 128-byte swizzle, eight rows 1024 bytes apart */
-__device__ __forceinline__ uint64_t operand(uint32_t address) {
-    return (uint64_t)((1024u >> 4) | (1u << 14) | (2u << 29)) << 32 | (1u << 16) | ((address & 0x3ffff) >> 4);
 }
 __device__ __forceinline__ void tensor_load(uint32_t address, uint32_t (&u)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
@@ -373,7 +409,8 @@ template <int BN, bool PAIR> struct ManyShape {
     static constexpr int CHUNK = PER >= 64 ? 32 : 16, CHUNKS = PER / CHUNK;   /* columns a load of tensor memory */
     static constexpr int THREADS = 128 + 32 * SCALE_WARPS;
     static constexpr bool SPLIT = PER == 128;     /* the scaling warps need more registers than an even share */
-    static constexpr int SMEM = STAGES * STAGE + 1024;
+    static constexpr int STORE_ROW = 80;           /* 64 bytes of a row of y, and 16 that keep its neighbours in other banks */
+    static constexpr int SMEM = STAGES * STAGE + 1024 + SCALE_WARPS * 32 * STORE_ROW;
 };
 
 template <typename T, int BN, bool PAIR>
@@ -453,20 +490,19 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
     } else if (warp == 1) {
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = 1u << 4 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(S::ROWS >> 4) << 24;
+            const uint32_t full0 = shared_address(&full[0]), empty0 = shared_address(&empty[0]);
+            const uint32_t summed0 = shared_address(&summed[0]), read0 = shared_address(&read[0]);
+            const uint32_t a0 = (1u << 16) | ring >> 4, b0 = a0 + (S::A_BYTES >> 4);
             int stage = 0, buffer = 0;
             uint32_t phase = 0, buffer_phase = 0;
             bool ok = true;
             for (int t = worker; t < tiles && ok; t += workers)
                 for (int b = 0; b < p.k_blocks; ++b) {
-                    if (!(ok = wait_for(shared_address(&read[buffer]), buffer_phase ^ 1, &abort, p.status, 2))) break;
-                    if (!(ok = wait_for(shared_address(&full[stage]), phase, &abort, p.status, 2))) break;
+                    if (!(ok = wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    const uint32_t a = ring + stage * S::STAGE;
-#pragma unroll
-                    for (int i = 0; i < BLOCK / 32; ++i)
-                        multiply<PAIR>(base + buffer * BN, operand(a + 32 * i), operand(a + S::A_BYTES + 32 * i), idesc, i > 0);
-                    commit<PAIR>(shared_address(&empty[stage]));
-                    commit<PAIR>(shared_address(&summed[buffer]));
+                    multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
+                    commit<PAIR>(summed0 + 8 * buffer);
+                    commit<PAIR>(empty0 + 8 * stage);
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                     if (++buffer == S::BUFFERS) buffer = 0, buffer_phase ^= 1;
                 }
@@ -538,21 +574,38 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                 }
                 if (!ok) break;
             }
-            if (!live || !ok) continue;
-            T *y = (T *)p.y + row * p.y_stride + col;
-            constexpr int V = 16 / sizeof(T);
+            if (!ok) continue;
+            /* 64 bytes of 32 rows at a time through shared memory, so that a store has whole sectors of a row */
+            constexpr int V = 16 / sizeof(T), WIDE = 64 / sizeof(T);
+            unsigned char *const rows = raw + (ring - shared_address(raw)) + S::STAGES * S::STAGE + (warp - 4) * 32 * S::STORE_ROW;
+            const int row0 = row - lane;
 #pragma unroll
-            for (int i = 0; i < S::PER; i += V) {
-                if (p.wide && col + i + V <= p.n) {
+            for (int c = 0; c < S::PER; c += WIDE) {
+#pragma unroll
+                for (int i = 0; i < WIDE; i += V) {
                     Pack<T, V> q;
 #pragma unroll
-                    for (int j = 0; j < V; ++j) q.at[j] = from_f32<T>(half_of(sum[(i + j) / 2], j & 1));
-                    *(Pack<T, V> *)(y + i) = q;
-                } else {
-#pragma unroll
-                    for (int j = 0; j < V; ++j)
-                        if (col + i + j < p.n) y[i + j] = from_f32<T>(half_of(sum[(i + j) / 2], j & 1));
+                    for (int j = 0; j < V; ++j) q.at[j] = from_f32<T>(half_of(sum[(c + i + j) / 2], j & 1));
+                    *(Pack<T, V> *)(rows + lane * S::STORE_ROW + i * sizeof(T)) = q;
                 }
+                __syncwarp();
+                if (p.wide && col + c + WIDE <= p.n) {
+                    const int piece = lane & 3;
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int at = 8 * i + (lane >> 2);
+                        if (row0 + at < p.m)
+                            *(Pack<T, V> *)((T *)p.y + (row0 + at) * p.y_stride + col + c + piece * V) =
+                                *(const Pack<T, V> *)(rows + at * S::STORE_ROW + piece * 16);
+                    }
+                } else {
+                    constexpr int AT_ONCE = 32 / WIDE;
+                    const int e = lane % WIDE;
+                    if (col + c + e < p.n)
+                        for (int at = lane / WIDE; at < 32 && row0 + at < p.m; at += AT_ONCE)
+                            ((T *)p.y)[(row0 + at) * p.y_stride + col + c + e] = *(const T *)(rows + at * S::STORE_ROW + e * sizeof(T));
+                }
+                __syncwarp();
             }
         }
     }
@@ -626,12 +679,25 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
     p.wide = aligned(a->y, 16) && a->y_stride * sizeof(T) % 16 == 0;
     int sms;
     if (int e = ops_sm_count(device, &sms)) return e;
-    /* the widest tiles that still give every SM one */
-    const int64_t rows = (a->m + 127) / 128;
-    if (a->m > 128 && ((a->m + 255) / 256) * ((a->n + 255) / 256) * 2 >= sms) return go_many<T, 256, true>(a, p, device, stream);
-    if (rows * ((a->n + 127) / 128) >= sms) return go_many<T, 128, false>(a, p, device, stream);
-    if (rows * ((a->n + 63) / 64) >= sms) return go_many<T, 64, false>(a, p, device, stream);
-    return go_many<T, 32, false>(a, p, device, stream);
+    /* The tiles whose rounds take least.  A block of 128 columns takes a tile 730 cycles (32 columns wide) to 1050 (256, on
+     * pairs of SMs), measured at k = 8192 with one tile an SM: the wider the tile, the less a column costs, as long
+     * as there are tiles for all SMs. */
+    const int64_t rows = (a->m + 127) / 128, pairs = (a->m + 255) / 256;
+    auto rounds = [&](int64_t tiles, int workers) { return (tiles + workers - 1) / workers; };
+    const struct { int which; int64_t cost; } choices[] = {
+        {0, rounds(rows * ((a->n + 31) / 32), sms) * 730},
+        {1, rounds(rows * ((a->n + 63) / 64), sms) * 760},
+        {2, rounds(rows * ((a->n + 127) / 128), sms) * 880},
+        {3, rounds(pairs * ((a->n + 255) / 256), sms / 2) * 1050}};
+    int best = 0;
+    for (int i = 1; i < (rows > 1 ? 4 : 3); ++i)
+        if (choices[i].cost < choices[best].cost) best = i;
+    switch (best) {
+    case 0: return go_many<T, 32, false>(a, p, device, stream);
+    case 1: return go_many<T, 64, false>(a, p, device, stream);
+    case 2: return go_many<T, 128, false>(a, p, device, stream);
+    default: return go_many<T, 256, true>(a, p, device, stream);
+    }
 }
 
 int check_matrix(const char *name, uint64_t at, int64_t rows, int64_t cols, int64_t stride, int size, int multiple) {
@@ -677,9 +743,10 @@ EMMY_EXPORT int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args
         QuantRowsParams p = {(const char *)(uintptr_t)a->x, (uint8_t *)(uintptr_t)a->q, (float *)(uintptr_t)a->s, a->rows, a->cols,
                              a->x_stride, a->q_stride, a->s_stride, wide, across};
         const dim3 grid((unsigned)((a->rows + down - 1) / down), (unsigned)tall);
-        e = a->dtype == EMMY_OPS_F32   ? launch(quantize_rows<float>, grid, dim3(256), 0, stream, p)
-            : a->dtype == EMMY_OPS_F16 ? launch(quantize_rows<__half>, grid, dim3(256), 0, stream, p)
-                                       : launch(quantize_rows<__nv_bfloat16>, grid, dim3(256), 0, stream, p);
+        auto go = [&](auto whole, auto parts) { return launch(wide && a->cols % 8 == 0 ? whole : parts, grid, dim3(256), 0, stream, p); };
+        e = a->dtype == EMMY_OPS_F32   ? go(quantize_rows<float, true>, quantize_rows<float, false>)
+            : a->dtype == EMMY_OPS_F16 ? go(quantize_rows<__half, true>, quantize_rows<__half, false>)
+                                       : go(quantize_rows<__nv_bfloat16, true>, quantize_rows<__nv_bfloat16, false>);
     }
     return ops_cuda(e, "FP8 quantisation");
 }
