@@ -261,10 +261,10 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) few_rows(Fe
 constexpr uint64_t TIMEOUT_NS = 2000000000ull;
 
 struct ManyParams {
-    const float *sx, *sw;
+    const float *sw;
     char *y;
     unsigned *status;
-    int64_t sx_stride, sw_stride, y_stride;
+    int64_t sw_stride, y_stride;
     int m, n, k_blocks, m_tiles, n_tiles, wide;
 };
 
@@ -403,6 +403,10 @@ template <int BN, bool PAIR> struct ManyShape {
     static constexpr int A_BYTES = 128 * BLOCK, B_BYTES = B_ROWS * BLOCK, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = STAGE > 40960 ? 4 : STAGE >= 32768 ? 6 : 8;
     static constexpr int BUFFERS = 512 / BN > 4 ? 4 : 512 / BN;
+    /* The copies are at most STAGES blocks ahead of the products, and these BUFFERS ahead of the scaling: a place that many
+     * and one more blocks on is free without a barrier of its own. */
+    static constexpr int SCALES = 16;
+    static_assert(STAGES + BUFFERS < SCALES, "the scales' ring");
     static constexpr int COLUMNS = BN * BUFFERS < 32 ? 32 : BN * BUFFERS;
     static constexpr int SCALE_WARPS = BN >= 128 ? 8 : 4;
     static constexpr int PER = BN / (SCALE_WARPS / 4);                /* columns a scaling thread */
@@ -415,10 +419,12 @@ template <int BN, bool PAIR> struct ManyShape {
 
 template <typename T, int BN, bool PAIR>
 __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
-    many_rows(const __grid_constant__ TensorMap x_map, const __grid_constant__ TensorMap w_map, ManyParams p) {
+    many_rows(const __grid_constant__ TensorMap x_map, const __grid_constant__ TensorMap w_map,
+              const __grid_constant__ TensorMap s_map, ManyParams p) {
     using S = ManyShape<BN, PAIR>;
     extern __shared__ unsigned char raw[];
     __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS];
+    __shared__ alignas(128) float scales[S::SCALES][128];      /* of x: a block's 128 rows, copied with its operands */
     __shared__ uint32_t tensor_base;
     __shared__ volatile unsigned abort;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -468,7 +474,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         if (lane == 0) {
             uint32_t leader = shared_address(&full[0]);
             if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(leader));
-            int stage = 0;
+            int stage = 0, slot = -1;
             uint32_t phase = 0;
             bool ok = true;
             for (int t = worker; t < tiles && ok; t += workers) {
@@ -477,35 +483,40 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                 if (PAIR) m0 += 128 * rank, n0 += S::B_ROWS * rank;
                 for (int b = 0; b < p.k_blocks; ++b) {
                     if (!(ok = wait_for(shared_address(&empty[stage]), phase ^ 1, &abort, p.status, 1))) break;
+                    if (++slot == S::SCALES) slot = 0;
                     if (rank == 0)      /* both copies of a pair complete on the leader's barrier */
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
-                                     ::"r"(shared_address(&full[stage])), "r"(S::STAGE * (PAIR ? 2 : 1)) : "memory");
+                                     ::"r"(shared_address(&full[stage])), "r"((S::STAGE + 512) * (PAIR ? 2 : 1)) : "memory");
                     const uint32_t to = ring + stage * S::STAGE, barrier = leader + 8 * stage;
                     tma_load<PAIR>(to, &x_map, b * BLOCK, m0, barrier);
                     tma_load<PAIR>(to + S::A_BYTES, &w_map, b * BLOCK, n0, barrier);
+                    tma_load<PAIR>(shared_address(scales[slot]), &s_map, m0, b, barrier);
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
             }
         }
-    } else if (warp == 1) {
+    } else if (warp == 1 || warp == 3) {
+        /* Two threads issue the products, every other block each: issuing one takes a thread longer than the tensor core
+         * takes to run it. */
         if (lane == 0 && rank == 0) {
             constexpr uint32_t idesc = 1u << 4 | (uint32_t)(BN >> 3) << 17 | (uint32_t)(S::ROWS >> 4) << 24;
             const uint32_t full0 = shared_address(&full[0]), empty0 = shared_address(&empty[0]);
             const uint32_t summed0 = shared_address(&summed[0]), read0 = shared_address(&read[0]);
             const uint32_t a0 = (1u << 16) | ring >> 4, b0 = a0 + (S::A_BYTES >> 4);
-            int stage = 0, buffer = 0;
+            const int own = worker < tiles ? (tiles - worker + workers - 1) / workers : 0;      /* tiles of this worker */
+            const int64_t blocks = (int64_t)own * p.k_blocks;
+            int stage = warp >> 1, buffer = warp >> 1;
             uint32_t phase = 0, buffer_phase = 0;
-            bool ok = true;
-            for (int t = worker; t < tiles && ok; t += workers)
-                for (int b = 0; b < p.k_blocks; ++b) {
-                    if (!(ok = wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2))) break;
-                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                    multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
-                    commit<PAIR>(summed0 + 8 * buffer);
-                    commit<PAIR>(empty0 + 8 * stage);
-                    if (++stage == S::STAGES) stage = 0, phase ^= 1;
-                    if (++buffer == S::BUFFERS) buffer = 0, buffer_phase ^= 1;
-                }
+            static_assert(S::STAGES % 2 == 0 && S::BUFFERS % 2 == 0, "every other stage and buffer");
+            for (int64_t i = warp >> 1; i < blocks; i += 2) {
+                if (!wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2)) break;
+                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
+                commit<PAIR>(summed0 + 8 * buffer);
+                commit<PAIR>(empty0 + 8 * stage);
+                if ((stage += 2) >= S::STAGES) stage -= S::STAGES, phase ^= 1;
+                if ((buffer += 2) >= S::BUFFERS) buffer -= S::BUFFERS, buffer_phase ^= 1;
+            }
         }
     } else if (warp >= 4) {
         if (S::SPLIT) asm volatile("setmaxnreg.inc.sync.aligned.u32 232;");      /* 256 of them, and 128 with 40: 384 of 168 */
@@ -513,23 +524,18 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         const uint32_t mine = base + (uint32_t)(quarter * 32) * 65536 + half * S::PER;
         uint32_t leader = shared_address(&read[0]);
         if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(leader));
-        int buffer = 0;
+        int buffer = 0, slot = 0;
         uint32_t phase = 0;
         bool ok = true;
         for (int t = worker; t < tiles && ok; t += workers) {
             int m0, n0;
             place(t, m0, n0);
             const int row = m0 + 128 * rank + 32 * quarter + lane, col = n0 + half * S::PER;
-            const float *sx = p.sx + row, *sw = p.sw + (int64_t)(min(col, p.n - 1) / BLOCK) * p.sw_stride;
-            const bool live = row < p.m;
+            const float *sw = p.sw + (int64_t)(min(col, p.n - 1) / BLOCK) * p.sw_stride;
             uint64_t sum[S::PER / 2];
 #pragma unroll
             for (int i = 0; i < S::PER / 2; ++i) sum[i] = 0;
-            /* scales are fetched four blocks ahead of their use, which hides their way from L2 */
-            float ahead[4], now[4];
-            auto fetch = [&](int b, int i) { ahead[i] = live && b + i < p.k_blocks ? sx[(b + i) * p.sx_stride] * sw[b + i] : 0.0f; };
-#pragma unroll
-            for (int i = 0; i < 4; ++i) fetch(0, i);
+            float next_w = *sw;
             /* a load of tensor memory is under way while the one before it is added, from block to block too */
             uint32_t v[2][S::CHUNK];
             auto begin = [&] {
@@ -541,13 +547,9 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             if (!(ok = begin())) continue;
 #pragma unroll 1
             for (int b = 0; b < p.k_blocks; ++b) {
-                if ((b & 3) == 0) {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) now[i] = ahead[i];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) fetch(b + 4, i);
-                }
-                const float one = (b & 2) ? ((b & 1) ? now[3] : now[2]) : ((b & 1) ? now[1] : now[0]);
+                const float one = next_w * scales[slot][32 * quarter + lane];
+                if (b + 1 < p.k_blocks) next_w = sw[b + 1];
+                slot = slot + 1 == S::SCALES ? 0 : slot + 1;
                 uint64_t s;
                 asm("mov.b64 %0, {%1, %1};" : "=l"(s) : "f"(one));
 #pragma unroll
@@ -622,11 +624,11 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
     }
 }
 
-int encode(TensorMap *map, uint64_t at, int64_t cols, int64_t rows, int64_t stride, int box_rows) {
+int encode(TensorMap *map, uint64_t at, int64_t cols, int64_t rows, int64_t stride, int box_rows, bool scales = false) {
     const uint64_t dims[2] = {(uint64_t)cols, (uint64_t)rows}, strides[1] = {(uint64_t)stride};
     const unsigned box[2] = {BLOCK, (unsigned)box_rows}, steps[2] = {1, 1};
-    /* bytes, no interleave, 128-byte swizzle, 256-byte L2 promotion, zeros outside */
-    if (int e = emmy_rt_tensor_map_encode_tiled(map, 0, 2, at, dims, strides, box, steps, 0, 3, 3, 0))
+    /* bytes with the 128-byte swizzle, or f32 without one; no interleave, 256-byte L2 promotion, zeros outside */
+    if (int e = emmy_rt_tensor_map_encode_tiled(map, scales ? 7 : 0, 2, at, dims, strides, box, steps, 0, scales ? 0 : 3, 3, 0))
         return ops_fail(e, "tensor map: %s", emmy_rt_last_error());
     return 0;
 }
@@ -639,9 +641,10 @@ template <typename T, int BN, bool PAIR> int go_many(const emmy_ops_blockfp8_arg
         if (e != cudaSuccess) return ops_cuda(e, "shared memory of the FP8 product");
         __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
     }
-    TensorMap x, w;
+    TensorMap x, w, scales;
     if (int e = encode(&x, a->xq, a->k, a->m, a->xq_stride, 128)) return e;
     if (int e = encode(&w, a->wq, a->k, a->n, a->wq_stride, S::B_ROWS)) return e;
+    if (int e = encode(&scales, a->xs, a->m, (a->k + BLOCK - 1) / BLOCK, a->xs_stride * 4, 1, true)) return e;
     int sms;
     if (int e = ops_sm_count(device, &sms)) return e;
     p.m_tiles = (int)((a->m + S::ROWS - 1) / S::ROWS);
@@ -657,7 +660,7 @@ template <typename T, int BN, bool PAIR> int go_many(const emmy_ops_blockfp8_arg
     attributes[1].id = cudaLaunchAttributeClusterDimension;
     attributes[1].val.clusterDim.x = PAIR ? 2 : 1, attributes[1].val.clusterDim.y = attributes[1].val.clusterDim.z = 1;
     cfg.attrs = attributes, cfg.numAttrs = 2;
-    return ops_cuda(cudaLaunchKernelEx(&cfg, many_rows<T, BN, PAIR>, x, w, p), "FP8 product");
+    return ops_cuda(cudaLaunchKernelEx(&cfg, many_rows<T, BN, PAIR>, x, w, scales, p), "FP8 product");
 }
 
 template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, uint64_t stream) {
@@ -672,9 +675,9 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
         return ops_cuda(e, "FP8 product of few rows");
     }
     ManyParams p = {};
-    p.sx = (const float *)(uintptr_t)a->xs, p.sw = (const float *)(uintptr_t)a->ws, p.y = (char *)(uintptr_t)a->y;
+    p.sw = (const float *)(uintptr_t)a->ws, p.y = (char *)(uintptr_t)a->y;
     p.status = (unsigned *)(uintptr_t)a->status;
-    p.sx_stride = a->xs_stride, p.sw_stride = a->ws_stride, p.y_stride = a->y_stride;
+    p.sw_stride = a->ws_stride, p.y_stride = a->y_stride;
     p.m = (int)a->m, p.n = (int)a->n, p.k_blocks = (int)((a->k + BLOCK - 1) / BLOCK);
     p.wide = aligned(a->y, 16) && a->y_stride * sizeof(T) % 16 == 0;
     int sms;
@@ -761,7 +764,8 @@ EMMY_EXPORT int emmy_ops_blockfp8_product(const emmy_ops_blockfp8_args *a, int d
     if (int e = check_matrix("wq", a->wq, a->n, a->k, a->wq_stride, 1, 16)) return e;
     if (a->xq_stride < (a->k + 15) / 16 * 16 || a->wq_stride < (a->k + 15) / 16 * 16)
         return ops_fail(EMMY_RT_EINVAL, "rows of xq and wq are not padded to 16 bytes");
-    if (int e = check_matrix("xs", a->m ? a->xs : 16, k_blocks, a->m > 0 ? a->m : 1, a->xs_stride, 4, 1)) return e;
+    if (int e = check_matrix("xs", a->m ? a->xs : 16, k_blocks, a->m > 0 ? a->m : 1, a->xs_stride, 4, 4)) return e;
+    if (a->xs_stride < 4) return ops_fail(EMMY_RT_EINVAL, "rows of xs are %lld apart", (long long)a->xs_stride);
     if (int e = check_matrix("ws", a->ws, n_blocks, k_blocks, a->ws_stride, 4, 1)) return e;
     if (int e = check_matrix("y", a->m ? a->y : 16, a->m, a->n, a->y_stride, es, 1)) return e;
     if (!a->status || !aligned(a->status, 4)) return ops_fail(EMMY_RT_EINVAL, "a status word is needed");

@@ -93,7 +93,8 @@ class BlockFp8Linear(Operator):
         self.max_rows = int(max_rows)
         # the quantised x, its scales and the status word
         x_bytes = -(-self.max_rows * pitch(self.k) // 256) * 256
-        s_bytes = -(-blocks(self.k) * self.max_rows * 4 // 256) * 256
+        self._xs_stride = -(-self.max_rows // 4) * 4
+        s_bytes = -(-blocks(self.k) * self._xs_stride * 4 // 256) * 256
         self._workspace = DeviceBuffer(x_bytes + s_bytes + 256)
         at = self._workspace.ptr
         self._xq, self._xs, self._status = at, at + x_bytes, at + x_bytes + s_bytes
@@ -145,7 +146,7 @@ class BlockFp8Linear(Operator):
         if rows > self.max_rows:
             raise ValueError(f"{rows} rows, the operator was made for {self.max_rows}")
         y = written(shaped(operand(operands[1], "y", FLOATS, 2, d), "y", (rows, self.n)), "y")
-        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, xq_stride=pitch(self.k), xs_stride=self.max_rows,
+        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
                                wq_stride=_stride(self.wq), ws_stride=self.ws.strides[0], y_stride=y.strides[0], m=rows,
                                n=self.n, k=self.k, dtype=CODE[y.dtype], x_stride=x.strides[0], x_dtype=CODE[x.dtype])
         checks = overlaps([(1, y, "y")], [(0, x, "x"), (2, self.wq, "wq"), (3, self.ws, "ws")])

@@ -103,7 +103,8 @@ typedef struct {
 int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args *a, int device, uint64_t stream);
 
 /* y[m, n] = sum over blocks b of xs[b, m] ws[n / 128, b] sum over k in b of xq[m, k] wq[n, k], in
- * f32, as quantised above (xq without square, its padding zero; wq with).  *status (a word of
+ * f32, as quantised above (xq without square, its padding zero, rows of xs a multiple of 4 apart; wq
+ * with).  *status (a word of
  * device memory, zeroed by the caller once) gets a bit when a wait inside the kernel gave
  * up after 2 s; y is then not valid. */
 typedef struct {
