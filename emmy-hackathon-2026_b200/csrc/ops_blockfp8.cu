@@ -25,9 +25,26 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 /* |v| as an ordered integer: a NaN is the largest */
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+/* largest / 448, correctly rounded (as divide8 below); 1 where that is 0 */
 __device__ __forceinline__ float scale_of(uint32_t largest) {
-    const float s = __fdiv_rn(__uint_as_float(largest), E4M3_MAX);
+    const float a = __uint_as_float(largest);
+    constexpr float R = 1.0f / E4M3_MAX;
+    if (a >= 0x1p-60f && a <= 0x1p100f) {
+        const float q = a * R;
+        return fmaf(fmaf(-E4M3_MAX, q, a), R, q);
+    }
+    const float s = __fdiv_rn(a, E4M3_MAX);
     return s == 0.0f ? 1.0f : s;
+}
+/* of two 16-bit floats side by side: the larger magnitudes, each in its half */
+__device__ __forceinline__ uint32_t larger2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+template <typename T> __device__ __forceinline__ uint32_t largest_of(uint32_t two) {       /* as f32 bits */
+    const uint32_t one = max(two & 0xffff, two >> 16);
+    return sizeof(T) == 4 ? two : __float_as_uint(to_f32(*(const T *)&one));
 }
 
 template <typename T> __device__ __forceinline__ void load8(const T *x, int64_t e, int64_t end, bool wide, float (&v)[8]) {
@@ -110,13 +127,20 @@ template <typename T, bool WHOLE> __global__ void __launch_bounds__(256) quantiz
     for (int i = 0; i < QUANT_ROWS; ++i, to += down * p.q_stride) {
         float v[8];
         uint32_t largest = 0;
+        if (sizeof(T) == 2) {
+            const uint32_t *two = (const uint32_t *)&x[i][0];
+            largest = larger2(larger2(two[0] & 0x7fff7fff, two[1] & 0x7fff7fff), larger2(two[2] & 0x7fff7fff, two[3] & 0x7fff7fff));
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            v[j] = to_f32(x[i][j / V].at[j % V]);
-            largest = max(largest, magnitude(v[j]));
+            for (int d = 8; d > 0; d >>= 1) largest = larger2(largest, __shfl_xor_sync(~0u, largest, d));
+            largest = largest_of<T>(largest);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(to_f32(x[i][j / V].at[j % V])));
+#pragma unroll
+            for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
         }
 #pragma unroll
-        for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
+        for (int j = 0; j < 8; ++j) v[j] = to_f32(x[i][j / V].at[j % V]);
         if (i * down >= left || b * BLOCK >= p.cols) continue;
         const float s = scale_of(largest);
         if (lane == 0) scale[i * down] = s;
@@ -178,7 +202,7 @@ struct FewParams {
     const float *sx, *sw;
     char *y;
     int64_t x_stride, w_stride, sx_stride, sw_stride, y_stride;
-    int m, n, k;
+    int m, n, k, stages;
 };
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -187,55 +211,89 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-/* 16 bytes of a row at byte k, zero from `end` on */
-__device__ __forceinline__ uint4 row16(const uint8_t *row, int k, int end) {
-    if (k + 16 <= end) return *(const uint4 *)(row + k);
-    uint32_t v[4] = {0, 0, 0, 0};
-    for (int i = 0; k + i < end; ++i) v[i >> 2] |= (uint32_t)row[k + i] << 8 * (i & 3);
-    return make_uint4(v[0], v[1], v[2], v[3]);
+/* 16 rows of W a block of threads; its 8 warps take every eighth block of 128 columns and join at the end.  W and x come
+ * through a ring of asynchronous copies in shared memory, FEW_STAGES blocks of a warp ahead: what is under way decides the rate
+ * at so little work a byte, and registers for it would halve what runs at once.  A thread takes 16 consecutive bytes of a row;
+ * the order of the columns inside a product is the same for x and W, and free.  W's bytes bound it, and at more than
+ * 4 rows the conversions of e4m3 that mma.sync is made of here. */
+constexpr int FEW_WARPS = 8;
+template <int NT> struct alignas(16) FewStage {
+    unsigned char w[16][BLOCK], x[8 * NT][BLOCK];
+    float sx[8 * NT], sw, unused[3];
+};
+constexpr int FEW_STAGES = 3;        /* two or three blocks of threads an SM; 1 x 4096 x 14336: 16.0 us, 22.1 with two stages, 16.4 with four */
+
+__device__ __forceinline__ void copy_async16(const void *shared, const void *from, int bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;"
+                 ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(from), "r"(bytes) : "memory");
 }
 
-/* 16 rows of W a block of threads; its 8 warps take every eighth block of 128 columns and join at the end.  A thread loads
- * 16 consecutive bytes of a row; the order of the columns inside a product is the same for x and W, and free. */
 template <typename T, int NT> __global__ void __launch_bounds__(256) few_rows(FewParams p) {
-    constexpr int WARPS = 8;
-    __shared__ float parts[WARPS][16][8 * NT + 1];
+    constexpr int STAGES = FEW_STAGES;
+    extern __shared__ __align__(128) unsigned char raw[];           /* [warps][stages] */
+    __shared__ float parts[FEW_WARPS][16][8 * NT + 1];
     enter_grid();
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, r = lane >> 2, c = lane & 3;
-    const int n0 = blockIdx.x * 16, blocks = (p.k + BLOCK - 1) / BLOCK;
-    const uint8_t *w0 = p.w + (int64_t)min(n0 + r, p.n - 1) * p.w_stride, *w1 = p.w + (int64_t)min(n0 + r + 8, p.n - 1) * p.w_stride;
+    const int n0 = blockIdx.x * 16, blocks = (p.k + BLOCK - 1) / BLOCK, steps = (blocks - warp + FEW_WARPS - 1) / FEW_WARPS;
+    FewStage<NT> *const ring = (FewStage<NT> *)raw + warp * p.stages;
+    /* A copy of the warp has four rows' 128 bytes; the 16 bytes `piece` of a row lie at a place that depends on the row's
+     * parity, as the reads below take two rows' halves at a time. */
+    const int down = lane >> 3, piece = lane & 7, place = (piece ^ ((down & 1) * 4)) * 16;
+    const uint8_t *w_row[4], *x_row[2 * NT];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w_row[i] = p.w + (int64_t)min(n0 + down + 4 * i, p.n - 1) * p.w_stride;
+#pragma unroll
+    for (int i = 0; i < 2 * NT; ++i) x_row[i] = p.x + (int64_t)min(down + 4 * i, p.m - 1) * p.x_stride;
+    const float *sw = p.sw + (n0 / BLOCK) * p.sw_stride;
+    auto issue = [&](int step, int stage) {
+        if (step < steps) {
+            FewStage<NT> &s = ring[stage];
+            const int b = warp + FEW_WARPS * step, k = b * BLOCK + piece * 16, bytes = max(0, min(16, p.k - k)), at = bytes ? k : 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) copy_async16(&s.w[down + 4 * i][place], w_row[i] + at, bytes);
+#pragma unroll
+            for (int i = 0; i < 2 * NT; ++i) copy_async16(&s.x[down + 4 * i][place], x_row[i] + at, down + 4 * i < p.m ? bytes : 0);
+            if (lane < 2 * NT) {
+                const int rest = max(0, min(4, p.m - 4 * lane));
+                copy_async16(&s.sx[4 * lane], p.sx + b * p.sx_stride + (rest ? 4 * lane : 0), 4 * rest);
+            } else if (lane == 31) {
+                asm volatile("cp.async.ca.shared.global [%0], [%1], 4;"
+                             ::"r"((uint32_t)__cvta_generic_to_shared(&s.sw)), "l"(sw + b) : "memory");
+            }
+        }
+        asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    for (int i = 0; i < p.stages; ++i) issue(i, i);
     float acc[NT][4];
 #pragma unroll
     for (int t = 0; t < NT; ++t)
 #pragma unroll
         for (int i = 0; i < 4; ++i) acc[t][i] = 0.0f;
-#pragma unroll 2
-    for (int b = warp; b < blocks; b += WARPS) {
-        const int k = b * BLOCK + 16 * c;
-        const uint4 a0 = row16(w0, k, p.k), a1 = row16(w1, k, p.k), a2 = row16(w0, k + 64, p.k), a3 = row16(w1, k + 64, p.k);
-        const float sw = p.sw[(n0 / BLOCK) * p.sw_stride + b];
+    const int low = (c ^ ((r & 1) * 4)) * 16, high = ((c + 4) ^ ((r & 1) * 4)) * 16;
+    for (int step = 0, stage = 0; step < steps; ++step) {
+        if (p.stages == STAGES)
+            asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+        else
+            asm volatile("cp.async.wait_all;" ::: "memory");
+        __syncwarp();
+        const FewStage<NT> &s = ring[stage];
+        const uint4 a0 = *(const uint4 *)&s.w[r][low], a1 = *(const uint4 *)&s.w[r + 8][low];
+        const uint4 a2 = *(const uint4 *)&s.w[r][high], a3 = *(const uint4 *)&s.w[r + 8][high];
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            const int row = 8 * t + r;
-            uint4 x0 = make_uint4(0, 0, 0, 0), x1 = x0;
-            if (row < p.m) {
-                const uint8_t *x = p.x + row * p.x_stride;
-                if (k < p.k) x0 = *(const uint4 *)(x + k);
-                if (k + 64 < p.k) x1 = *(const uint4 *)(x + k + 64);
-            }
+            const uint4 x0 = *(const uint4 *)&s.x[8 * t + r][low], x1 = *(const uint4 *)&s.x[8 * t + r][high];
             float d[4] = {0.0f, 0.0f, 0.0f, 0.0f};
             mma_e4m3(d, a0.x, a1.x, a0.y, a1.y, x0.x, x0.y);
             mma_e4m3(d, a0.z, a1.z, a0.w, a1.w, x0.z, x0.w);
             mma_e4m3(d, a2.x, a3.x, a2.y, a3.y, x1.x, x1.y);
             mma_e4m3(d, a2.z, a3.z, a2.w, a3.w, x1.z, x1.w);
+            const float2 sx = *(const float2 *)&s.sx[8 * t + 2 * c];
 #pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                const int own = 8 * t + 2 * c + i;
-                const float s = own < p.m ? sw * p.sx[b * p.sx_stride + own] : 0.0f;
-                acc[t][i] = fmaf(s, d[i], acc[t][i]);
-                acc[t][2 + i] = fmaf(s, d[2 + i], acc[t][2 + i]);
-            }
+            for (int i = 0; i < 4; ++i) acc[t][i] = fmaf(s.sw * (i & 1 ? sx.y : sx.x), d[i], acc[t][i]);
         }
+        __syncwarp();
+        issue(step + p.stages, stage);
+        stage = stage + 1 == p.stages ? 0 : stage + 1;
     }
 #pragma unroll
     for (int t = 0; t < NT; ++t)
@@ -247,9 +305,23 @@ template <typename T, int NT> __global__ void __launch_bounds__(256) few_rows(Fe
         if (m >= p.m || n0 + n >= p.n) continue;
         float s = 0.0f;
 #pragma unroll
-        for (int v = 0; v < WARPS; ++v) s += parts[v][n][m];
+        for (int v = 0; v < FEW_WARPS; ++v) s += parts[v][n][m];
         ((T *)p.y)[m * p.y_stride + n0 + n] = from_f32<T>(s);
     }
+}
+
+template <typename T, int NT> cudaError_t go_few(FewParams p, int device, uint64_t stream) {
+    static uint64_t allowed;
+    constexpr size_t STAGE = FEW_WARPS * sizeof(FewStage<NT>);
+    if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
+        cudaError_t e = cudaFuncSetAttribute(few_rows<T, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_STAGES * STAGE);
+        if (e != cudaSuccess) return e;
+        __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
+    }
+    /* as many stages as a warp has blocks, up to all: short rows leave the room to more blocks of threads */
+    const int steps = ((p.k + BLOCK - 1) / BLOCK + FEW_WARPS - 1) / FEW_WARPS;
+    p.stages = steps < FEW_STAGES ? steps : FEW_STAGES;
+    return launch(few_rows<T, NT>, dim3((unsigned)((p.n + 15) / 16)), dim3(256), p.stages * STAGE, stream, p);
 }
 
 /* ---- many rows of x: tcgen05 ------------------------------------------------------------ */
@@ -264,8 +336,8 @@ struct ManyParams {
     const float *sw;
     char *y;
     unsigned *status;
-    int64_t sw_stride, y_stride;
-    int m, n, k_blocks, m_tiles, n_tiles, wide;
+    int64_t sw_stride, y_stride, split_stride;
+    int m, n, k_blocks, m_tiles, n_tiles, wide, splits, per_split;
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -459,14 +531,19 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     const uint32_t base = tensor_base;
     const int worker = PAIR ? blockIdx.x / 2 : blockIdx.x, workers = PAIR ? gridDim.x / 2 : gridDim.x;
-    const int tiles = p.m_tiles * p.n_tiles;
+    const int tiles = p.m_tiles * p.n_tiles * p.splits;
 
     /* tiles that run together share rows and columns: groups of 16 row tiles, column by column */
-    auto place = [&](int t, int &m0, int &n0) {
+    struct Unit { int m0, n0, from, to, split; };
+    auto place = [&](int t) {
+        Unit u;
+        u.split = t % p.splits, t /= p.splits;
+        u.from = u.split * p.per_split, u.to = min(u.from + p.per_split, p.k_blocks);
         const int group = t / (16 * p.n_tiles), first = group * 16, rows = min(16, p.m_tiles - first);
         const int r = t - first * p.n_tiles;
-        n0 = r / rows * BN;
-        m0 = (first + r % rows) * S::ROWS;
+        u.n0 = r / rows * BN;
+        u.m0 = (first + r % rows) * S::ROWS;
+        return u;
     };
 
     if (warp < 4 && S::SPLIT) asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
@@ -478,10 +555,9 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             uint32_t phase = 0;
             bool ok = true;
             for (int t = worker; t < tiles && ok; t += workers) {
-                int m0, n0;
-                place(t, m0, n0);
-                if (PAIR) m0 += 128 * rank, n0 += S::B_ROWS * rank;
-                for (int b = 0; b < p.k_blocks; ++b) {
+                const Unit u = place(t);
+                const int m0 = u.m0 + (PAIR ? 128 * rank : 0), n0 = u.n0 + (PAIR ? S::B_ROWS * rank : 0);
+                for (int b = u.from; b < u.to; ++b) {
                     if (!(ok = wait_for(shared_address(&empty[stage]), phase ^ 1, &abort, p.status, 1))) break;
                     if (++slot == S::SCALES) slot = 0;
                     if (rank == 0)      /* both copies of a pair complete on the leader's barrier */
@@ -503,19 +579,23 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             const uint32_t full0 = shared_address(&full[0]), empty0 = shared_address(&empty[0]);
             const uint32_t summed0 = shared_address(&summed[0]), read0 = shared_address(&read[0]);
             const uint32_t a0 = (1u << 16) | ring >> 4, b0 = a0 + (S::A_BYTES >> 4);
-            const int own = worker < tiles ? (tiles - worker + workers - 1) / workers : 0;      /* tiles of this worker */
-            const int64_t blocks = (int64_t)own * p.k_blocks;
-            int stage = warp >> 1, buffer = warp >> 1;
+            int stage = warp >> 1, buffer = warp >> 1, skip = warp >> 1;
             uint32_t phase = 0, buffer_phase = 0;
+            bool ok = true;
             static_assert(S::STAGES % 2 == 0 && S::BUFFERS % 2 == 0, "every other stage and buffer");
-            for (int64_t i = warp >> 1; i < blocks; i += 2) {
-                if (!wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2)) break;
-                asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
-                multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
-                commit<PAIR>(summed0 + 8 * buffer);
-                commit<PAIR>(empty0 + 8 * stage);
-                if ((stage += 2) >= S::STAGES) stage -= S::STAGES, phase ^= 1;
-                if ((buffer += 2) >= S::BUFFERS) buffer -= S::BUFFERS, buffer_phase ^= 1;
+            for (int t = worker; t < tiles && ok; t += workers) {
+                const Unit u = place(t);
+                int b = u.from + skip;
+                for (; b < u.to; b += 2) {
+                    if (!(ok = wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2))) break;
+                    asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
+                    multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
+                    commit<PAIR>(summed0 + 8 * buffer);
+                    commit<PAIR>(empty0 + 8 * stage);
+                    if ((stage += 2) >= S::STAGES) stage -= S::STAGES, phase ^= 1;
+                    if ((buffer += 2) >= S::BUFFERS) buffer -= S::BUFFERS, buffer_phase ^= 1;
+                }
+                skip = b - u.to;        /* the next tile's first block is the other thread's, or this one's */
             }
         }
     } else if (warp >= 4) {
@@ -528,14 +608,13 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         uint32_t phase = 0;
         bool ok = true;
         for (int t = worker; t < tiles && ok; t += workers) {
-            int m0, n0;
-            place(t, m0, n0);
-            const int row = m0 + 128 * rank + 32 * quarter + lane, col = n0 + half * S::PER;
+            const Unit u = place(t);
+            const int row = u.m0 + 128 * rank + 32 * quarter + lane, col = u.n0 + half * S::PER;
             const float *sw = p.sw + (int64_t)(min(col, p.n - 1) / BLOCK) * p.sw_stride;
             uint64_t sum[S::PER / 2];
 #pragma unroll
             for (int i = 0; i < S::PER / 2; ++i) sum[i] = 0;
-            float next_w = *sw;
+            float next_w = sw[u.from];
             /* a load of tensor memory is under way while the one before it is added, from block to block too */
             uint32_t v[2][S::CHUNK];
             auto begin = [&] {
@@ -546,9 +625,9 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             };
             if (!(ok = begin())) continue;
 #pragma unroll 1
-            for (int b = 0; b < p.k_blocks; ++b) {
+            for (int b = u.from; b < u.to; ++b) {
                 const float one = next_w * scales[slot][32 * quarter + lane];
-                if (b + 1 < p.k_blocks) next_w = sw[b + 1];
+                if (b + 1 < u.to) next_w = sw[b + 1];
                 slot = slot + 1 == S::SCALES ? 0 : slot + 1;
                 uint64_t s;
                 asm("mov.b64 %0, {%1, %1};" : "=l"(s) : "f"(one));
@@ -568,7 +647,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                                 asm volatile("mbarrier.arrive.relaxed.cta.shared::cta.b64 _, [%0];" ::"r"(leader + 8 * buffer) : "memory");
                         }
                         if (++buffer == S::BUFFERS) buffer = 0, phase ^= 1;
-                        if (b + 1 < p.k_blocks) ok = begin();
+                        if (b + 1 < u.to) ok = begin();
                     }
 #pragma unroll
                     for (int i = 0; i < S::CHUNK; i += 2)
@@ -581,6 +660,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             constexpr int V = 16 / sizeof(T), WIDE = 64 / sizeof(T);
             unsigned char *const rows = raw + (ring - shared_address(raw)) + S::STAGES * S::STAGE + (warp - 4) * 32 * S::STORE_ROW;
             const int row0 = row - lane;
+            T *const y = (T *)p.y + u.split * p.split_stride;
 #pragma unroll
             for (int c = 0; c < S::PER; c += WIDE) {
 #pragma unroll
@@ -597,7 +677,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     for (int i = 0; i < 4; ++i) {
                         const int at = 8 * i + (lane >> 2);
                         if (row0 + at < p.m)
-                            *(Pack<T, V> *)((T *)p.y + (row0 + at) * p.y_stride + col + c + piece * V) =
+                            *(Pack<T, V> *)(y + (row0 + at) * p.y_stride + col + c + piece * V) =
                                 *(const Pack<T, V> *)(rows + at * S::STORE_ROW + piece * 16);
                     }
                 } else {
@@ -605,7 +685,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     const int e = lane % WIDE;
                     if (col + c + e < p.n)
                         for (int at = lane / WIDE; at < 32 && row0 + at < p.m; at += AT_ONCE)
-                            ((T *)p.y)[(row0 + at) * p.y_stride + col + c + e] = *(const T *)(rows + at * S::STORE_ROW + e * sizeof(T));
+                            y[(row0 + at) * p.y_stride + col + c + e] = *(const T *)(rows + at * S::STORE_ROW + e * sizeof(T));
                 }
                 __syncwarp();
             }
@@ -622,6 +702,30 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         else
             asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(base), "n"(S::COLUMNS));
     }
+}
+
+/* y = the sum of the parts of a product that was cut along its columns, in their order */
+struct JoinParams {
+    const float *parts;
+    char *y;
+    int64_t part_stride, split_stride, y_stride;
+    int m, n, splits;
+};
+template <typename T> __global__ void __launch_bounds__(256) join_parts(JoinParams p) {
+    enter_grid();
+    const int col = (blockIdx.x * 256 + threadIdx.x) * 4, row = blockIdx.y;
+    if (col >= p.n) return;
+    const float *from = p.parts + row * p.part_stride + col;       /* rows of the parts are whole fours */
+    float4 s = *(const float4 *)from;
+    for (int i = 1; i < p.splits; ++i) {
+        const float4 v = *(const float4 *)(from + i * p.split_stride);
+        s.x += v.x, s.y += v.y, s.z += v.z, s.w += v.w;
+    }
+    T *y = (T *)p.y + row * p.y_stride + col;
+    const float v[4] = {s.x, s.y, s.z, s.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+        if (col + j < p.n) y[j] = from_f32<T>(v[j]);
 }
 
 int encode(TensorMap *map, uint64_t at, int64_t cols, int64_t rows, int64_t stride, int box_rows, bool scales = false) {
@@ -649,7 +753,7 @@ template <typename T, int BN, bool PAIR> int go_many(const emmy_ops_blockfp8_arg
     if (int e = ops_sm_count(device, &sms)) return e;
     p.m_tiles = (int)((a->m + S::ROWS - 1) / S::ROWS);
     p.n_tiles = (int)((a->n + BN - 1) / BN);
-    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles;
+    const int64_t tiles = (int64_t)p.m_tiles * p.n_tiles * p.splits;
     const int workers = PAIR ? sms / 2 : sms, blocks = (int)(tiles < workers ? tiles : workers) * (PAIR ? 2 : 1);
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(blocks), cfg.blockDim = dim3(S::THREADS), cfg.dynamicSmemBytes = S::SMEM;
@@ -663,15 +767,23 @@ template <typename T, int BN, bool PAIR> int go_many(const emmy_ops_blockfp8_arg
     return ops_cuda(cudaLaunchKernelEx(&cfg, many_rows<T, BN, PAIR>, x, w, scales, p), "FP8 product");
 }
 
+template <typename T> int by_tile(int which, const emmy_ops_blockfp8_args *a, const ManyParams &p, int device, uint64_t stream) {
+    switch (which) {
+    case 0: return go_many<T, 32, false>(a, p, device, stream);
+    case 1: return go_many<T, 64, false>(a, p, device, stream);
+    case 2: return go_many<T, 128, false>(a, p, device, stream);
+    default: return go_many<T, 256, true>(a, p, device, stream);
+    }
+}
+
 template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, uint64_t stream) {
-    if (a->m <= 32) {
+    /* Up to 8 rows, and up to 16 where W is small: 16 x 4096 x 4096 takes 7.6 us here and 8.8 us in tiles cut in four,
+     * 16 x 4096 x 14336 20.9 us here and 18.1 us there. */
+    if (a->m <= 8 || (a->m <= 16 && a->n * a->k <= (1 << 25))) {
         FewParams p = {(const uint8_t *)(uintptr_t)a->xq, (const uint8_t *)(uintptr_t)a->wq, (const float *)(uintptr_t)a->xs,
                        (const float *)(uintptr_t)a->ws, (char *)(uintptr_t)a->y, a->xq_stride, a->wq_stride, a->xs_stride,
-                       a->ws_stride, a->y_stride, (int)a->m, (int)a->n, (int)a->k};
-        const dim3 grid((unsigned)((a->n + 15) / 16));
-        cudaError_t e = a->m <= 8    ? launch(few_rows<T, 1>, grid, dim3(256), 0, stream, p)
-                        : a->m <= 16 ? launch(few_rows<T, 2>, grid, dim3(256), 0, stream, p)
-                                     : launch(few_rows<T, 4>, grid, dim3(256), 0, stream, p);
+                       a->ws_stride, a->y_stride, (int)a->m, (int)a->n, (int)a->k, 0};
+        const cudaError_t e = a->m <= 8 ? go_few<T, 1>(p, device, stream) : go_few<T, 2>(p, device, stream);
         return ops_cuda(e, "FP8 product of few rows");
     }
     ManyParams p = {};
@@ -682,25 +794,33 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
     p.wide = aligned(a->y, 16) && a->y_stride * sizeof(T) % 16 == 0;
     int sms;
     if (int e = ops_sm_count(device, &sms)) return e;
-    /* The tiles whose rounds take least.  A block of 128 columns takes a tile 730 cycles (32 columns wide) to 1050 (256, on
-     * pairs of SMs), measured at k = 8192 with one tile an SM: the wider the tile, the less a column costs, as long
-     * as there are tiles for all SMs. */
-    const int64_t rows = (a->m + 127) / 128, pairs = (a->m + 255) / 256;
-    auto rounds = [&](int64_t tiles, int workers) { return (tiles + workers - 1) / workers; };
-    const struct { int which; int64_t cost; } choices[] = {
-        {0, rounds(rows * ((a->n + 31) / 32), sms) * 730},
-        {1, rounds(rows * ((a->n + 63) / 64), sms) * 760},
-        {2, rounds(rows * ((a->n + 127) / 128), sms) * 880},
-        {3, rounds(pairs * ((a->n + 255) / 256), sms / 2) * 1050}};
-    int best = 0;
-    for (int i = 1; i < (rows > 1 ? 4 : 3); ++i)
-        if (choices[i].cost < choices[best].cost) best = i;
-    switch (best) {
-    case 0: return go_many<T, 32, false>(a, p, device, stream);
-    case 1: return go_many<T, 64, false>(a, p, device, stream);
-    case 2: return go_many<T, 128, false>(a, p, device, stream);
-    default: return go_many<T, 256, true>(a, p, device, stream);
-    }
+    /* The tiles and the cut along k whose rounds take least.  A block of 128 columns takes a tile 680 cycles (32 columns
+     * wide) to 1000 (256, on pairs of SMs), measured at k = 8192 with one tile an SM: the wider the tile, the less a
+     * column costs, as long as there are tiles for all SMs.  Where there are not, k is cut into parts that SMs take
+     * beside each other; joining them costs a launch (about 4000 cycles) and their bytes through L2. */
+    const int64_t rows = (a->m + 127) / 128, pairs = (a->m + 255) / 256, part_row = (a->n + 3) / 4 * 4;
+    const struct { int64_t tiles, workers, cycles; } shapes[] = {{rows * ((a->n + 31) / 32), sms, 680},
+                                                                  {rows * ((a->n + 63) / 64), sms, 710},
+                                                                  {rows * ((a->n + 127) / 128), sms, 930},
+                                                                  {pairs * ((a->n + 255) / 256), sms / 2, 1000}};
+    int best = 0, splits = 1;
+    int64_t least = INT64_MAX;
+    for (int i = 0; i < (rows > 1 ? 4 : 3); ++i)
+        for (int cut = 1; cut <= 16 && (cut == 1 || cut * 4 <= p.k_blocks); cut *= 2) {
+            if (cut > 1 && (shapes[i].tiles > shapes[i].workers || cut * a->m * part_row * 4 > (a->parts ? (int64_t)a->parts_bytes : 0) || a->m > 65535)) break;
+            const int64_t per = (p.k_blocks + cut - 1) / cut;
+            const int64_t cost = (shapes[i].tiles * cut + shapes[i].workers - 1) / shapes[i].workers * (per * shapes[i].cycles + 3000) +
+                                 (cut > 1 ? 4000 + a->m * part_row * cut / 512 : 0);
+            if (cost < least) least = cost, best = i, splits = cut;
+        }
+    p.per_split = (p.k_blocks + splits - 1) / splits;
+    p.splits = splits = (p.k_blocks + p.per_split - 1) / p.per_split;
+    if (splits == 1) return by_tile<T>(best, a, p, device, stream);
+    JoinParams j = {(const float *)(uintptr_t)a->parts, p.y, part_row, a->m * part_row, p.y_stride, p.m, p.n, splits};
+    p.y = (char *)(uintptr_t)a->parts, p.y_stride = part_row, p.split_stride = j.split_stride, p.wide = 1;
+    if (int e = by_tile<float>(best, a, p, device, stream)) return e;
+    return ops_cuda(launch(join_parts<T>, dim3((unsigned)((a->n + 1023) / 1024), (unsigned)a->m), dim3(256), 0, stream, j),
+                    "joining the FP8 product's parts");
 }
 
 int check_matrix(const char *name, uint64_t at, int64_t rows, int64_t cols, int64_t stride, int size, int multiple) {
@@ -768,6 +888,7 @@ EMMY_EXPORT int emmy_ops_blockfp8_product(const emmy_ops_blockfp8_args *a, int d
     if (a->xs_stride < 4) return ops_fail(EMMY_RT_EINVAL, "rows of xs are %lld apart", (long long)a->xs_stride);
     if (int e = check_matrix("ws", a->ws, n_blocks, k_blocks, a->ws_stride, 4, 1)) return e;
     if (int e = check_matrix("y", a->m ? a->y : 16, a->m, a->n, a->y_stride, es, 1)) return e;
+    if (a->parts && !aligned(a->parts, 16)) return ops_fail(EMMY_RT_EINVAL, "parts start on 16 bytes");
     if (!a->status || !aligned(a->status, 4)) return ops_fail(EMMY_RT_EINVAL, "a status word is needed");
     if (((a->m + 127) / 128) * ((a->n + 31) / 32) > 0x7fffffffLL)
         return ops_fail(EMMY_RT_EINVAL, "y of %lld x %lld", (long long)a->m, (long long)a->n);

@@ -513,7 +513,7 @@ class BlockFp8QuantizeArgs(ctypes.Structure):
 
 class BlockFp8Args(ctypes.Structure):
     """emmy_ops_blockfp8_args"""
-    _fields_ = [(n, _u64) for n in ("xq", "xs", "wq", "ws", "y", "status")] + \
+    _fields_ = [(n, _u64) for n in ("xq", "xs", "wq", "ws", "y", "status", "parts", "parts_bytes")] + \
         [(n, ctypes.c_int64) for n in ("xq_stride", "xs_stride", "wq_stride", "ws_stride", "y_stride", "m", "n", "k")] + \
         [("dtype", ctypes.c_int32), ("reserved", ctypes.c_int32)]
 

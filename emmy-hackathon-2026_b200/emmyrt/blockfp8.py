@@ -95,10 +95,12 @@ class BlockFp8Linear(Operator):
         x_bytes = -(-self.max_rows * pitch(self.k) // 256) * 256
         self._xs_stride = -(-self.max_rows // 4) * 4
         s_bytes = -(-blocks(self.k) * self._xs_stride * 4 // 256) * 256
-        self._workspace = DeviceBuffer(x_bytes + s_bytes + 256)
+        # parts of a product that is cut along k: few rows of y at a time, so 16 MB hold every cut that pays
+        self._parts_bytes = 0 if self.max_rows <= 8 else min(16 << 20, 16 * min(self.max_rows, 1024) * (self.n + 3) * 4)
+        self._workspace = DeviceBuffer(x_bytes + s_bytes + 256 + self._parts_bytes)
         at = self._workspace.ptr
         self._xq, self._xs, self._status = at, at + x_bytes, at + x_bytes + s_bytes
-        self._status_offset = x_bytes + s_bytes
+        self._parts = self._status + 256
         self._clear_status()
 
     @classmethod
@@ -146,7 +148,7 @@ class BlockFp8Linear(Operator):
         if rows > self.max_rows:
             raise ValueError(f"{rows} rows, the operator was made for {self.max_rows}")
         y = written(shaped(operand(operands[1], "y", FLOATS, 2, d), "y", (rows, self.n)), "y")
-        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
+        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, parts=self._parts if self._parts_bytes else 0, parts_bytes=self._parts_bytes, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
                                wq_stride=_stride(self.wq), ws_stride=self.ws.strides[0], y_stride=y.strides[0], m=rows,
                                n=self.n, k=self.k, dtype=CODE[y.dtype], x_stride=x.strides[0], x_dtype=CODE[x.dtype])
         checks = overlaps([(1, y, "y")], [(0, x, "x"), (2, self.wq, "wq"), (3, self.ws, "ws")])

@@ -106,9 +106,11 @@ int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args *a, int dev
  * f32, as quantised above (xq without square, its padding zero, rows of xs a multiple of 4 apart; wq
  * with).  *status (a word of
  * device memory, zeroed by the caller once) gets a bit when a wait inside the kernel gave
- * up after 2 s; y is then not valid. */
+ * up after 2 s; y is then not valid.  parts (0: none, else on 16 bytes) is memory for the parts of a
+ * product that is cut along k where y alone has too few tiles for the GPU: 16 times m rows of n f32
+ * serve every cut. */
 typedef struct {
-    uint64_t xq, xs, wq, ws, y, status;
+    uint64_t xq, xs, wq, ws, y, status, parts, parts_bytes;
     int64_t xq_stride, xs_stride, wq_stride, ws_stride, y_stride, m, n, k;
     int32_t dtype, reserved;                  /* dtype of y */
 } emmy_ops_blockfp8_args;
