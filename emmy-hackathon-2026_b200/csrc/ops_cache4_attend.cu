@@ -167,34 +167,6 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
-/* pairs of f32 that one instruction works on: a row of the scores has two neighbours in a thread */
-struct Two {
-    uint64_t v;
-    __device__ __forceinline__ Two() {}
-    __device__ __forceinline__ explicit Two(uint64_t both) : v(both) {}
-    __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
-    __device__ __forceinline__ float2 get() const {
-        float2 f;
-        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
-        return f;
-    }
-};
-__device__ __forceinline__ Two operator*(Two a, Two b) {
-    Two d;
-    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Two operator+(Two a, Two b) {
-    Two d;
-    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
-    return d;
-}
-__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
-    Two d;
-    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
-    return d;
-}
-
 /* The token that row r (0 .. 7) of an eight-token group stands for.  A warp reads a token's keys by
  * r = lane / 4 and its values by the pairs r = 2 (lane % 4) + {0, 1}; these orders (with the
  * swizzle below at dim 128) put both into different banks. */

@@ -72,3 +72,72 @@ template <> __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(flo
 template <typename T, int V> struct alignas(sizeof(T) * V) Pack {
     T at[V];
 };
+
+/* a pair of f32 that one instruction works on */
+struct Two {
+    uint64_t v;
+    __device__ __forceinline__ Two() {}
+    __device__ __forceinline__ explicit Two(uint64_t both) : v(both) {}
+    __device__ __forceinline__ Two(float x, float y) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(x), "f"(y)); }
+    __device__ __forceinline__ float2 get() const {
+        float2 f;
+        asm("mov.b64 {%0, %1}, %2;" : "=f"(f.x), "=f"(f.y) : "l"(v));
+        return f;
+    }
+};
+__device__ __forceinline__ Two operator*(Two a, Two b) {
+    Two d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Two operator+(Two a, Two b) {
+    Two d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ Two fma2(Two a, Two b, Two c) {
+    Two d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+
+/* the values of an access in f32, and back with one rounding each */
+template <typename T, int V> static __device__ __forceinline__ void unpack(const Pack<T, V> &q, float (&f)[V]) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) f[i] = to_f32(q.at[i]);
+}
+template <int V> static __device__ __forceinline__ void unpack(const Pack<__nv_bfloat16, V> &q, float (&f)[V]) {
+    if (V % 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) f[i] = to_f32(q.at[i]);
+    } else {
+        const uint32_t *u = (const uint32_t *)&q;
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) {
+            f[2 * i] = __uint_as_float(u[i] << 16);
+            f[2 * i + 1] = __uint_as_float(u[i] & 0xffff0000u);
+        }
+    }
+}
+template <int V> static __device__ __forceinline__ void pack(const float (&f)[V], Pack<float, V> &q) {
+#pragma unroll
+    for (int i = 0; i < V; ++i) q.at[i] = f[i];
+}
+template <int V> static __device__ __forceinline__ void pack(const float (&f)[V], Pack<__half, V> &q) {
+    if (V % 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.at[i] = __float2half_rn(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) ((__half2 *)&q)[i] = __floats2half2_rn(f[2 * i], f[2 * i + (V > 1)]);
+    }
+}
+template <int V> static __device__ __forceinline__ void pack(const float (&f)[V], Pack<__nv_bfloat16, V> &q) {
+    if (V % 2) {
+#pragma unroll
+        for (int i = 0; i < V; ++i) q.at[i] = __float2bfloat16_rn(f[i]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V / 2; ++i) ((__nv_bfloat162 *)&q)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + (V > 1)]);
+    }
+}

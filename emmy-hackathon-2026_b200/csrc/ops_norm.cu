@@ -4,10 +4,12 @@
  *     y = x + scale * gate * N(block),   h = N(y)
  *
  * The bytes bound it: x and block are read once, y and h written once; the row stays in
- * registers between its two norms.  A row belongs to a group of 8 .. 1024 threads with at
- * most 16 elements each (32-bit sums: shuffles inside a warp, shared memory across the
- * warps of a row).  The layer norm's variance is taken about the mean of the registers'
- * values, not as a difference of two sums, which would lose it when the mean is large.
+ * registers between its two norms.  A row belongs to 8, 16 or 32 lanes of a warp, or to a
+ * block of threads of its own; a thread holds 8 elements of it, or 32 where there are rows
+ * enough to fill the GPU: fewer warps then have to meet at a row's sums (one barrier each), and
+ * more bytes are under way for each of them.  32-bit sums: shuffles inside a warp, shared
+ * memory across a row's warps.  The layer norm's variance is taken about the mean of the
+ * registers' values, not as a difference of two sums, which would lose it when the mean is large.
  */
 #include "ops_common.cuh"
 
@@ -21,193 +23,219 @@ struct Vector {          /* a weight, bias or gate row of any element type; 0 po
 struct NormParams {
     const char *x, *block;
     char *y, *h;
-    int64_t x_stride, block_stride, y_stride, h_stride, gate_stride, rows_per_gate, rows;
+    int64_t x_stride, block_stride, y_stride, h_stride, gate_stride, rows;
+    int rows_per_gate;
     Vector post_weight, post_bias, gate, pre_weight, pre_bias;
     int dim, group, layer, post_norm, wide;
     float eps, scale;
 };
 
-template <int V> __device__ __forceinline__ void load_vector(const Vector &w, int64_t e, bool wide, float (&out)[V]) {
-    if (w.dtype == EMMY_OPS_F32) {
-        const float *p = (const float *)w.at + e;
-        if (V >= 4 && wide) {
+/* A thread's elements: N accesses of V, at e[n], as E = N V values in a row; in pairs (Two) where an access has pairs, else one
+ * by one. */
+template <bool PAIRS> struct Unit {
+    using type = Two;
+    static constexpr int SIZE = 2;
+};
+template <> struct Unit<false> {
+    using type = float;
+    static constexpr int SIZE = 1;
+};
+__device__ __forceinline__ float fma2(float a, float b, float c) { return fmaf(a, b, c); }
+__device__ __forceinline__ float total(float v) { return v; }
+__device__ __forceinline__ float total(Two v) { return v.get().x + v.get().y; }
+template <typename U> __device__ __forceinline__ U both(float a, float b);
+template <> __device__ __forceinline__ float both<float>(float a, float) { return a; }
+template <> __device__ __forceinline__ Two both<Two>(float a, float b) { return Two(a, b); }
+__device__ __forceinline__ float value(float v, int) { return v; }
+__device__ __forceinline__ float value(Two v, int i) { return i ? v.get().y : v.get().x; }
+
+/* Runs op(first element of an access, its V values) over a thread's piece of a vector.  The choice of its type stands outside
+ * the loops, so that as many loads as registers allow are under way at once. */
+template <int V, int N, typename W, typename Op>
+__device__ __forceinline__ void each_as(const W *w, const int (&e)[N], bool wide, Op op) {
+    constexpr int A = 16 / (int)sizeof(W) < V ? 16 / (int)sizeof(W) : V;        /* elements an access */
+    Pack<W, A> q[N][V / A];
+    if (V == 1 || wide) {
 #pragma unroll
-            for (int i = 0; i < V; i += 4) {
-                const float4 q = *(const float4 *)(p + (V >= 4 ? i : 0));
-                out[i] = q.x;
-                if (V >= 4) out[i + 1] = q.y, out[i + 2] = q.z, out[i + 3] = q.w;
-            }
-        } else {
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = p[i];
-        }
-    } else if (w.dtype == EMMY_OPS_F16) {
-        const __half *p = (const __half *)w.at + e;
-        if (V > 1 && wide) {
-            const Pack<__half, V> q = *(const Pack<__half, V> *)p;
-#pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = to_f32(q.at[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = to_f32(p[i]);
-        }
+            for (int i = 0; i < V / A; ++i) q[n][i] = *(const Pack<W, A> *)(w + e[n] + i * A);
     } else {
-        const __nv_bfloat16 *p = (const __nv_bfloat16 *)w.at + e;
-        if (V > 1 && wide) {
-            const Pack<__nv_bfloat16, V> q = *(const Pack<__nv_bfloat16, V> *)p;
 #pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = to_f32(q.at[i]);
-        } else {
+        for (int n = 0; n < N; ++n)
 #pragma unroll
-            for (int i = 0; i < V; ++i) out[i] = to_f32(p[i]);
+            for (int i = 0; i < V; ++i) q[n][i / A].at[i % A] = w[e[n] + i];
+    }
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float f[V];
+#pragma unroll
+        for (int i = 0; i < V / A; ++i) {
+            float part[A];
+            unpack(q[n][i], part);
+#pragma unroll
+            for (int j = 0; j < A; ++j) f[i * A + j] = part[j];
         }
+        op(n * V, f);
     }
 }
+template <int V, int N, typename Op>
+__device__ __forceinline__ void each(const Vector &w, int64_t skip, const int (&e)[N], bool wide, Op op) {
+    if (w.dtype == EMMY_OPS_F32)
+        each_as<V>((const float *)w.at + skip, e, wide, op);
+    else if (w.dtype == EMMY_OPS_F16)
+        each_as<V>((const __half *)w.at + skip, e, wide, op);
+    else
+        each_as<V>((const __nv_bfloat16 *)w.at + skip, e, wide, op);
+}
 
-/* the sum over a row's group of threads, to each of them */
-__device__ __forceinline__ float group_sum(float v, int group, float *shared) {
+/* the sum over a row's threads, to each of them; `shared`: 32 floats of this sum's own */
+__device__ __forceinline__ float row_sum(float v, int group, float *shared) {
     for (int d = min(group, 32) / 2; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
-    if (group > 32) {
-        const int warp = threadIdx.x >> 5, warps = group >> 5, first = warp & ~(warps - 1);
-        __syncthreads();                        /* the last sum's readers are done */
-        if ((threadIdx.x & 31) == 0) shared[warp] = v;
+    if (group > 32) {           /* the row is this block of threads */
+        const int lane = threadIdx.x & 31;
+        if (lane == 0) shared[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = shared[first + (threadIdx.x & (warps - 1))];
-        for (int d = warps / 2; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
+        v = lane < group >> 5 ? shared[lane] : 0.0f;
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) v += __shfl_xor_sync(~0u, v, d);
     }
     return v;
 }
 
-/* V elements an access, N accesses a thread */
 template <typename T, int V, int N>
-__global__ void __launch_bounds__(1024) residual_norm(NormParams p) {
-    __shared__ float shared[32];
+__global__ void __launch_bounds__(N * V > 16 ? 512 : 1024) residual_norm(NormParams p) {
+    /* few elements a thread: rows are few too, and the weights are fetched before the sums they wait for */
+    constexpr int E = N * V, K = Unit<V % 2 == 0>::SIZE;
+    using U = typename Unit<V % 2 == 0>::type;
+    constexpr bool EARLY = E <= 8;
+    __shared__ float shared[4][32];
     enter_grid();
-    const int group = p.group, lane = threadIdx.x & (group - 1);
-    const int64_t row = (int64_t)blockIdx.x * (blockDim.x / group) + threadIdx.x / group;
-    const bool live = row < p.rows;
+    const int group = p.group, lane = group > 32 ? threadIdx.x : threadIdx.x & (group - 1);
+    const int64_t place = group > 32 ? blockIdx.x : (int64_t)blockIdx.x * (blockDim.x / group) + threadIdx.x / group;
+    const int64_t row = min(place, p.rows - 1);
     const float inv_dim = 1.0f / p.dim;
-    Pack<T, V> x[N];
-    float b[N][V];
+    /* Accesses past the row take its last one once more: no branch stands between the loads, and only the sums and the
+     * stores ask what is in the row. */
+    int e[N];
     bool in[N];
+    Pack<T, V> x[N], raw[N];
+    U b[E / K];
+    float w[EARLY ? E : 1];
+    const T *const from = (const T *)p.block + row * p.block_stride, *const stream = (const T *)p.x + row * p.x_stride;
 #pragma unroll
     for (int n = 0; n < N; ++n) {
-        const int e = (n * group + lane) * V;
-        in[n] = live && e < p.dim;
-        if (in[n]) {
-            const Pack<T, V> q = *(const Pack<T, V> *)((const T *)p.block + row * p.block_stride + e);
-            x[n] = *(const Pack<T, V> *)((const T *)p.x + row * p.x_stride + e);
-#pragma unroll
-            for (int i = 0; i < V; ++i) b[n][i] = to_f32(q.at[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < V; ++i) b[n][i] = 0.0f;
-        }
+        const int at = (n * group + lane) * V;
+        in[n] = at < p.dim && place < p.rows;
+        e[n] = min(at, p.dim - V);
+        raw[n] = *(const Pack<T, V> *)(from + e[n]);
     }
-    auto statistics = [&](float &mean, float &rstd) {
-        mean = 0.0f;
-        if (p.layer) {
-            float s = 0.0f;
 #pragma unroll
-            for (int n = 0; n < N; ++n)
+    for (int n = 0; n < N; ++n) x[n] = *(const Pack<T, V> *)(stream + e[n]);
+    auto early = [&](const Vector &v) {
+        each<V>(v, 0, e, p.wide, [&](int at, const float (&f)[V]) {
 #pragma unroll
-                for (int i = 0; i < V; ++i) s += b[n][i];
-            mean = group_sum(s, group, shared) * inv_dim;
-        }
-        float s = 0.0f;
-#pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (in[n]) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) s += (b[n][i] - mean) * (b[n][i] - mean);
-            }
-        rstd = 1.0f / sqrtf(group_sum(s, group, shared) * inv_dim + p.eps);
+            for (int i = 0; i < V; ++i) w[EARLY ? at + i : 0] = f[i];
+        });
     };
-    float mean, rstd;
-    if (p.post_norm) {
-        statistics(mean, rstd);
+    if (EARLY && p.post_weight.at) early(p.post_weight);
 #pragma unroll
-        for (int n = 0; n < N; ++n)
-            if (in[n]) {
-                const int e = (n * group + lane) * V;
-                float w[V];
+    for (int n = 0; n < N; ++n) {
+        float f[V];
+        unpack(raw[n], f);
 #pragma unroll
-                for (int i = 0; i < V; ++i) b[n][i] = (b[n][i] - mean) * rstd;
-                if (p.post_weight.at) {
-                    load_vector(p.post_weight, e, p.wide, w);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) b[n][i] *= w[i];
-                }
-                if (p.post_bias.at) {
-                    load_vector(p.post_bias, e, p.wide, w);
-#pragma unroll
-                    for (int i = 0; i < V; ++i) b[n][i] += w[i];
-                }
-            }
+        for (int i = 0; i < V / K; ++i) b[n * V / K + i] = both<U>(f[K * i], f[K * i + K - 1]);
     }
-    const int64_t gate_row = p.gate.at && live ? row / p.rows_per_gate * p.gate_stride : 0;
+    /* op over an access's values and V others */
+    auto with = [&](int at, const float (&f)[V], auto op) {
 #pragma unroll
-    for (int n = 0; n < N; ++n)
-        if (in[n]) {
-            const int e = (n * group + lane) * V;
-            if (p.gate.at) {
-                float w[V];
-                load_vector(p.gate, gate_row + e, p.wide, w);
+        for (int i = 0; i < V / K; ++i) b[at / K + i] = op(b[at / K + i], both<U>(f[K * i], f[K * i + K - 1]));
+    };
+    auto product = [](U a, U c) { return a * c; };
+    auto sum = [](U a, U c) { return a + c; };
+    /* the sum over the row of each(b) */
+    auto over_row = [&](float *shared, auto each) {
+        float all = 0.0f;
 #pragma unroll
-                for (int i = 0; i < V; ++i) b[n][i] *= w[i];
-            }
-            Pack<T, V> q;
+        for (int n = 0; n < N; ++n) {
+            U s = both<U>(0.0f, 0.0f);
 #pragma unroll
-            for (int i = 0; i < V; ++i) {
-                b[n][i] = fmaf(p.scale, b[n][i], to_f32(x[n].at[i]));
-                q.at[i] = from_f32<T>(b[n][i]);
-            }
-            *(Pack<T, V> *)((T *)p.y + row * p.y_stride + e) = q;
+            for (int i = 0; i < V / K; ++i) s = each(b[n * V / K + i], s);
+            all += in[n] ? total(s) : 0.0f;
         }
+        return row_sum(all, group, shared);
+    };
+    /* (b - mean) / deviation, in place */
+    auto normalise = [&](int first) {
+        if (p.layer) {
+            const float mean = over_row(shared[first], [](U v, U s) { return s + v; }) * inv_dim;
+#pragma unroll
+            for (int i = 0; i < E / K; ++i) b[i] = b[i] + both<U>(-mean, -mean);
+        }
+        const float r = rsqrtf(over_row(shared[first + 1], [](U v, U s) { return fma2(v, v, s); }) * inv_dim + p.eps);
+#pragma unroll
+        for (int i = 0; i < E / K; ++i) b[i] = b[i] * both<U>(r, r);
+    };
+    auto weigh = [&](const Vector &v) {
+        if (EARLY) {
+#pragma unroll
+            for (int i = 0; i < E / K; ++i) b[i] = b[i] * both<U>(w[EARLY ? K * i : 0], w[EARLY ? K * i + K - 1 : 0]);
+        } else {
+            each<V>(v, 0, e, p.wide, [&](int at, const float (&f)[V]) { with(at, f, product); });
+        }
+    };
+    auto store = [&](char *to, int64_t stride) {
+        T *const y = (T *)to + row * stride;
+#pragma unroll
+        for (int n = 0; n < N; ++n) {
+            float f[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) f[i] = value(b[(n * V + i) / K], i % K);
+            Pack<T, V> q;
+            pack(f, q);
+            if (in[n]) *(Pack<T, V> *)(y + e[n]) = q;
+        }
+    };
+    if (p.post_norm) normalise(0);
+    if (p.post_weight.at) weigh(p.post_weight);
+    if (p.post_bias.at) each<V>(p.post_bias, 0, e, p.wide, [&](int at, const float (&f)[V]) { with(at, f, sum); });
+    if (p.gate.at) {
+        const int64_t skip = (int64_t)((uint32_t)row / (uint32_t)p.rows_per_gate) * p.gate_stride;
+        each<V>(p.gate, skip, e, p.wide, [&](int at, const float (&f)[V]) { with(at, f, product); });
+    }
+    const U scale = both<U>(p.scale, p.scale);
+#pragma unroll
+    for (int n = 0; n < N; ++n) {
+        float f[V];
+        unpack(x[n], f);
+        with(n * V, f, [&](U a, U c) { return fma2(scale, a, c); });
+    }
+    store(p.y, p.y_stride);
     if (!p.h) return;
-    statistics(mean, rstd);
-#pragma unroll
-    for (int n = 0; n < N; ++n)
-        if (in[n]) {
-            const int e = (n * group + lane) * V;
-            float w[V];
-#pragma unroll
-            for (int i = 0; i < V; ++i) b[n][i] = (b[n][i] - mean) * rstd;
-            if (p.pre_weight.at) {
-                load_vector(p.pre_weight, e, p.wide, w);
-#pragma unroll
-                for (int i = 0; i < V; ++i) b[n][i] *= w[i];
-            }
-            if (p.pre_bias.at) {
-                load_vector(p.pre_bias, e, p.wide, w);
-#pragma unroll
-                for (int i = 0; i < V; ++i) b[n][i] += w[i];
-            }
-            Pack<T, V> q;
-#pragma unroll
-            for (int i = 0; i < V; ++i) q.at[i] = from_f32<T>(b[n][i]);
-            *(Pack<T, V> *)((T *)p.h + row * p.h_stride + e) = q;
-        }
+    if (EARLY && p.pre_weight.at) early(p.pre_weight);
+    normalise(2);
+    if (p.pre_weight.at) weigh(p.pre_weight);
+    if (p.pre_bias.at) each<V>(p.pre_bias, 0, e, p.wide, [&](int at, const float (&f)[V]) { with(at, f, sum); });
+    store(p.h, p.h_stride);
 }
 
-template <typename T, int V, int N> cudaError_t go(const NormParams &p, int threads, uint64_t stream) {
-    const int64_t rows = threads / p.group;
-    return launch(residual_norm<T, V, N>, dim3((unsigned)((p.rows + rows - 1) / rows)), dim3(threads), 0, stream, p);
+template <typename T, int V, int N> cudaError_t go(NormParams &p, uint64_t stream) {
+    const int threads = (p.dim + V * N - 1) / (V * N);
+    p.group = threads <= 8 ? 8 : threads <= 16 ? 16 : (threads + 31) / 32 * 32;
+    const int block = p.group > 32 ? p.group : 128, rows = p.group > 32 ? 1 : 128 / p.group;
+    return launch(residual_norm<T, V, N>, dim3((unsigned)((p.rows + rows - 1) / rows)), dim3(block), 0, stream, p);
 }
 
-/* Accesses of 16 bytes where every row allows them, else of 4, else of one element.  A thread
- * takes 8 elements, and 16 only where 1024 threads would not cover the row otherwise. */
+/* Accesses of 16 bytes where every row allows them, else of 4, else of one element.  8 elements a thread while the rows
+ * do not fill the GPU (they are bound by the chain from load to store) and where accesses are narrow; else 32, over
+ * which a row's sums and addresses cost little; 16 in narrow accesses for rows that 1024 threads of 8 would not hold. */
 template <typename T> cudaError_t dispatch(NormParams &p, int bytes, uint64_t stream) {
-    const int per = p.dim > 8192 ? 16 : 8;
-    int group = 8;
-    while ((int64_t)group * per < p.dim) group *= 2;
-    p.group = group;
-    const int threads = group < 128 ? 128 : group;
+    const bool many = p.dim > 8192 || p.rows * p.dim > 148 * 4096 * 2;
     constexpr int W = 16 / sizeof(T);
-    if (bytes == 16) return per == 16 ? go<T, W, 16 / W>(p, threads, stream) : go<T, W, 8 / W>(p, threads, stream);
-    if (bytes == 4 && sizeof(T) == 2)
-        return per == 16 ? go<T, 2, 8>(p, threads, stream) : go<T, 2, 4>(p, threads, stream);
-    return per == 16 ? go<T, 1, 16>(p, threads, stream) : go<T, 1, 8>(p, threads, stream);
+    const bool large = p.dim > 8192;
+    if (bytes == 16) return many ? go<T, W, 32 / W>(p, stream) : go<T, W, 8 / W>(p, stream);
+    if (bytes == 4 && sizeof(T) == 2) return large ? go<T, 2, 8>(p, stream) : go<T, 2, 4>(p, stream);
+    return large ? go<T, 1, 16>(p, stream) : go<T, 1, 8>(p, stream);
 }
 
 }  // namespace
@@ -259,7 +287,8 @@ EMMY_EXPORT int emmy_ops_residual_norm(const emmy_ops_norm_args *a, int device, 
     p.y = (char *)(uintptr_t)a->y;
     p.h = (char *)(uintptr_t)a->h;
     p.x_stride = a->x_stride, p.block_stride = a->block_stride, p.y_stride = a->y_stride, p.h_stride = a->h_stride;
-    p.gate_stride = a->gate_stride, p.rows_per_gate = a->rows_per_gate, p.rows = a->rows;
+    p.gate_stride = a->gate_stride, p.rows = a->rows;
+    p.rows_per_gate = (int)(a->rows_per_gate < a->rows ? a->rows_per_gate : a->rows);
     p.dim = (int)a->dim, p.layer = a->kind, p.post_norm = a->post_norm != 0, p.eps = a->eps, p.scale = a->scale;
     DeviceScope scope(device);
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
