@@ -25,14 +25,11 @@ __device__ __forceinline__ uint32_t e4m3x4(float a, float b, float c, float d) {
 
 /* |v| as an ordered integer: a NaN is the largest */
 __device__ __forceinline__ uint32_t magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
-/* largest / 448, correctly rounded (as divide8 below); 1 where that is 0 */
+/* largest / 448, correctly rounded; 1 where that is 0 */
 __device__ __forceinline__ float scale_of(uint32_t largest) {
     const float a = __uint_as_float(largest);
     constexpr float R = 1.0f / E4M3_MAX;
-    if (a >= 0x1p-60f && a <= 0x1p100f) {
-        const float q = a * R;
-        return fmaf(fmaf(-E4M3_MAX, q, a), R, q);
-    }
+    if (a >= 0x1p-60f && a <= 0x1p100f) return quotient(a, E4M3_MAX, R);
     const float s = __fdiv_rn(a, E4M3_MAX);
     return s == 0.0f ? 1.0f : s;
 }
@@ -62,19 +59,12 @@ template <typename T> __device__ __forceinline__ void load8(const T *x, int64_t 
     }
 }
 
-/* v / s for the eight values of a block's scale, correctly rounded.  By Markstein's theorem (IBM J. Res. Dev. 34, 1990) the
- * quotient q0 = v r of the correctly rounded r = 1 / s is put right by one step, q0 + (v - s q0) r with both
- * sums fused, where nothing underflows: for s within 2^-60 .. 2^60 that is so for every quotient that e4m3 does
- * not round to zero anyway.  Three instructions a value; the eight divisions were most of the kernel (39 -> 20 us at
- * 4096 x 8192). */
+/* v / s for the eight values of a block's scale.  The eight divisions were most of the kernel: 39 -> 31 us at 4096 x 8192. */
 __device__ __forceinline__ void divide8(float (&v)[8], float s) {
     if (s >= 0x1p-60f && s <= 0x1p60f) {
         const float r = __frcp_rn(s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float q = v[i] * r;
-            v[i] = fmaf(fmaf(-s, q, v[i]), r, q);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = quotient(v[i], s, r);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], s);

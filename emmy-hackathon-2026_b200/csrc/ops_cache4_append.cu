@@ -18,38 +18,43 @@ struct AppendParams {
     const char *x[2];
     char *level[2], *stored[2];
     __half2 *meta[2];
-    int64_t token[2], head[2], tokens, slots_in_cache;
+    int64_t token[2], head[2], slots_in_cache;
     const void *slots;
-    int heads, page, slots_64, wide;
+    int tokens, heads, page, slots_64, wide;
 };
 
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+/* DIM / 8 lanes a vector; blocks of threads y = 0 take keys, y = 1 values */
 template <typename T, int DIM>
 __global__ void __launch_bounds__(256) cache4_append(AppendParams p) {
     constexpr int LANES = DIM / 8;
     constexpr float LARGEST = 65504.0f;
     enter_grid();
-    const int lane = threadIdx.x % LANES;
-    const int64_t item = ((int64_t)blockIdx.x * 256 + threadIdx.x) / LANES;
-    const int64_t vectors = p.tokens * p.heads;
-    const int which = item >= vectors;             /* keys first, then values */
-    const int64_t at = which ? item - vectors : item;
-    const int64_t token = at / p.heads;
-    const int head = (int)(at - token * p.heads);
-    const bool live = token < p.tokens;
+    const int lane = threadIdx.x % LANES, which = blockIdx.y;
+    const uint32_t item = blockIdx.x * (256 / LANES) + threadIdx.x / LANES, token = item / (uint32_t)p.heads;
+    const int head = item - token * p.heads;
+    const bool live = token < (uint32_t)p.tokens;
     int64_t slot = -1;
     if (live) slot = p.slots_64 ? ((const int64_t *)p.slots)[token] : ((const int32_t *)p.slots)[token];
     float v[8];
     if (live) {
         const T *x = (const T *)p.x[which] + token * p.token[which] + head * p.head[which] + lane * 8;
         if (p.wide) {
-            if (sizeof(T) == 2) {
-                const Pack<T, 8> q = *(const Pack<T, 8> *)x;
+            constexpr int V = 16 / sizeof(T);
+            Pack<T, V> q[8 / V];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = to_f32(q.at[i]);
-            } else {
-                const Pack<T, 4> q[2] = {*(const Pack<T, 4> *)x, *(const Pack<T, 4> *)(x + 4)};
+            for (int i = 0; i < 8 / V; ++i) q[i] = *(const Pack<T, V> *)(x + i * V);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) v[i] = to_f32(q[i / 4].at[i % 4]);
+            for (int i = 0; i < 8 / V; ++i) {
+                float f[V];
+                unpack(q[i], f);
+#pragma unroll
+                for (int j = 0; j < V; ++j) v[i * V + j] = f[j];
             }
         } else {
 #pragma unroll
@@ -59,59 +64,63 @@ __global__ void __launch_bounds__(256) cache4_append(AppendParams p) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = 0.0f;
     }
-    float low = LARGEST, high = -LARGEST;
-    int nan = 0;
+    auto extremes = [&](float &low, float &high) {
+        low = high = v[0];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        nan |= v[i] != v[i];
-        v[i] = fminf(fmaxf(v[i], -LARGEST), LARGEST);
-        low = fminf(low, v[i]);
-        high = fmaxf(high, v[i]);
-    }
+        for (int i = 1; i < 8; ++i) low = fminf(low, v[i]), high = max_or_nan(high, v[i]);
 #pragma unroll
-    for (int d = LANES / 2; d > 0; d >>= 1) {
-        low = fminf(low, __shfl_xor_sync(~0u, low, d));
-        high = fmaxf(high, __shfl_xor_sync(~0u, high, d));
-        nan |= __shfl_xor_sync(~0u, nan, d);
+        for (int d = LANES / 2; d > 0; d >>= 1) {
+            low = fminf(low, __shfl_xor_sync(~0u, low, d));
+            high = max_or_nan(high, __shfl_xor_sync(~0u, high, d));
+        }
+    };
+    float low, high;
+    extremes(low, high);
+    const bool nan = high != high;
+    if (__any_sync(~0u, nan || low < -LARGEST || high > LARGEST)) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = fminf(fmaxf(v[i], -LARGEST), LARGEST);      /* a NaN becomes a number, too */
+        extremes(low, high);
     }
     const __half least = __float2half_rn(low);
-    const __half step = nan ? __ushort_as_half(0x7fff) : __float2half_rn((high - low) / 15.0f);
-    const float z = __half2float(least), s = __half2float(step);
-    uint32_t levels = 0;
-    float said[8];
+    const __half step = nan ? __ushort_as_half(0x7fff) : __float2half_rn(__fdiv_rn(high - low, 15.0f));
+    const float z = __half2float(least), s = __half2float(step), r = s > 0.0f ? __frcp_rn(s) : 0.0f;
+    /* The level to the nearest even by adding 1.5 2^23, whose last bit is 1; four levels make 16 bits, exact in f32.  With a
+     * step of 0 (or NaN) all levels are 0: r is 0. */
+    constexpr float ROUND = 12582912.0f;
+    float n[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const float n = s > 0.0f ? fminf(fmaxf(rintf((v[i] - z) / s), 0.0f), 15.0f) : 0.0f;
-        levels |= (uint32_t)n << 4 * i;
-        said[i] = fmaf(n, s, z);
+        const float q = s > 0.0f ? quotient(v[i] - z, s, r) : 0.0f;
+        n[i] = (fminf(fmaxf(q, 0.0f), 15.0f) + ROUND) - ROUND;
     }
     if (!live) return;
     if (slot >= 0 && slot < p.slots_in_cache) {
-        const int64_t page = slot / p.page, row = slot - page * p.page;
+        const int64_t page = slot <= 0xffffffffll ? (uint32_t)slot / (uint32_t)p.page : slot / p.page, row = slot - page * p.page;
         const int64_t to = (page * p.heads + head) * p.page + row;
-        *(uint32_t *)(p.level[which] + to * (DIM / 2) + lane * 4) = levels;
+        const float first = fmaf(fmaf(fmaf(n[3], 16.0f, n[2]), 16.0f, n[1]), 16.0f, n[0]);
+        const float second = fmaf(fmaf(fmaf(n[7], 16.0f, n[6]), 16.0f, n[5]), 16.0f, n[4]);
+        *(uint32_t *)(p.level[which] + to * (DIM / 2) + lane * 4) = (uint32_t)first | (uint32_t)second << 16;
         if (lane == 0) p.meta[which][to] = __halves2half2(step, least);
     }
     if (p.stored[which]) {
-        T *out = (T *)p.stored[which] + (token * p.heads + head) * DIM + lane * 8;
-        if (sizeof(T) == 2) {
-            Pack<T, 8> q;
+        constexpr int V = 16 / sizeof(T);
+        T *out = (T *)p.stored[which] + ((int64_t)token * p.heads + head) * DIM + lane * 8;
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q.at[i] = from_f32<T>(said[i]);
-            *(Pack<T, 8> *)out = q;
-        } else {
-            Pack<T, 4> q[2];
+        for (int i = 0; i < 8; i += V) {
+            float f[V];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i / 4].at[i % 4] = from_f32<T>(said[i]);
-            *(Pack<T, 4> *)out = q[0];
-            *(Pack<T, 4> *)(out + 4) = q[1];
+            for (int j = 0; j < V; ++j) f[j] = fmaf(n[i + j], s, z);
+            Pack<T, V> q;
+            pack(f, q);
+            *(Pack<T, V> *)(out + i) = q;
         }
     }
 }
 
 template <typename T> cudaError_t dispatch(const AppendParams &p, int dim, uint64_t stream) {
-    const int64_t items = 2 * p.tokens * p.heads, per = 256 / (dim / 8);
-    const dim3 grid((unsigned)((items + per - 1) / per));
+    const int64_t items = (int64_t)p.tokens * p.heads, per = 256 / (dim / 8);
+    const dim3 grid((unsigned)((items + per - 1) / per), 2);
     return dim == 64 ? launch(cache4_append<T, 64>, grid, dim3(256), 0, stream, p)
                      : launch(cache4_append<T, 128>, grid, dim3(256), 0, stream, p);
 }
@@ -135,7 +144,7 @@ EMMY_EXPORT int emmy_ops_cache4_append(const emmy_ops_cache4_append_args *a, int
     if (a->tokens < 0 || a->tokens > 0x7fffffffLL) return ops_fail(EMMY_RT_EINVAL, "tokens %lld", (long long)a->tokens);
     if (a->tokens == 0) return 0;
     const int es = elem_size(a->dtype);
-    if (2 * a->tokens * a->cache.heads > 0x7fffffffLL * 8)
+    if (a->tokens * a->cache.heads > 0x7fffff00LL)
         return ops_fail(EMMY_RT_EINVAL, "%lld tokens of %d heads are too many for one call", (long long)a->tokens, a->cache.heads);
     if (!a->k || !a->v || !a->slots || !aligned(a->k, es) || !aligned(a->v, es) || !aligned(a->slots, a->slots_64 ? 8 : 4))
         return ops_fail(EMMY_RT_EINVAL, "k, v and slots are needed, aligned to their elements");
@@ -147,7 +156,7 @@ EMMY_EXPORT int emmy_ops_cache4_append(const emmy_ops_cache4_append_args *a, int
     p.meta[0] = (__half2 *)(uintptr_t)a->cache.k_meta, p.meta[1] = (__half2 *)(uintptr_t)a->cache.v_meta;
     p.stored[0] = (char *)(uintptr_t)a->k_stored, p.stored[1] = (char *)(uintptr_t)a->v_stored;
     p.token[0] = a->k_token, p.token[1] = a->v_token, p.head[0] = a->k_head, p.head[1] = a->v_head;
-    p.tokens = a->tokens, p.slots_in_cache = a->cache.pages * a->cache.page;
+    p.tokens = (int)a->tokens, p.slots_in_cache = a->cache.pages * a->cache.page;
     p.slots = (const void *)(uintptr_t)a->slots, p.slots_64 = a->slots_64 != 0;
     p.heads = a->cache.heads, p.page = a->cache.page;
     p.wide = aligned(a->k, 16) && aligned(a->v, 16);

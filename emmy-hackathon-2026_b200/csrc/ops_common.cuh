@@ -141,3 +141,11 @@ template <int V> static __device__ __forceinline__ void pack(const float (&f)[V]
         for (int i = 0; i < V / 2; ++i) ((__nv_bfloat162 *)&q)[i] = __floats2bfloat162_rn(f[2 * i], f[2 * i + (V > 1)]);
     }
 }
+
+/* v / s, correctly rounded, with r = 1 / s correctly rounded.  By Markstein's theorem (IBM J. Res. Dev. 34, 1990) the
+ * quotient q0 = v r is put right by one step, q0 + (v - s q0) r with both sums fused, where nothing underflows: for s
+ * within 2^-60 .. 2^60 and quotients that are not below 2^-60 of interest.  Three instructions. */
+static __device__ __forceinline__ float quotient(float v, float s, float r) {
+    const float q = v * r;
+    return fmaf(fmaf(-s, q, v), r, q);
+}

@@ -26,13 +26,46 @@ struct RotaryParams {
     float magnitude;
 };
 
-/* V pairs a step (half: V elements of either half; interleaved: 2 V consecutive elements) */
+/* V pairs a step (half: V elements of either half; interleaved: 2 V consecutive elements).  A thread keeps its place in the
+ * heads and goes over the block's (token, head) pairs, AT_ONCE of them under way; the first ones' loads are issued before the
+ * angles are worked out. */
 template <typename T, int V, bool HALF>
 __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
-    extern __shared__ float2 table[];             /* [per_block][pairs] (cos, sin) */
+    constexpr int AT_ONCE = 2;
+    extern __shared__ __align__(16) float2 table[];             /* [per_block][pairs] (cos, sin) */
     enter_grid();
     const int64_t first = (int64_t)blockIdx.x * p.per_block;
     const int live = (int)min((int64_t)p.per_block, p.tokens - first);
+    const int units = p.pairs / V, per_head = units + (p.copies ? p.rest / V : 0), heads = p.heads[0] + p.heads[1];
+    const int side = per_head < (int)blockDim.x ? blockDim.x / per_head : 1;      /* heads side by side */
+    const int own = threadIdx.x / per_head, second = HALF ? p.pairs : V;          /* from an access to its partner */
+    struct Item {
+        int token, head;
+    };
+    Item next = {own / heads, own % heads};
+    if (own >= side) next.token = live;                         /* no place: nothing to do */
+    auto advance = [&] {
+        next.head += side;
+        while (next.head >= heads) next.head -= heads, ++next.token;
+    };
+    int unit = threadIdx.x - own * per_head;
+    Item item[AT_ONCE];
+    Pack<T, V> a[AT_ONCE], b[AT_ONCE];
+    auto element = [&] { return unit >= units ? 2 * p.pairs + (unit - units) * V : HALF ? unit * V : 2 * unit * V; };
+    auto load = [&] {
+#pragma unroll
+        for (int i = 0; i < AT_ONCE; ++i) {
+            item[i] = next;
+            if (next.token < live) {
+                const int which = next.head >= p.heads[0], h = which ? next.head - p.heads[0] : next.head;
+                const T *x = (const T *)p.x[which] + (first + next.token) * p.x_token[which] + h * p.x_head[which] + element();
+                a[i] = *(const Pack<T, V> *)x;
+                if (unit < units) b[i] = *(const Pack<T, V> *)(x + second);
+                advance();
+            }
+        }
+    };
+    load();
     for (int i = threadIdx.x; i < live * p.pairs; i += blockDim.x) {
         const int token = i / p.pairs, pair = i - token * p.pairs;
         const int64_t position = p.positions_64 ? ((const int64_t *)p.positions)[first + token]
@@ -43,57 +76,53 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
         table[i] = make_float2(c * p.magnitude, (p.transpose ? -s : s) * p.magnitude);
     }
     __syncthreads();
-    const int units = p.pairs / V, rest = p.copies ? p.rest / V : 0;
-    const int per_head = units + rest, heads = p.heads[0] + p.heads[1], per_token = heads * per_head;
-    for (int i = threadIdx.x; i < live * per_token; i += blockDim.x) {
-        const int token = i / per_token, r = i - token * per_token, head = r / per_head, unit = r - head * per_head;
-        const int which = head >= p.heads[0], h = which ? head - p.heads[0] : head;
-        const T *x = (const T *)p.x[which] + (first + token) * p.x_token[which] + h * p.x_head[which];
-        T *out = (T *)p.out[which] + (first + token) * p.out_token[which] + h * p.out_head[which];
-        if (unit >= units) {
-            const int e = 2 * p.pairs + (unit - units) * V;
-            *(Pack<T, V> *)(out + e) = *(const Pack<T, V> *)(x + e);
-            continue;
-        }
-        const float2 *cs = table + token * p.pairs + unit * V;
-        if (HALF) {
-            const int e = unit * V;
-            const Pack<T, V> a = *(const Pack<T, V> *)(x + e), b = *(const Pack<T, V> *)(x + p.pairs + e);
-            Pack<T, V> ra, rb;
+    while (true) {
+        while (item[0].token < live) {
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float2 q = cs[j];
-                const float u = to_f32(a.at[j]), v = to_f32(b.at[j]);
-                ra.at[j] = from_f32<T>(u * q.x - v * q.y);
-                rb.at[j] = from_f32<T>(u * q.y + v * q.x);
-            }
-            *(Pack<T, V> *)(out + e) = ra;
-            *(Pack<T, V> *)(out + p.pairs + e) = rb;
-        } else {
-            /* two accesses of V elements hold V pairs */
-            const int e = 2 * unit * V;
-            Pack<T, V> a[2] = {*(const Pack<T, V> *)(x + e), *(const Pack<T, V> *)(x + e + V)}, r[2];
+            for (int i = 0; i < AT_ONCE; ++i) {
+                if (item[i].token >= live) continue;
+                const int which = item[i].head >= p.heads[0], h = which ? item[i].head - p.heads[0] : item[i].head;
+                T *out = (T *)p.out[which] + (first + item[i].token) * p.out_token[which] + h * p.out_head[which] + element();
+                if (unit >= units) {
+                    *(Pack<T, V> *)out = a[i];
+                    continue;
+                }
+                const float2 *cs = table + item[i].token * p.pairs + unit * V;
+                float u[V], v[V], ru[V], rv[V];
+                unpack(a[i], u);
+                unpack(b[i], v);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                const float2 q = cs[j];
-                const float u = to_f32(a[2 * j / V].at[2 * j % V]), v = to_f32(a[(2 * j + 1) / V].at[(2 * j + 1) % V]);
-                r[2 * j / V].at[2 * j % V] = from_f32<T>(u * q.x - v * q.y);
-                r[(2 * j + 1) / V].at[(2 * j + 1) % V] = from_f32<T>(u * q.y + v * q.x);
+                for (int j = 0; j < V; ++j) {
+                    /* pair j: u[j] and v[j], or elements 2 j and 2 j + 1 of u and v in a row */
+                    const float2 q = cs[j];
+                    const int k = 2 * j, l = 2 * j + 1;
+                    const float c = HALF ? u[j] : k < V ? u[k % V] : v[k % V], d = HALF ? v[j] : l < V ? u[l % V] : v[l % V];
+                    const float rc = c * q.x - d * q.y, rd = c * q.y + d * q.x;
+                    (HALF ? ru[j] : k < V ? ru[k % V] : rv[k % V]) = rc;
+                    (HALF ? rv[j] : l < V ? ru[l % V] : rv[l % V]) = rd;
+                }
+                Pack<T, V> ra, rb;
+                pack(ru, ra);
+                pack(rv, rb);
+                *(Pack<T, V> *)out = ra;
+                *(Pack<T, V> *)(out + second) = rb;
             }
-            *(Pack<T, V> *)(out + e) = r[0];
-            *(Pack<T, V> *)(out + e + V) = r[1];
+            load();
         }
+        /* more places in a head than threads: the next ones, from the first head on */
+        if (side > 1 || (unit += blockDim.x) >= per_head) return;
+        next = {0, 0};
+        load();
     }
 }
 
 template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, uint64_t stream) {
-    /* tokens a block: enough for two steps of its 256 threads where there are many, one where
-     * there are few, as long as the table fits 32 KB */
-    const int per_token = (p.heads[0] + p.heads[1]) * (p.pairs / V + (p.copies ? p.rest / V : 0));
-    int64_t per = 512 / (per_token > 0 ? per_token : 1);
-    const int64_t spread = p.tokens / (148 * 4);
+    /* tokens a block: about two (token, head) pairs for each of its 256 threads where there are many tokens, one token
+     * where there are few, as long as the table fits 32 KB */
+    const int64_t per_token = (int64_t)(p.heads[0] + p.heads[1]) * (p.pairs / V + (p.copies ? p.rest / V : 0));
+    int64_t per = (512 + per_token / 2) / per_token;
+    const int64_t spread = p.tokens / (148 * 4), most = 32768 / ((int64_t)p.pairs * 8);
     if (per > spread) per = spread;
-    const int64_t most = 32768 / ((int64_t)p.pairs * 8);
     if (per > most) per = most;
     p.per_block = per < 1 ? 1 : (int)per;
     const dim3 grid((unsigned)((p.tokens + p.per_block - 1) / p.per_block));
