@@ -78,38 +78,29 @@ struct QuantRowsParams {
     uint8_t *q;
     float *s;
     int64_t rows, cols, x_stride, q_stride, s_stride;
-    int wide, across;
+    int across;
 };
 
 /* 16 lanes a block of 128, eight elements each; 1 << across blocks of a row side by side in a block of threads, which
- * takes QUANT_ROWS rows for each of its 16 groups of lanes, all loads before the first use.  WHOLE: every lane's eight
- * elements are in the row or past it, and allow 16-byte accesses. */
+ * takes QUANT_ROWS rows for each of its 16 groups of lanes, all loads before the first use.  A: the elements of an
+ * access, which rows, their ends and the pointer allow. */
 constexpr int QUANT_ROWS = 4;
-template <typename T, bool WHOLE> __global__ void __launch_bounds__(256) quantize_rows(QuantRowsParams p) {
+template <typename T, int A> __global__ void __launch_bounds__(256) quantize_rows(QuantRowsParams p) {
     enter_grid();
     const int group = threadIdx.x / 16, lane = threadIdx.x & 15, down = 16 >> p.across;
     const int64_t b = ((int64_t)blockIdx.y << p.across) + (group & ((1 << p.across) - 1)), e = b * BLOCK + lane * 8;
     const int64_t first = (int64_t)blockIdx.x * (down * QUANT_ROWS) + (group >> p.across);
     const int left = (int)min((int64_t)(QUANT_ROWS * 16), p.rows - first);       /* rows from `first` on */
-    const bool in = e < p.cols;
-    constexpr int V = 16 / sizeof(T);
-    Pack<T, V> x[QUANT_ROWS][8 / V];
+    Pack<T, A> x[QUANT_ROWS][8 / A];
     const T *from = (const T *)p.x + first * p.x_stride + e;
 #pragma unroll
-    for (int i = 0; i < QUANT_ROWS; ++i, from += down * p.x_stride) {
+    for (int i = 0; i < QUANT_ROWS; ++i, from += down * p.x_stride)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j / V].at[j % V] = from_f32<T>(0.0f);
-        if (i * down >= left) continue;
-        if (WHOLE) {
-            if (in)
+        for (int j = 0; j < 8 / A; ++j) {
 #pragma unroll
-                for (int j = 0; j < 8 / V; ++j) x[i][j] = *(const Pack<T, V> *)(from + j * V);
-        } else {
-#pragma unroll
-            for (int j = 0; j < 8; ++j)
-                if (e + j < p.cols) x[i][j / V].at[j % V] = from[j];
+            for (int k = 0; k < A; ++k) x[i][j].at[k] = from_f32<T>(0.0f);
+            if (i * down < left && e + j * A < p.cols) x[i][j] = *(const Pack<T, A> *)(from + j * A);
         }
-    }
     float *scale = p.s + b * p.s_stride + first;
     uint8_t *to = p.q + first * p.q_stride + e;
     const bool stores = e < ((p.cols + 15) & ~15ll);    /* columns past the end, up to a multiple of 16, become zero */
@@ -117,7 +108,7 @@ template <typename T, bool WHOLE> __global__ void __launch_bounds__(256) quantiz
     for (int i = 0; i < QUANT_ROWS; ++i, to += down * p.q_stride) {
         float v[8];
         uint32_t largest = 0;
-        if (sizeof(T) == 2) {
+        if (sizeof(T) == 2 && A > 1) {
             const uint32_t *two = (const uint32_t *)&x[i][0];
             largest = larger2(larger2(two[0] & 0x7fff7fff, two[1] & 0x7fff7fff), larger2(two[2] & 0x7fff7fff, two[3] & 0x7fff7fff));
 #pragma unroll
@@ -125,12 +116,12 @@ template <typename T, bool WHOLE> __global__ void __launch_bounds__(256) quantiz
             largest = largest_of<T>(largest);
         } else {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(to_f32(x[i][j / V].at[j % V])));
+            for (int j = 0; j < 8; ++j) largest = max(largest, magnitude(to_f32(x[i][j / A].at[j % A])));
 #pragma unroll
             for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32(x[i][j / V].at[j % V]);
+        for (int j = 0; j < 8; ++j) v[j] = to_f32(x[i][j / A].at[j % A]);
         if (i * down >= left || b * BLOCK >= p.cols) continue;
         const float s = scale_of(largest);
         if (lane == 0) scale[i * down] = s;
@@ -393,7 +384,7 @@ struct ManyParams {
     char *y;
     unsigned *status;
     int64_t sw_stride, y_stride, split_stride;
-    int m, n, k_blocks, m_tiles, n_tiles, wide, splits, per_split;
+    int m, n, k_blocks, m_tiles, n_tiles, wide, even, splits, per_split;
 };
 
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
@@ -736,6 +727,13 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                             *(Pack<T, V> *)(y + (row0 + at) * p.y_stride + col + c + piece * V) =
                                 *(const Pack<T, V> *)(rows + at * S::STORE_ROW + piece * 16);
                     }
+                } else if (sizeof(T) == 2 && p.even && col + c + WIDE <= p.n) {
+                    /* rows that start on 4 bytes: pairs, two rows at a time */
+                    const int e = 2 * (lane & 15);
+#pragma unroll 4
+                    for (int at = lane >> 4; at < 32; at += 2)
+                        if (row0 + at < p.m)
+                            *(uint32_t *)(y + (row0 + at) * p.y_stride + col + c + e) = *(const uint32_t *)(rows + at * S::STORE_ROW + 2 * e);
                 } else {
                     constexpr int AT_ONCE = 32 / WIDE;
                     const int e = lane % WIDE;
@@ -848,6 +846,7 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
     p.sw_stride = a->ws_stride, p.y_stride = a->y_stride;
     p.m = (int)a->m, p.n = (int)a->n, p.k_blocks = (int)((a->k + BLOCK - 1) / BLOCK);
     p.wide = aligned(a->y, 16) && a->y_stride * sizeof(T) % 16 == 0;
+    p.even = aligned(a->y, 4) && a->y_stride * sizeof(T) % 4 == 0;
     int sms;
     if (int e = ops_sm_count(device, &sms)) return e;
     /* The tiles and the cut along k whose rounds take least.  A block of 128 columns takes a tile 680 cycles (32 columns
@@ -947,12 +946,19 @@ EMMY_EXPORT int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args
         const int64_t down = (16 >> across) * QUANT_ROWS, tall = (col_blocks + (1 << across) - 1) >> across;
         if (tall > 65535) return ops_fail(EMMY_RT_EINVAL, "%lld columns", (long long)a->cols);
         QuantRowsParams p = {(const char *)(uintptr_t)a->x, (uint8_t *)(uintptr_t)a->q, (float *)(uintptr_t)a->s, a->rows, a->cols,
-                             a->x_stride, a->q_stride, a->s_stride, wide, across};
+                             a->x_stride, a->q_stride, a->s_stride, across};
         const dim3 grid((unsigned)((a->rows + down - 1) / down), (unsigned)tall);
-        auto go = [&](auto whole, auto parts) { return launch(wide && a->cols % 8 == 0 ? whole : parts, grid, dim3(256), 0, stream, p); };
-        e = a->dtype == EMMY_OPS_F32   ? go(quantize_rows<float, true>, quantize_rows<float, false>)
-            : a->dtype == EMMY_OPS_F16 ? go(quantize_rows<__half, true>, quantize_rows<__half, false>)
-                                       : go(quantize_rows<__nv_bfloat16, true>, quantize_rows<__nv_bfloat16, false>);
+        auto fits = [&](int bytes) { return aligned(a->x, bytes) && a->x_stride * es % bytes == 0 && a->cols * es % bytes == 0; };
+        const int access = fits(16) ? 16 : fits(4) ? 4 : es;
+        auto go = [&](auto kernel) { return launch(kernel, grid, dim3(256), 0, stream, p); };
+        if (a->dtype == EMMY_OPS_F32)
+            e = access == 16 ? go(quantize_rows<float, 4>) : go(quantize_rows<float, 1>);
+        else if (a->dtype == EMMY_OPS_F16)
+            e = access == 16 ? go(quantize_rows<__half, 8>) : access == 4 ? go(quantize_rows<__half, 2>) : go(quantize_rows<__half, 1>);
+        else
+            e = access == 16  ? go(quantize_rows<__nv_bfloat16, 8>)
+                : access == 4 ? go(quantize_rows<__nv_bfloat16, 2>)
+                              : go(quantize_rows<__nv_bfloat16, 1>);
     }
     return ops_cuda(e, "FP8 quantisation");
 }
