@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import BlockFp8LinearArgs, BlockFp8QuantizeArgs, DeviceBuffer
+from . import BlockFp8LinearArgs, BlockFp8QuantizeArgs, DeviceBuffer, check, lib
 from .operands import CODE, FLOATS, Array, Operator, Plan, operand, overlaps, shaped, written
 
 BLOCK = 128
@@ -66,8 +66,7 @@ def _stride(q: Array) -> int:
 
 def _with_padding(q: Array) -> Array:
     """``q`` with the columns that the row quantiser fills with zeros."""
-    a = Array(q.ptr, q.dtype, (q.shape[0], pitch(q.shape[1])), (_stride(q), 1), q.device)
-    return a
+    return Array(q.ptr, q.dtype, (q.shape[0], pitch(q.shape[1])), (_stride(q), 1), q.device)
 
 
 class BlockFp8Linear(Operator):
@@ -119,15 +118,12 @@ class BlockFp8Linear(Operator):
         return d
 
     def _clear_status(self) -> None:
-        word = Array(self._status, "i32", (1,))
-        from . import check, lib
-        check(lib.emmy_rt_memset(word.ptr, 0, 4, 0), "memset")
+        check(lib.emmy_rt_memset(self._status, 0, 4, 0), "memset")
         check(lib.emmy_rt_stream_synchronize(0), "sync")
 
     def status(self) -> int:
         """The calls' status word (0 = ok; non-zero = a bounded wait inside the kernel gave up and y is not valid).
         Waits for the legacy default stream; a non-zero word is cleared."""
-        from . import check, lib
         out = np.zeros(1, np.uint32)
         check(lib.emmy_rt_memcpy_dtoh(out.ctypes.data, self._status, 4, 0), "dtoh")
         check(lib.emmy_rt_stream_synchronize(0), "sync")
@@ -148,7 +144,8 @@ class BlockFp8Linear(Operator):
         if rows > self.max_rows:
             raise ValueError(f"{rows} rows, the operator was made for {self.max_rows}")
         y = written(shaped(operand(operands[1], "y", FLOATS, 2, d), "y", (rows, self.n)), "y")
-        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, parts=self._parts if self._parts_bytes else 0, parts_bytes=self._parts_bytes, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
+        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, parts=self._parts if self._parts_bytes else 0,
+                               parts_bytes=self._parts_bytes, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
                                wq_stride=_stride(self.wq), ws_stride=self.ws.strides[0], y_stride=y.strides[0], m=rows,
                                n=self.n, k=self.k, dtype=CODE[y.dtype], x_stride=x.strides[0], x_dtype=CODE[x.dtype])
         checks = overlaps([(1, y, "y")], [(0, x, "x"), (2, self.wq, "wq"), (3, self.ws, "ws")])

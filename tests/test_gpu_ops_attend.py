@@ -1,4 +1,4 @@
-"""Attention over the 4-bit cache on the B200 against its definition in f64, and the decoder layer's operators in a row.
+"""Attention over the 4-bit cache on the B200 against its definition in f64.
 
 Tolerances, for one output element with probabilities p, steps s, levels n and least values z of the values:
 half a step of the type; the rounding of p s to f16, 2^-11 of sum p s n (where the result is f16, sum p and sum p z are taken

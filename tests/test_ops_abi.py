@@ -110,6 +110,72 @@ def test_append_refusals(change, what):
     refused("emmy_ops_cache4_append", append(**change), what)
 
 
-@pytest.mark.parametrize("entry", ["emmy_ops_residual_norm", "emmy_ops_rotary", "emmy_ops_cache4_append"])
+def attend(**change):
+    import emmyrt
+    a = dict(cache_k=1 << 20, cache_v=2 << 20, cache_k_meta=3 << 20, cache_v_meta=4 << 20, cache_pages=4, cache_heads=2,
+             cache_page=16, cache_dim=64, q=5 << 20, out=6 << 20, table=7 << 20, lengths=8 << 20, workspace=9 << 20,
+             workspace_bytes=1 << 40, q_batch=256, q_token=256, q_head=64, out_batch=256, out_token=256, out_head=64,
+             table_stride=2, batch=3, tokens=1, q_heads=4, max_pages=2, dtype=2, scale=1.0)
+    return emmyrt.Cache4AttendArgs(**{**a, **change})
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(cache_dim=32), "head dim"), (dict(dtype=0), "f16 or bf16"), (dict(batch=-1), "batch"), (dict(batch=4097), "batch"),
+    (dict(tokens=-1), "tokens"), (dict(q_heads=0), "heads"), (dict(q_heads=3), "heads"), (dict(tokens=1 << 20, q_heads=8), "tokens"),
+    (dict(max_pages=-1), "pages"), (dict(max_pages=1 << 30), "pages"), (dict(q=0), "needed"), (dict(table=0), "needed"),
+    (dict(workspace=0), "workspace"), (dict(workspace=(9 << 20) + 8), "workspace"), (dict(q=(5 << 20) + 1), "aligned"),
+    (dict(lengths=(8 << 20) + 2), "aligned"), (dict(batch=4096, cache_heads=4096, q_heads=4096, max_pages=1 << 20), "too many")])
+def test_attend_refusals(change, what):
+    refused("emmy_ops_cache4_attend", attend(**change), what)
+
+
+def test_attend_workspace_of_an_unknown_dim():
+    import emmyrt
+    n = ctypes.c_uint64()
+    assert emmyrt.ops_lib().emmy_ops_cache4_attend_workspace(96, 0, ctypes.byref(n)) == -3
+    assert emmyrt.ops_lib().emmy_ops_cache4_attend_workspace(64, 0, None) == -3
+
+
+def product(**change):
+    import emmyrt
+    a = dict(xq=1 << 20, xs=2 << 20, wq=3 << 20, ws=4 << 20, y=5 << 20, status=6 << 20, xq_stride=144, xs_stride=8, wq_stride=144,
+             ws_stride=2, y_stride=10, m=8, n=10, k=130, dtype=2)
+    return emmyrt.BlockFp8Args(**{**a, **change})
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(dtype=4), "element type"), (dict(n=0), "n 0"), (dict(m=-1), "xq"), (dict(k=0), "xq"), (dict(xq=0), "xq"),
+    (dict(xq=(1 << 20) + 8), "xq"), (dict(xq_stride=136), "xq"), (dict(xq_stride=128), "xq"), (dict(k=143, wq_stride=160, xq_stride=128), "xq"),
+    (dict(wq_stride=136), "wq"), (dict(wq=(3 << 20) + 1), "wq"), (dict(xs=0), "xs"), (dict(xs_stride=7), "xs"), (dict(xs_stride=10), "xs"),
+    (dict(ws_stride=1, n=300, y_stride=300), "overlap"), (dict(y_stride=9), "overlap"), (dict(y=(5 << 20) + 1), "y"), (dict(status=0), "status"),
+    (dict(parts=(7 << 20) + 4, parts_bytes=64), "parts"), (dict(m=0x7fffff00, n=0x7fffff00, y_stride=0x7fffff00, xs_stride=0x7fffff00), "y of")])
+def test_product_refusals(change, what):
+    refused("emmy_ops_blockfp8_product", product(**change), what)
+
+
+def quantise(**change):
+    import emmyrt
+    a = dict(x=1 << 20, q=2 << 20, s=3 << 20, x_stride=130, q_stride=144, s_stride=8, rows=8, cols=130, dtype=2)
+    return emmyrt.BlockFp8QuantizeArgs(**{**a, **change})
+
+
+@pytest.mark.parametrize("change,what", [
+    (dict(dtype=5), "element type"), (dict(rows=-1), "x of"), (dict(cols=0), "x of"), (dict(x=0), "x is needed"),
+    (dict(x=(1 << 20) + 1), "x is needed"), (dict(q=(2 << 20) + 4), "q is needed"), (dict(q_stride=130), "16"), (dict(q_stride=128), "overlap"),
+    (dict(s=2), "s is needed"), (dict(s_stride=7), "overlap"), (dict(square=1, rows=300, s_stride=1), "overlap")])
+def test_quantise_refusals(change, what):
+    refused("emmy_ops_blockfp8_quantize", quantise(**change), what)
+
+
+@pytest.mark.parametrize("change,what", [(dict(x=0), "x is needed"), (dict(x_dtype=7), "element type"), (dict(x_stride=100), "overlap"),
+                                         (dict(x_stride=100, m=2), "overlap"), (dict(wq=0), "wq")])
+def test_linear_refusals(change, what):
+    import emmyrt
+    a = {n: getattr(product(), n) for n, _ in emmyrt.BlockFp8Args._fields_}
+    refused("emmy_ops_blockfp8_linear", emmyrt.BlockFp8LinearArgs(**{**a, "x": 8 << 20, "x_stride": 130, "x_dtype": 2, **change}), what)
+
+
+@pytest.mark.parametrize("entry", ["emmy_ops_residual_norm", "emmy_ops_rotary", "emmy_ops_cache4_append", "emmy_ops_cache4_attend",
+                                   "emmy_ops_blockfp8_quantize", "emmy_ops_blockfp8_product", "emmy_ops_blockfp8_linear"])
 def test_no_arguments(entry):
     refused(entry, None, "no arguments")
