@@ -619,15 +619,9 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
             }
-            /* Nothing may arrive in shared memory that is no longer this block's: the products' last arrivals here, or,
-             * where a wait gave up, the copies under way (a pair's all complete on the leader's barriers; what was never
-             * copied ends by its limit). */
-            if (ok) {
-                for (int i = 0; i < S::STAGES; ++i) {
-                    if (!wait_for(shared_address(&empty[stage]), phase ^ 1, &abort, p.status, 1)) break;
-                    if (++stage == S::STAGES) stage = 0, phase ^= 1;
-                }
-            } else if (rank == 0) {
+            /* Where a wait gave up: nothing may arrive in shared memory that is no longer this block's, so the copies under way
+             * are waited for (a pair's all complete on the leader's barriers; what was never copied ends by its limit). */
+            if (!ok && rank == 0) {
                 const uint64_t start = now_ns();
                 for (int i = 0; i < S::STAGES; ++i) {
                     while (!try_wait(shared_address(&full[stage]), phase ^ 1) && now_ns() - start < TIMEOUT_NS) {}
@@ -649,13 +643,21 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             static_assert(S::STAGES % 2 == 0 && S::BUFFERS % 2 == 0, "every other stage and buffer");
             for (int t = worker; t < tiles && ok; t += workers) {
                 const Unit u = place(t);
+                /* blocks of later tiles, as far as they matter: a stage that is not filled again is not handed back either, so
+                 * that no arrival is under way when the block of threads ends */
+                int rest = 0;
+                for (int later = t + workers; later < tiles && rest < S::STAGES; later += workers) {
+                    const int from = later % p.splits * p.per_split;
+                    rest += min(from + p.per_split, p.k_blocks) - from;
+                }
+                const int hand_back = u.to + rest - S::STAGES;
                 int b = u.from + skip;
                 for (; b < u.to; b += 2) {
                     if (!(ok = wait_for_both(read0 + 8 * buffer, buffer_phase ^ 1, full0 + 8 * stage, phase, &abort, p.status, 2))) break;
                     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
                     multiply_block<PAIR>(base + buffer * BN, a0 + stage * (S::STAGE >> 4), b0 + stage * (S::STAGE >> 4), idesc);
                     commit<PAIR>(summed0 + 8 * buffer);
-                    commit<PAIR>(empty0 + 8 * stage);
+                    if (b < hand_back) commit<PAIR>(empty0 + 8 * stage);
                     if ((stage += 2) >= S::STAGES) stage -= S::STAGES, phase ^= 1;
                     if ((buffer += 2) >= S::BUFFERS) buffer -= S::BUFFERS, buffer_phase ^= 1;
                 }
