@@ -747,7 +747,7 @@ EMMY_EXPORT int emmy_ops_cache4_attend(const emmy_ops_cache4_attend_args *a, int
     p.out_wide = aligned(a->out, 8) && !((p.out_batch | p.out_token | p.out_head) & 3);
     p.batch = a->batch, p.tokens = a->tokens, p.heads = a->cache.heads, p.group = group;
     p.row_groups = (rows + 8 * nt - 1) / (8 * nt), p.page = a->cache.page;
-    p.max_positions = a->max_pages * a->cache.page;
+    p.max_positions = a->cache.pages ? a->max_pages * a->cache.page : 0;     /* nothing to see in a cache without pages */
     p.scale_log2 = (float)(a->scale * 1.4426950408889634);
     if ((int64_t)p.batch * p.heads * p.row_groups > 0x7fffffffLL / ((int64_t)p.max_positions / TILE + 1))
         return ops_fail(EMMY_RT_EINVAL, "%d sequences of %d positions are too many for one call", p.batch, p.max_positions);

@@ -227,10 +227,12 @@ template <typename T, int V, int N> cudaError_t go(NormParams &p, uint64_t strea
 }
 
 /* Accesses of 16 bytes where every row allows them, else of 4, else of one element.  8 elements a thread while the rows
- * do not fill the GPU (they are bound by the chain from load to store) and where accesses are narrow; else 32, over
- * which a row's sums and addresses cost little; 16 in narrow accesses for rows that 1024 threads of 8 would not hold. */
+ * do not fill the GPU (they are bound by the chain from load to store), where accesses are narrow, and up to 128 elements a
+ * row, of which 32 each would leave half of the 8 lanes idle (200000 rows of 64 in bf16: 44 us, 20 with 8 each); else
+ * 32, over which a row's sums and addresses cost little (100000 rows of 200: 44 us, 56 with 8 each); 16 in narrow accesses
+ * for rows that 1024 threads of 8 would not hold. */
 template <typename T> cudaError_t dispatch(NormParams &p, int bytes, uint64_t stream) {
-    const bool many = p.dim > 8192 || p.rows * p.dim > 148 * 4096 * 2;
+    const bool many = p.dim > 8192 || (p.dim > 128 && p.rows * p.dim > 148 * 4096 * 2);
     constexpr int W = 16 / sizeof(T);
     const bool large = p.dim > 8192;
     if (bytes == 16) return many ? go<T, W, 32 / W>(p, stream) : go<T, W, 8 / W>(p, stream);
