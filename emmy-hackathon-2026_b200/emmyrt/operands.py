@@ -185,15 +185,18 @@ class Operator:
         raise NotImplementedError
 
     def _call(self, operands, options, stream: int) -> None:
-        key = [options]
+        key, at = [options], []
         try:
             for x in operands:
                 if x is None:
                     key.append(None)
+                    at.append(0)
                 elif type(x) is Array:
                     key += (x.dtype, x.shape, x.strides, x.device)
+                    at.append(x.ptr)
                 else:
                     key += (x.dtype, x.shape, x.stride(), x.device)
+                    at.append(x.data_ptr())
             key = tuple(key)
             plan = self._plans.get(key)
         except (AttributeError, TypeError):
@@ -204,7 +207,6 @@ class Operator:
                 if len(self._plans) >= self.PLANS:
                     self._plans.clear()
                 self._plans[key] = plan
-        at = [0 if x is None else x.ptr if type(x) is Array else x.data_ptr() for x in operands]
         for i, j, span_i, span_j, check in plan.checks:
             p, q = at[i], at[j]
             if p < q + span_j and q < p + span_i:
