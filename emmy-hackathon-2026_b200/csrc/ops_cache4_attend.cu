@@ -167,6 +167,12 @@ __device__ __forceinline__ float exp2_approx(float x) {
     return y;
 }
 
+__device__ __forceinline__ float reciprocal_approx(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 /* The token that row r (0 .. 7) of an eight-token group stands for.  A warp reads a token's keys by
  * r = lane / 4 and its values by the pairs r = 2 (lane % 4) + {0, 1}; these orders (with the
  * swizzle below at dim 128) put both into different banks. */
@@ -488,7 +494,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
                 const ulonglong2 v = doubled[16 * m + 8 * h + token_of<DIM>(r)].v;
-                const float inverse = EXACT ? 1.0f / Two(v.x).get().x : 0.0f;
+                const float inverse = EXACT ? reciprocal_approx(Two(v.x).get().x) : 0.0f;      /* off by 2^-23: as p itself */
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     const float2 x = fma2(by[n], Two(score[m][n][2 * h], score[m][n][2 * h + 1]), minus[n]).get();
