@@ -59,15 +59,20 @@ template <typename T> __device__ __forceinline__ void load8(const T *x, int64_t 
     }
 }
 
-/* v / s for the eight values of a block's scale.  The eight divisions were most of the kernel: 39 -> 31 us at 4096 x 8192. */
-__device__ __forceinline__ void divide8(float (&v)[8], float s) {
+/* v / s for N values of a block's scale, two at a time.  With divisions the quantiser took 39 us for 4096 x 8192 in bf16, now 20 us
+ * (5.1 TB/s). */
+template <int N> __device__ __forceinline__ void divide(float (&v)[N], float s) {
     if (s >= 0x1p-60f && s <= 0x1p60f) {
         const float r = __frcp_rn(s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = quotient(v[i], s, r);
+        for (int i = 0; i < N; i += 2) {
+            const Two both(v[i], v[i + 1]), q = both * Two(r, r);
+            const float2 f = fma2(fma2(Two(-s, -s), q, both), Two(r, r), q).get();
+            v[i] = f.x, v[i + 1] = f.y;
+        }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = __fdiv_rn(v[i], s);
+        for (int i = 0; i < N; ++i) v[i] = __fdiv_rn(v[i], s);
     }
 }
 
@@ -121,11 +126,16 @@ template <typename T, int A> __global__ void __launch_bounds__(256) quantize_row
             for (int d = 8; d > 0; d >>= 1) largest = max(largest, __shfl_xor_sync(~0u, largest, d));
         }
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = to_f32(x[i][j / A].at[j % A]);
+        for (int j = 0; j < 8; j += A) {
+            float f[A];
+            unpack(x[i][j / A], f);
+#pragma unroll
+            for (int k = 0; k < A; ++k) v[j + k] = f[k];
+        }
         if (i * down >= left || b * BLOCK >= p.cols) continue;
         const float s = scale_of(largest);
         if (lane == 0) scale[i * down] = s;
-        divide8(v, s);
+        divide(v, s);
         if (stores) *(uint2 *)to = make_uint2(e4m3x4(v[0], v[1], v[2], v[3]), e4m3x4(v[4], v[5], v[6], v[7]));
     }
 }
@@ -165,7 +175,7 @@ template <typename T> __global__ void __launch_bounds__(256) quantize_blocks(Qua
     for (int i = 0; i < 8; ++i) {
         const int64_t row = row0 + 16 * i;
         if (row >= p.rows) continue;
-        divide8(v[i], s);
+        divide(v[i], s);
         const uint2 q = make_uint2(e4m3x4(v[i][0], v[i][1], v[i][2], v[i][3]), e4m3x4(v[i][4], v[i][5], v[i][6], v[i][7]));
         uint8_t *to = p.q + row * p.q_stride + e;
         if (e + 8 <= p.cols) {
@@ -284,15 +294,8 @@ template <typename T, int NT, typename X = Quantised> __global__ void __launch_b
 #pragma unroll
                 for (int i = 0; i < 4; ++i) largest = max(largest, magnitude(ahead[m][i]));
                 const float scale = scale_of(__reduce_max_sync(~0u, largest));
-                float v[4];
-                if (scale >= 0x1p-60f && scale <= 0x1p60f) {
-                    const float r = __frcp_rn(scale);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = quotient(ahead[m][i], scale, r);
-                } else {
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) v[i] = __fdiv_rn(ahead[m][i], scale);
-                }
+                float (&v)[4] = ahead[m];
+                divide(v, scale);
                 *(uint32_t *)&s.x[m][((lane >> 2) ^ ((m & 1) * 4)) * 16 + (lane & 3) * 4] = e4m3x4(v[0], v[1], v[2], v[3]);
                 if (lane == 0) s.sx[m] = scale;
             }
