@@ -16,20 +16,6 @@
 
 namespace {
 
-/* a / b for a below 2^31 without a division: the upper half of a * inverse, shifted (exact: inverse = ceil(2^(31 + s) / b) with
- * 2^s >= b); b = 1: inverse = 0 */
-struct Divisor {
-    uint32_t by, inverse, shift;
-    Divisor(uint32_t b = 1) : by(b), inverse(0), shift(0) {
-        if (b == 1) return;
-        uint32_t s = 1;
-        while ((1u << s) < b) ++s;
-        inverse = (uint32_t)((((uint64_t)1 << (31 + s)) + b - 1) / b);
-        shift = s - 1;
-    }
-    __device__ __forceinline__ uint32_t divides(uint32_t a) const { return inverse ? __umulhi(a, inverse) >> shift : a; }
-};
-
 struct AppendParams {
     const char *x[2];
     char *level[2], *stored[2];

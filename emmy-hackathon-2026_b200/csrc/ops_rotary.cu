@@ -22,7 +22,9 @@ struct RotaryParams {
     const void *positions;
     const uint64_t *turns;
     int64_t tokens;
-    int positions_64, pairs, rest, per_block, transpose, copies;
+    int positions_64, rest, per_block, transpose;
+    Divisor pairs, per_head, all_heads;     /* per_head: accesses (of V pairs, or V copied elements) a head */
+    int side;                               /* heads that 256 threads take side by side, or 1 */
     float magnitude;
 };
 
@@ -36,13 +38,13 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
     enter_grid();
     const int64_t first = (int64_t)blockIdx.x * p.per_block;
     const int live = (int)min((int64_t)p.per_block, p.tokens - first);
-    const int units = p.pairs / V, per_head = units + (p.copies ? p.rest / V : 0), heads = p.heads[0] + p.heads[1];
-    const int side = per_head < (int)blockDim.x ? blockDim.x / per_head : 1;      /* heads side by side */
-    const int own = threadIdx.x / per_head, second = HALF ? p.pairs : V;          /* from an access to its partner */
+    const int pairs = p.pairs.by, units = pairs / V, per_head = p.per_head.by, heads = p.all_heads.by, side = p.side;
+    const int own = p.per_head.divides(threadIdx.x), second = HALF ? pairs : V;    /* from an access to its partner */
     struct Item {
         int token, head;
     };
-    Item next = {own / heads, own % heads};
+    const int over = p.all_heads.divides(own);
+    Item next = {over, own - over * heads};
     if (own >= side) next.token = live;                         /* no place: nothing to do */
     auto advance = [&] {
         next.head += side;
@@ -51,7 +53,7 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
     int unit = threadIdx.x - own * per_head;
     Item item[AT_ONCE];
     Pack<T, V> a[AT_ONCE], b[AT_ONCE];
-    auto element = [&] { return unit >= units ? 2 * p.pairs + (unit - units) * V : HALF ? unit * V : 2 * unit * V; };
+    auto element = [&] { return unit >= units ? 2 * pairs + (unit - units) * V : HALF ? unit * V : 2 * unit * V; };
     auto load = [&] {
 #pragma unroll
         for (int i = 0; i < AT_ONCE; ++i) {
@@ -66,8 +68,8 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
         }
     };
     load();
-    for (int i = threadIdx.x; i < live * p.pairs; i += blockDim.x) {
-        const int token = i / p.pairs, pair = i - token * p.pairs;
+    for (int i = threadIdx.x; i < live * pairs; i += blockDim.x) {
+        const int token = p.pairs.divides(i), pair = i - token * pairs;
         const int64_t position = p.positions_64 ? ((const int64_t *)p.positions)[first + token]
                                                 : ((const int32_t *)p.positions)[first + token];
         const uint64_t turn = (uint64_t)position * p.turns[pair];
@@ -87,7 +89,7 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
                     *(Pack<T, V> *)out = a[i];
                     continue;
                 }
-                const float2 *cs = table + item[i].token * p.pairs + unit * V;
+                const float2 *cs = table + item[i].token * pairs + unit * V;
                 float u[V], v[V], ru[V], rv[V];
                 unpack(a[i], u);
                 unpack(b[i], v);
@@ -116,17 +118,20 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
     }
 }
 
-template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, uint64_t stream) {
+template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, bool copies, uint64_t stream) {
     /* tokens a block: about two (token, head) pairs for each of its 256 threads where there are many tokens, one token
      * where there are few, as long as the table fits 32 KB */
-    const int64_t per_token = (int64_t)(p.heads[0] + p.heads[1]) * (p.pairs / V + (p.copies ? p.rest / V : 0));
+    const int pairs = p.pairs.by, per_head = pairs / V + (copies ? p.rest / V : 0);
+    p.per_head = Divisor(per_head), p.all_heads = Divisor(p.heads[0] + p.heads[1]);
+    p.side = per_head < 256 ? 256 / per_head : 1;
+    const int64_t per_token = (int64_t)(p.heads[0] + p.heads[1]) * per_head;
     int64_t per = (512 + per_token / 2) / per_token;
-    const int64_t spread = p.tokens / (148 * 4), most = 32768 / ((int64_t)p.pairs * 8);
+    const int64_t spread = p.tokens / (148 * 4), most = 32768 / ((int64_t)pairs * 8);
     if (per > spread) per = spread;
     if (per > most) per = most;
     p.per_block = per < 1 ? 1 : (int)per;
     const dim3 grid((unsigned)((p.tokens + p.per_block - 1) / p.per_block));
-    const size_t smem = (size_t)p.per_block * p.pairs * 8;
+    const size_t smem = (size_t)p.per_block * pairs * 8;
     return layout == EMMY_OPS_ROTARY_HALF ? launch(rotary<T, V, true>, grid, dim3(256), smem, stream, p)
                                           : launch(rotary<T, V, false>, grid, dim3(256), smem, stream, p);
 }
@@ -149,6 +154,7 @@ EMMY_EXPORT int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint6
     const int es = elem_size(a->dtype);
     RotaryParams p = {};
     int bytes = 16;
+    bool copies = false;
     for (int i = 0; i < 2; ++i) {
         p.heads[i] = a->heads[i];
         if (!a->heads[i]) continue;
@@ -165,11 +171,12 @@ EMMY_EXPORT int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint6
         p.out[i] = (char *)(uintptr_t)a->out[i];
         p.x_token[i] = a->x_token[i], p.x_head[i] = a->x_head[i];
         p.out_token[i] = a->out_token[i], p.out_head[i] = a->out_head[i];
-        p.copies |= a->x[i] != a->out[i] || a->x_token[i] != a->out_token[i] || a->x_head[i] != a->out_head[i];
+        copies |= a->x[i] != a->out[i] || a->x_token[i] != a->out_token[i] || a->x_head[i] != a->out_head[i];
     }
-    p.pairs = a->rotary / 2;
+    const int pairs = a->rotary / 2;
+    p.pairs = Divisor(pairs);
     p.rest = a->dim - a->rotary;
-    while (bytes > es && (p.pairs % (bytes / es) || p.rest % (bytes / es))) bytes = bytes == 16 && es == 2 ? 4 : es;
+    while (bytes > es && (pairs % (bytes / es) || p.rest % (bytes / es))) bytes = bytes == 16 && es == 2 ? 4 : es;
     p.positions = (const void *)(uintptr_t)a->positions;
     p.turns = (const uint64_t *)(uintptr_t)a->turns;
     p.tokens = a->tokens, p.positions_64 = a->positions_64 != 0, p.transpose = a->transpose != 0;
@@ -178,14 +185,14 @@ EMMY_EXPORT int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint6
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
     cudaError_t e;
     if (a->dtype == EMMY_OPS_F32)
-        e = bytes == 16 ? go<float, 4>(p, a->layout, stream) : go<float, 1>(p, a->layout, stream);
+        e = bytes == 16 ? go<float, 4>(p, a->layout, copies, stream) : go<float, 1>(p, a->layout, copies, stream);
     else if (a->dtype == EMMY_OPS_F16)
-        e = bytes == 16  ? go<__half, 8>(p, a->layout, stream)
-            : bytes == 4 ? go<__half, 2>(p, a->layout, stream)
-                         : go<__half, 1>(p, a->layout, stream);
+        e = bytes == 16  ? go<__half, 8>(p, a->layout, copies, stream)
+            : bytes == 4 ? go<__half, 2>(p, a->layout, copies, stream)
+                         : go<__half, 1>(p, a->layout, copies, stream);
     else
-        e = bytes == 16  ? go<__nv_bfloat16, 8>(p, a->layout, stream)
-            : bytes == 4 ? go<__nv_bfloat16, 2>(p, a->layout, stream)
-                         : go<__nv_bfloat16, 1>(p, a->layout, stream);
+        e = bytes == 16  ? go<__nv_bfloat16, 8>(p, a->layout, copies, stream)
+            : bytes == 4 ? go<__nv_bfloat16, 2>(p, a->layout, copies, stream)
+                         : go<__nv_bfloat16, 1>(p, a->layout, copies, stream);
     return ops_cuda(e, "rotary");
 }
