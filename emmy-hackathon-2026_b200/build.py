@@ -81,10 +81,23 @@ def build_ops(verbose: bool = False) -> Path:
     return out
 
 
+def build_calls(verbose: bool = False) -> Path:
+    """``emmyrt/_calls.so``: the operators' calls from Python (csrc/calls.c)."""
+    import sysconfig
+    out = PKG / "emmyrt" / "_calls.so"
+    cmd = ["gcc", "-O2", "-fPIC", "-shared", "-fvisibility=hidden", "-Wall", "-Wextra", "-Werror",
+           f"-I{sysconfig.get_paths()['include']}", str(PKG / "csrc" / "calls.c"), "-o", str(out)]
+    if verbose:
+        print(" ".join(cmd))
+    subprocess.run(cmd, check=True)
+    return out
+
+
 def main() -> int:
     build_runtime(verbose=True)
     build_static_scratch(verbose=True)
     build_ops(verbose=True)
+    build_calls(verbose=True)
     print("built", PKG / "emmyrt" / "libemmyrt.so")
     return 0
 

@@ -10,7 +10,7 @@ from __future__ import annotations
 import numpy as np
 
 from . import BlockFp8LinearArgs, BlockFp8QuantizeArgs, DeviceBuffer, check, lib
-from .operands import CODE, FLOATS, Array, Operator, Plan, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, Array, Operator, operand, overlaps, shaped, written
 
 BLOCK = 128
 
@@ -37,7 +37,7 @@ class BlockFp8Quantizer(Operator):
         [blocks of cols, rows], with ``square`` [blocks of rows, blocks of cols]."""
         self._call((x, q, s), None, stream)
 
-    def _plan(self, operands, options) -> Plan:
+    def _plan(self, operands, options) -> tuple:
         d = self.device
         x = operand(operands[0], "x", FLOATS, 2, d)
         rows, cols = x.shape
@@ -50,7 +50,7 @@ class BlockFp8Quantizer(Operator):
         a = BlockFp8QuantizeArgs(x_stride=x.strides[0], q_stride=_stride(q), s_stride=s.strides[0], rows=rows, cols=cols,
                                  dtype=CODE[x.dtype], square=self.square)
         checks = overlaps([(1, _with_padding(q) if not self.square else q, "q"), (2, s, "s")], [(0, x, "x")])
-        return Plan("emmy_ops_blockfp8_quantize", a, ("x", "q", "s"), checks)
+        return "emmy_ops_blockfp8_quantize", a, ("x", "q", "s"), checks
 
 
 def _padded(q: Array, name: str) -> Array:
@@ -133,9 +133,9 @@ class BlockFp8Linear(Operator):
 
     def __call__(self, x, y, *, stream: int = 0) -> None:
         """``x`` [rows, k] and ``y`` [rows, n], each f32, f16 or bf16."""
-        self._call((x, y, self.wq, self.ws), None, stream)
+        self._call((x, y), None, stream)
 
-    def _plan(self, operands, options) -> Plan:
+    def _plan(self, operands, options) -> tuple:
         d = self.device
         x = operand(operands[0], "x", FLOATS, 2, d)
         rows = x.shape[0]
@@ -144,9 +144,10 @@ class BlockFp8Linear(Operator):
         if rows > self.max_rows:
             raise ValueError(f"{rows} rows, the operator was made for {self.max_rows}")
         y = written(shaped(operand(operands[1], "y", FLOATS, 2, d), "y", (rows, self.n)), "y")
-        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, status=self._status, parts=self._parts if self._parts_bytes else 0,
-                               parts_bytes=self._parts_bytes, xq_stride=pitch(self.k), xs_stride=self._xs_stride,
-                               wq_stride=_stride(self.wq), ws_stride=self.ws.strides[0], y_stride=y.strides[0], m=rows,
-                               n=self.n, k=self.k, dtype=CODE[y.dtype], x_stride=x.strides[0], x_dtype=CODE[x.dtype])
+        a = BlockFp8LinearArgs(xq=self._xq, xs=self._xs, wq=self.wq.ptr, ws=self.ws.ptr, status=self._status,
+                               parts=self._parts if self._parts_bytes else 0, parts_bytes=self._parts_bytes,
+                               xq_stride=pitch(self.k), xs_stride=self._xs_stride, wq_stride=_stride(self.wq),
+                               ws_stride=self.ws.strides[0], y_stride=y.strides[0], m=rows, n=self.n, k=self.k,
+                               dtype=CODE[y.dtype], x_stride=x.strides[0], x_dtype=CODE[x.dtype])
         checks = overlaps([(1, y, "y")], [(0, x, "x"), (2, self.wq, "wq"), (3, self.ws, "ws")])
-        return Plan("emmy_ops_blockfp8_linear", a, ("x", "y", "wq", "ws"), checks)
+        return "emmy_ops_blockfp8_linear", a, ("x", "y"), checks, (self.wq, self.ws)

@@ -10,7 +10,7 @@ import ctypes
 import math
 
 from . import Cache4AppendArgs, Cache4AttendArgs, DeviceBuffer, EmmyRTError, ops_lib
-from .operands import CODE, FLOATS, INDICES, Array, Operator, Plan, apart, contiguous, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, INDICES, Array, Operator, apart, contiguous, operand, overlaps, shaped, written
 
 DIMS = (64, 128)
 
@@ -49,24 +49,27 @@ class Cache4(Operator):
             made.append(Array(buffer, dtype, (pages, heads, page, last)))
         return cls(*made)
 
+    def _held(self) -> dict:
+        return dict(cache_k=self.k.ptr, cache_v=self.v.ptr, cache_k_meta=self.k_meta.ptr, cache_v_meta=self.v_meta.ptr,
+                    cache_pages=self.pages, cache_heads=self.heads, cache_page=self.page, cache_dim=self.dim)
+
     def append(self, k, v, slots, *, k_stored=None, v_stored=None, stream: int = 0) -> None:
         """Quantises ``k`` and ``v`` [tokens, heads, dim] into ``slots`` [tokens] (int32 or int64).  A token whose slot is
         negative or past the cache is left out (padding); two tokens of one call must not have the same slot.
         ``k_stored`` / ``v_stored`` receive the values that the cache then stands for, in the operands' type."""
-        self._call((k, v, slots, k_stored, v_stored, *self.arrays), None, stream)
+        self._call((k, v, slots, k_stored, v_stored), None, stream)
 
-    _FIELDS = ("k", "v", "slots", "k_stored", "v_stored", "cache_k", "cache_v", "cache_k_meta", "cache_v_meta")
+    _FIELDS = ("k", "v", "slots", "k_stored", "v_stored")
 
-    def _plan(self, operands, options) -> Plan:
-        k, v, slots, k_stored, v_stored = operands[:5]
+    def _plan(self, operands, options) -> tuple:
+        k, v, slots, k_stored, v_stored = operands
         d = self.device
         k = operand(k, "k", FLOATS, 3, d)
         n = k.shape[0]
         shaped(k, "k", (n, self.heads, self.dim))
         v = shaped(operand(v, "v", (k.dtype,), 3, d), "v", k.shape)
         slots = shaped(operand(slots, "slots", INDICES, 1, d), "slots", (n,))
-        a = Cache4AppendArgs(cache_pages=self.pages, cache_heads=self.heads, cache_page=self.page, cache_dim=self.dim,
-                             k_token=k.strides[0], k_head=k.strides[1], v_token=v.strides[0],
+        a = Cache4AppendArgs(**self._held(), k_token=k.strides[0], k_head=k.strides[1], v_token=v.strides[0],
                              v_head=v.strides[1], tokens=n, slots_64=slots.dtype == "i64", dtype=CODE[k.dtype])
         ins, outs = [(0, k, "k"), (1, v, "v"), (2, slots, "slots")], []
         for place, name, out in ((3, "k_stored", k_stored), (4, "v_stored", v_stored)):
@@ -76,7 +79,7 @@ class Cache4(Operator):
         checks = overlaps(outs, ins)
         for part in held:
             checks += overlaps([part], ins + outs)
-        return Plan("emmy_ops_cache4_append", a, self._FIELDS, checks)
+        return "emmy_ops_cache4_append", a, self._FIELDS, checks, self.arrays
 
 
 class Cache4Attention(Operator):
@@ -106,12 +109,12 @@ class Cache4Attention(Operator):
         to its own; a query that sees nothing gives zeros.  Lengths beyond the table are cut there; pages that are none
         are not seen.  ``scale`` is 1 / sqrt(dim) by default.  ``out`` may be ``q``."""
         scale = self.cache.dim ** -0.5 if scale is None else float(scale)
-        self._call((q, out, table, lengths, *self.cache.arrays), scale, stream)
+        self._call((q, out, table, lengths), scale, stream)
 
-    _FIELDS = ("q", "out", "table", "lengths", "cache_k", "cache_v", "cache_k_meta", "cache_v_meta")
+    _FIELDS = ("q", "out", "table", "lengths")
 
-    def _plan(self, operands, scale) -> Plan:
-        q, out, table, lengths = operands[:4]
+    def _plan(self, operands, scale) -> tuple:
+        q, out, table, lengths = operands
         c, d = self.cache, self.device
         if not math.isfinite(scale):
             raise ValueError(f"scale {scale}")
@@ -123,11 +126,10 @@ class Cache4Attention(Operator):
         if table.shape[0] != batch:
             raise ValueError(f"table has {table.shape[0]} rows for {batch} sequences")
         lengths = shaped(operand(lengths, "lengths", ("i32",), 1, d), "lengths", (batch,))
-        a = Cache4AttendArgs(cache_pages=c.pages, cache_heads=c.heads, cache_page=c.page, cache_dim=c.dim,
-                             workspace=self._workspace.ptr, workspace_bytes=self._workspace.nbytes, q_batch=q.strides[0],
-                             q_token=q.strides[1], q_head=q.strides[2], out_batch=out.strides[0], out_token=out.strides[1],
-                             out_head=out.strides[2], table_stride=table.strides[0], batch=batch, tokens=tokens,
-                             q_heads=self.q_heads, max_pages=table.shape[1], dtype=CODE[q.dtype], scale=scale)
+        a = Cache4AttendArgs(**c._held(), workspace=self._workspace.ptr, workspace_bytes=self._workspace.nbytes,
+                             q_batch=q.strides[0], q_token=q.strides[1], q_head=q.strides[2], out_batch=out.strides[0],
+                             out_token=out.strides[1], out_head=out.strides[2], table_stride=table.strides[0], batch=batch,
+                             tokens=tokens, q_heads=self.q_heads, max_pages=table.shape[1], dtype=CODE[q.dtype], scale=scale)
         others = [(0, q, "q"), (2, table, "table"), (3, lengths, "lengths")]
         others += [(4 + i, part, "the cache") for i, part in enumerate(c.arrays)]
-        return Plan("emmy_ops_cache4_attend", a, self._FIELDS, overlaps([(1, out, "out")], others, same=((1, 0),)))
+        return "emmy_ops_cache4_attend", a, self._FIELDS, overlaps([(1, out, "out")], others, same=((1, 0),)), c.arrays

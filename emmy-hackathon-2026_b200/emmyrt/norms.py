@@ -10,7 +10,7 @@ from __future__ import annotations
 import math
 
 from . import NormArgs
-from .operands import CODE, FLOATS, Operator, Plan, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, Operator, operand, overlaps, shaped, written
 
 KINDS = {"rms": 0, "layer": 1}
 MAX_DIM = 16384
@@ -43,7 +43,7 @@ class ResidualNorm(Operator):
 
     _FIELDS = ("x", "block", "y", "h", "post_weight", "post_bias", "gate", "pre_weight", "pre_bias")
 
-    def _plan(self, operands, rows_per_gate) -> Plan:
+    def _plan(self, operands, rows_per_gate) -> tuple:
         x, block, y, h, post_weight, post_bias, gate, pre_weight, pre_bias = operands
         d = self.device
         x = operand(x, "x", FLOATS, 2, d)
@@ -80,4 +80,4 @@ class ResidualNorm(Operator):
             vectors.append((6, gate, "gate"))
         checks = overlaps([(2, y, "y"), (3, h, "h")], [(0, x, "x"), (1, block, "block"), *vectors],
                           same=((2, 0), (2, 1), (3, 0), (3, 1)))
-        return Plan("emmy_ops_residual_norm", a, self._FIELDS, checks)
+        return "emmy_ops_residual_norm", a, self._FIELDS, checks

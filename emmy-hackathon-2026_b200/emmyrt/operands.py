@@ -10,7 +10,7 @@ from __future__ import annotations
 
 import ctypes
 
-from . import EmmyRTError, current_device, ops_lib
+from . import EmmyRTError, _calls, current_device, ops_lib
 
 CODE = {"f32": 0, "f16": 1, "bf16": 2}
 ITEMSIZE = {"f32": 4, "f16": 2, "bf16": 2, "e4m3": 1, "u8": 1, "i32": 4, "i64": 8, "f64": 8, "u64": 8}
@@ -50,6 +50,9 @@ class Array:
         held = getattr(at, "nbytes", None)
         if held is not None and span(self) > held:
             raise ValueError(f"{span(self)} bytes of {dtype} {self.shape} in a buffer of {held}")
+
+
+_calls.set_array(Array)
 
 
 def span(a: Array) -> int:
@@ -159,16 +162,13 @@ def own_device() -> int:
     return current_device()
 
 
-class Plan:
-    """What calls with operands of the same types, shapes and strides have in common: the argument block without its
-    addresses (``fields`` names them, one for each operand) and the overlaps to look for."""
-
-    __slots__ = ("entry", "name", "args", "type", "fields", "checks")
-
-    def __init__(self, name: str, args: ctypes.Structure, fields, checks):
-        self.name, self.entry, self.args, self.type = name, getattr(ops_lib(), name), args, type(args)
-        self.fields = fields
-        self.checks = [(c.i, c.j, c.span_i, c.span_j, c) for c in checks if c.span_i and c.span_j]
+def plan(name: str, args: ctypes.Structure, fields, checks, own=()) -> "_calls.Plan":
+    """What calls with operands of the same types, shapes and strides have in common: the entry, the argument block without
+    the operands' addresses (``fields`` names them, one for each operand) and the overlaps to look for.  ``own``: the
+    operator's own arrays, whose places come after the operands'."""
+    entry = ctypes.cast(getattr(ops_lib(), name), ctypes.c_void_p).value
+    wanted = [(c.i, c.j, c.span_i, c.span_j, c.meets) for c in checks if c.span_i and c.span_j]
+    return _calls.Plan(entry, bytes(args), tuple(getattr(type(args), f).offset for f in fields), tuple(a.ptr for a in own), wanted)
 
 
 class Operator:
@@ -181,42 +181,22 @@ class Operator:
         self.device = own_device()
         self._plans: dict = {}
 
-    def _plan(self, operands, options) -> Plan:
+    def _plan(self, operands, options) -> tuple:
+        """The arguments of :func:`plan` for a call, or a ``ValueError`` that says what is wrong with it."""
         raise NotImplementedError
 
     def _call(self, operands, options, stream: int) -> None:
-        key, at = [options], []
-        try:
-            for x in operands:
-                if x is None:
-                    key.append(None)
-                    at.append(0)
-                elif type(x) is Array:
-                    key += (x.dtype, x.shape, x.strides, x.device)
-                    at.append(x.ptr)
-                else:
-                    key += (x.dtype, x.shape, x.stride(), x.device)
-                    at.append(x.data_ptr())
-            key = tuple(key)
-            plan = self._plans.get(key)
-        except (AttributeError, TypeError):
-            plan = key = None       # the full check says what is wrong
-        if plan is None:
-            plan = self._plan(operands, options)
-            if key is not None:
-                if len(self._plans) >= self.PLANS:
-                    self._plans.clear()
-                self._plans[key] = plan
-        for i, j, span_i, span_j, check in plan.checks:
-            p, q = at[i], at[j]
-            if p < q + span_j and q < p + span_i:
-                check.meets(p, q)
-        args = plan.type.from_buffer_copy(plan.args)
-        for field, p in zip(plan.fields, at):
-            setattr(args, field, p)
-        status = plan.entry(ctypes.byref(args), self.device, stream)
+        status = _calls.call(self._plans, operands, options, self.device, stream)
+        while type(status) is not int:      # the call's kind, which the plans do not have (yet, or any more)
+            what = self._plan(operands, options)
+            if status is None:
+                raise ValueError("an operand is neither an Array nor a tensor")
+            if len(self._plans) >= self.PLANS:
+                self._plans.clear()
+            self._plans[status] = plan(*what)
+            status = _calls.call(self._plans, operands, options, self.device, stream)
         if status:
-            raise EmmyRTError(status, plan.name, ops_lib().emmy_ops_last_error().decode(errors="replace"))
+            raise EmmyRTError(status, type(self).__name__, ops_lib().emmy_ops_last_error().decode(errors="replace"))
 
 
 def overlaps(outs, others, *, same=()) -> list:

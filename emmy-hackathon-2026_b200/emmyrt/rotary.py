@@ -12,7 +12,7 @@ import math
 import numpy as np
 
 from . import DeviceBuffer, RotaryArgs
-from .operands import CODE, FLOATS, INDICES, Operator, Plan, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, INDICES, Operator, operand, overlaps, shaped, written
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = ("none", "linear", "base", "parts")
@@ -87,7 +87,7 @@ class Rotary(Operator):
 
     _FIELDS = ("positions", "x0", "x1", "out0", "out1")
 
-    def _plan(self, operands, inverse) -> Plan:
+    def _plan(self, operands, inverse) -> tuple:
         d = self.device
         positions = operand(operands[0], "positions", INDICES, 1, d)
         n = positions.shape[0]
@@ -112,4 +112,4 @@ class Rotary(Operator):
             ins.append((1 + i, v, name))
             outs.append((3 + i, o, name + "_out"))
         a.dtype = CODE[dtype]
-        return Plan("emmy_ops_rotary", a, self._FIELDS, overlaps(outs, ins, same=((3, 1), (4, 2))))
+        return "emmy_ops_rotary", a, self._FIELDS, overlaps(outs, ins, same=((3, 1), (4, 2)))

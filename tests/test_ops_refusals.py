@@ -1,6 +1,8 @@
 """What the operators' Python side refuses before anything is enqueued, on the CPU: operands are made-up addresses, and the
 library's entries are replaced by one that records its call."""
 
+import ctypes
+
 import pytest
 
 
@@ -46,21 +48,28 @@ def calls(monkeypatch):
 
         zero = upload
 
-    class Lib:
-        def __getattr__(self, name):
-            def entry(args, *rest):
-                if name.endswith("workspace"):
-                    rest[-1]._obj.value = 1 << 20
-                else:
-                    made.append((name, args._obj))
-                return 0
-            return entry
+    kinds = {"emmy_ops_residual_norm": emmyrt.NormArgs, "emmy_ops_rotary": emmyrt.RotaryArgs,
+             "emmy_ops_cache4_append": emmyrt.Cache4AppendArgs, "emmy_ops_cache4_attend": emmyrt.Cache4AttendArgs,
+             "emmy_ops_blockfp8_quantize": emmyrt.BlockFp8QuantizeArgs, "emmy_ops_blockfp8_linear": emmyrt.BlockFp8LinearArgs}
 
+    class Lib:
+        def __init__(self):
+            for name, kind in kinds.items():
+                def entry(args, device, stream, name=name, kind=kind):
+                    made.append((name, kind.from_buffer_copy(ctypes.string_at(args, ctypes.sizeof(kind)))))
+                    return 0
+                setattr(self, name, ctypes.CFUNCTYPE(ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_uint64)(entry))
+
+        def emmy_ops_cache4_attend_workspace(self, dim, device, need):
+            need._obj.value = 1 << 20
+            return 0
+
+    library = Lib()
     for module in (emmyrt.blockfp8, emmyrt.cache4, emmyrt.rotary):
         monkeypatch.setattr(module, "DeviceBuffer", Buffer)
     monkeypatch.setattr(emmyrt.operands, "current_device", lambda: 0)
-    monkeypatch.setattr(emmyrt.operands, "ops_lib", lambda: Lib())
-    monkeypatch.setattr(emmyrt.cache4, "ops_lib", lambda: Lib())
+    monkeypatch.setattr(emmyrt.operands, "ops_lib", lambda: library)
+    monkeypatch.setattr(emmyrt.cache4, "ops_lib", lambda: library)
     monkeypatch.setattr(emmyrt.blockfp8.BlockFp8Linear, "_clear_status", lambda self: None)
     return made
 
