@@ -204,12 +204,11 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-/* 16 rows of W a block of threads; its 8 warps take every eighth block of 128 columns and join at the end.  W and x come
+/* 16 rows of W a block of threads; its 8 or 16 warps take every 8th or 16th block of 128 columns and join at the end.  W and x come
  * through a ring of asynchronous copies in shared memory, FEW_STAGES blocks of a warp ahead: what is under way decides the rate
  * at so little work a byte, and registers for it would halve what runs at once.  A thread takes 16 consecutive bytes of a row;
  * the order of the columns inside a product is the same for x and W, and free.  W's bytes bound it, and at more than
  * 4 rows the conversions of e4m3 that mma.sync is made of here. */
-constexpr int FEW_WARPS = 8;
 template <int NT> struct alignas(16) FewStage {
     unsigned char w[16][BLOCK], x[8 * NT][BLOCK];
     float sx[8 * NT], sw, unused[3];
@@ -223,12 +222,12 @@ __device__ __forceinline__ void copy_async16(const void *shared, const void *fro
                  ::"r"((uint32_t)__cvta_generic_to_shared(shared)), "l"(from), "r"(bytes) : "memory");
 }
 
-/* X: the type of an x that is not quantised yet, of up to 2 rows: each warp quantises what it takes, 4 elements a lane, which
+/* X: the type of an x that is not quantised yet, of up to 2 rows: a warp quantises what it takes, 4 elements a lane, which
  * saves the launch of the quantiser (1 x 4321 x 648: 4.4 -> 3.0 us).  Quantised: p.x and p.sx have it. */
 struct Quantised {};
 constexpr int FUSED_ROWS = 2;
 
-template <typename T, int NT, typename X = Quantised> __global__ void __launch_bounds__(256) few_rows(FewParams p) {
+template <typename T, int NT, typename X, int FEW_WARPS> __global__ void __launch_bounds__(32 * FEW_WARPS) few_rows(FewParams p) {
     constexpr int STAGES = FEW_STAGES;
     constexpr bool FUSED = !__is_same(X, Quantised);
     extern __shared__ __align__(128) unsigned char raw[];           /* [warps][stages] */
@@ -352,7 +351,7 @@ template <typename T, int NT, typename X = Quantised> __global__ void __launch_b
 #pragma unroll
         for (int i = 0; i < 4; ++i) parts[warp][r + 8 * (i >> 1)][8 * t + 2 * c + (i & 1)] = acc[t][i];
     __syncthreads();
-    for (int i = threadIdx.x; i < 16 * 8 * NT; i += 256) {
+    for (int i = threadIdx.x; i < 16 * 8 * NT; i += 32 * FEW_WARPS) {
         const int n = i & 15, m = i >> 4;
         if (m >= p.m || n0 + n >= p.n) continue;
         float s = 0.0f;
@@ -362,18 +361,25 @@ template <typename T, int NT, typename X = Quantised> __global__ void __launch_b
     }
 }
 
-template <typename T, int NT, typename X = Quantised> cudaError_t go_few(FewParams p, int device, uint64_t stream) {
+template <typename T, int NT, typename X, int WARPS> cudaError_t go_warps(FewParams p, int device, uint64_t stream) {
     static uint64_t allowed;
-    constexpr size_t STAGE = FEW_WARPS * sizeof(FewStage<NT>);
+    constexpr size_t STAGE = WARPS * sizeof(FewStage<NT>);
     if (!(__atomic_load_n(&allowed, __ATOMIC_ACQUIRE) >> device & 1)) {
-        cudaError_t e = cudaFuncSetAttribute(few_rows<T, NT, X>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_STAGES * STAGE);
+        cudaError_t e = cudaFuncSetAttribute(few_rows<T, NT, X, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, FEW_STAGES * STAGE);
         if (e != cudaSuccess) return e;
         __atomic_fetch_or(&allowed, 1ull << device, __ATOMIC_RELEASE);
     }
     /* as many stages as a warp has blocks, up to all: short rows leave the room to more blocks of threads */
-    const int steps = ((p.k + BLOCK - 1) / BLOCK + FEW_WARPS - 1) / FEW_WARPS;
+    const int steps = ((p.k + BLOCK - 1) / BLOCK + WARPS - 1) / WARPS;
     p.stages = steps < FEW_STAGES ? steps : FEW_STAGES;
-    return launch(few_rows<T, NT, X>, dim3((unsigned)((p.n + 15) / 16)), dim3(256), p.stages * STAGE, stream, p);
+    return launch(few_rows<T, NT, X, WARPS>, dim3((unsigned)((p.n + 15) / 16)), dim3(32 * WARPS), p.stages * STAGE, stream, p);
+}
+/* 16 warps a block of threads where there is a block for each SM at most, and rows have more than 8 blocks of 128 to share: 1 x 1024 x
+ * 8192 takes 6.7 us, with 8 warps 9.8; 8 x 1321 x 6450 7.3 and 9.9; where SMs hold several blocks 8 warps are as fast. */
+template <typename T, int NT, typename X = Quantised> cudaError_t go_few(const FewParams &p, int device, uint64_t stream) {
+    int sms;
+    if (ops_sm_count(device, &sms)) return cudaErrorInvalidDevice;
+    return p.n <= 16 * sms && p.k > 8 * BLOCK ? go_warps<T, NT, X, 16>(p, device, stream) : go_warps<T, NT, X, 8>(p, device, stream);
 }
 
 /* ---- many rows of x: tcgen05 ------------------------------------------------------------ */
