@@ -1011,9 +1011,10 @@ EMMY_EXPORT int emmy_ops_blockfp8_linear(const emmy_ops_blockfp8_linear_args *a,
     const emmy_ops_blockfp8_args &q = a->product;
     if (int e = check_product(&q)) return e;
     const emmy_ops_blockfp8_quantize_args x = {a->x, q.xq, q.xs, a->x_stride, q.xq_stride, q.xs_stride, q.m, q.k, a->x_dtype, 0};
-    /* one launch or two: what a warp quantises itself stands before its products, which shows in long rows (2 x 170 x 11248: 9.5 us
-     * in two launches, 14.6 in one) */
-    if (q.m > FUSED_ROWS || q.k > 8192 || !known_dtype(a->x_dtype)) {
+    /* One launch or two: in one, every 16 rows of W quantise x again, which shows where there are many or rows are long.  Device
+     * times in one launch and in two: 2 x 1000 x 1000 3.1 and 3.7 us, 1 x 6144 x 2048 6.0 and 6.7, 1 x 4096 x 4096 6.5 and 6.2 (and
+     * 2.5 us less of the host's time), 2 x 4096 x 4096 7.8 and 6.9, 2 x 14336 x 4096 27 and 19. */
+    if (q.m > FUSED_ROWS || q.m * q.n * q.k > (1 << 24) || !known_dtype(a->x_dtype)) {
         if (int e = emmy_ops_blockfp8_quantize(&x, device, stream)) return e;
         return emmy_ops_blockfp8_product(&q, device, stream);
     }

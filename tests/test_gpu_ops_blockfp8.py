@@ -121,6 +121,12 @@ def test_product(runtime, m, n, k):
     check(m, n, k, y_type="f32")
 
 
+@pytest.mark.parametrize("m", [1, 2, 3, 8, 16])
+@pytest.mark.parametrize("n,k", [(2400, 1500), (2368, 1025), (4101, 4200), (40, 12000), (9000, 1000)])
+def test_few_rows(runtime, m, n, k):
+    check(m, n, k)
+
+
 @pytest.mark.parametrize("x_type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("y_type", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("m", [5, 150])
