@@ -42,6 +42,7 @@ constexpr int WARPS = 2, WARP_TOKENS = 64, TILE = WARPS * WARP_TOKENS, STAGES = 
 /* what registers and shared memory let an SM hold of 8-row and of 16-row blocks */
 template <int NT> constexpr int BLOCKS_PER_SM = NT == 1 ? 6 : 4;
 constexpr int MAX_BATCH = 4096;
+constexpr uint32_t NOT_FINITE = 0x7c00;      /* magnitudes of f16 from here on are infinity and NaN */
 
 struct AttendParams {
     const char *k, *v;
@@ -399,14 +400,31 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         }
         /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
         float rescale = 1.0f;
+        /* A hidden token's probability is 0, and 0 times infinity is no 0: where a value of such a tile is not finite, the
+         * products leave it out, and the rows that see it take it by itself. */
+        bool guarded = false;
         Doubled *const doubled = (Doubled *)s.k;
         __syncwarp();                   /* all lanes are done with the keys */
         {
             const bool lives[2] = {(s.held >> lane & 1) != 0, (s.held >> (lane + 32) & 1) != 0};
             const __half2 vm[2] = {s.v_meta[lane], s.v_meta[lane + 32]}, zero = __halves2half2(__half(), __half());
-            const __half2 of_v[2] = {lives[0] ? vm[0] : zero, lives[1] ? vm[1] : zero};
-            const uint32_t bits = max(__half_as_ushort(__low2half(of_v[0])) & 0x7fff, __half_as_ushort(__low2half(of_v[1])) & 0x7fff);
-            const int exponent = (int)(__reduce_max_sync(~0u, bits) >> 10) - 15;
+            __half2 of_v[2] = {lives[0] ? vm[0] : zero, lives[1] ? vm[1] : zero};
+            /* the largest step's bits; NOT_FINITE and more where a step or a least value is infinite or NaN */
+            auto step_bits = [&](int i) { return (uint32_t)__half_as_ushort(__low2half(of_v[i])) & 0x7fff; };
+            auto least_bits = [&](int i) { return (uint32_t)__half_as_ushort(__high2half(of_v[i])) & 0x7fff; };
+            auto either = [&](int i) { return least_bits(i) >= NOT_FINITE ? NOT_FINITE : step_bits(i); };
+            uint32_t bits = __reduce_max_sync(~0u, max(either(0), either(1)));
+            if (bits >= NOT_FINITE) {
+                guarded = s.held != ~0ull || at.tile * TILE + (warp + 1) * WARP_TOKENS > all_see;
+                uint32_t finite = 0;
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    if (step_bits(i) < NOT_FINITE) finite = max(finite, step_bits(i));
+                    if (guarded && max(step_bits(i), least_bits(i)) >= NOT_FINITE) of_v[i] = zero;
+                }
+                bits = __reduce_max_sync(~0u, finite);
+            }
+            const int exponent = (int)(bits >> 10) - 15;
             if (exponent > v_exponent) {
                 rescale = v_exponent < -15 ? 1.0f : exp2_approx((float)(v_exponent - exponent));
                 v_exponent = exponent;
@@ -489,6 +507,22 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 for (int i = 0; i < OT; ++i)
                     o[n][i][0] *= f0, o[n][i][1] *= f1, o[n][i][2] *= f0, o[n][i][3] *= f1;
             }
+        }
+        if (guarded) {
+#pragma unroll
+            for (int m = 0; m < MT; ++m)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int token = 16 * m + 8 * h + token_of<DIM>(r);
+                    const float2 v = __half22float2(s.v_meta[token]);
+                    if (!(held >> token & 1) || (fabsf(v.x) < INFINITY && fabsf(v.y) < INFINITY)) continue;
+#pragma unroll
+                    for (int n = 0; n < NT; ++n) {
+                        const float2 x = fma2(by[n], Two(score[m][n][2 * h], score[m][n][2 * h + 1]), minus[n]).get();
+                        least[n] = least[n] + Two(from + token < sees[n][0] ? exp2_approx(x.x) * (v.x + v.y) : 0.0f,
+                                                  from + token < sees[n][1] ? exp2_approx(x.y) * (v.x + v.y) : 0.0f);
+                    }
+                }
         }
         uint32_t pf[MT][NT][2];
 #pragma unroll

@@ -235,3 +235,27 @@ def test_graph(runtime):
         torch.cuda.synchronize()
         ref, bound = reference(a, q, table, lens.tolist(), 16, 0.125)
         close(out, ref, bound)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dim,heads,group,tokens,page,lengths", [
+    (64, 2, 4, 2, 16, [100, 64, 2, 3000]), (128, 1, 4, 3, 64, [130, 65, 64, 5000]), (64, 1, 1, 7, 24, [127, 129, 7, 700]),
+    (128, 2, 2, 5, 16, [63, 128, 5, 2500])])
+@pytest.mark.parametrize("part,value", [(0, float("nan")), (1, float("nan")), (0, float("inf")), (1, float("-inf"))])
+def test_not_finite_behind_a_query(runtime, dtype, dim, heads, group, tokens, page, lengths, part, value):
+    """A key and a value that are not finite at the last position are seen by the last query alone: the earlier ones of the same
+    call, which share its tile, give what they give without it."""
+    from emmyrt.cache4 import Cache4Attention
+    batch, per = len(lengths), -(-max(lengths) // page)
+    cache, a = make(batch * per, heads, page, dim, seed=3)
+    table = torch.randperm(batch * per, generator=torch.Generator(device="cuda").manual_seed(4), device="cuda").to(torch.int32).view(batch, per)
+    lens = torch.tensor(lengths, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, tokens, heads * group, dim, generator=torch.Generator(device="cuda").manual_seed(5), device="cuda").to(TYPES[dtype])
+    for b, n in enumerate(lengths):
+        for name in ("k_meta", "v_meta"):
+            a[name][table[b, (n - 1) // page].long(), :, (n - 1) % page, part] = value
+    out = torch.full_like(q, 7.0)
+    Cache4Attention(cache, heads * group)(q, out, table, lens, stream=stream())
+    ref, bound = reference(a, q[:, :-1], table, [n - 1 for n in lengths], page, dim ** -0.5)
+    close(out[:, :-1], ref, bound)
+    assert not out[:, -1].isfinite().any()
