@@ -196,6 +196,9 @@ struct FewParams {
     int m, n, k, stages;
     int64_t raw_stride;                 /* of x before quantisation, where the product quantises it itself */
     int raw_wide;
+    uint8_t *xq;                        /* where the first block of threads leaves what it quantised */
+    float *xs;
+    int64_t xq_stride, xs_stride;
 };
 
 __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -223,7 +226,8 @@ __device__ __forceinline__ void copy_async16(const void *shared, const void *fro
 }
 
 /* X: the type of an x that is not quantised yet, of up to 2 rows: a warp quantises what it takes, 4 elements a lane, which
- * saves the launch of the quantiser (1 x 4321 x 648: 4.4 -> 3.0 us).  Quantised: p.x and p.sx have it. */
+ * saves the launch of the quantiser (1 x 4321 x 648: 4.4 -> 3.0 us); the first block of threads leaves it in p.xq and p.xs.  Quantised:
+ * p.x and p.sx have it. */
 struct Quantised {};
 constexpr int FUSED_ROWS = 2;
 
@@ -286,8 +290,9 @@ template <typename T, int NT, typename X, int FEW_WARPS> __global__ void __launc
             }
         }
     };
-    auto quantise = [&](FewStage<NT> &s) {
+    auto quantise = [&](FewStage<NT> &s, int step) {
         if constexpr (FUSED) {
+            const int b = warp + FEW_WARPS * step, e = b * BLOCK + 4 * lane;
 #pragma unroll
             for (int m = 0; m < FUSED_ROWS; ++m) {
                 if (m >= p.m) break;
@@ -297,8 +302,13 @@ template <typename T, int NT, typename X, int FEW_WARPS> __global__ void __launc
                 const float scale = scale_of(__reduce_max_sync(~0u, largest));
                 float (&v)[4] = ahead[m];
                 divide(v, scale);
-                *(uint32_t *)&s.x[m][((lane >> 2) ^ ((m & 1) * 4)) * 16 + (lane & 3) * 4] = e4m3x4(v[0], v[1], v[2], v[3]);
+                const uint32_t four = e4m3x4(v[0], v[1], v[2], v[3]);
+                *(uint32_t *)&s.x[m][((lane >> 2) ^ ((m & 1) * 4)) * 16 + (lane & 3) * 4] = four;
                 if (lane == 0) s.sx[m] = scale;
+                if (blockIdx.x == 0) {
+                    if (e < ((p.k + 15) & ~15)) *(uint32_t *)(p.xq + m * p.xq_stride + e) = four;   /* zeros up to a multiple of 16 */
+                    if (lane == 0) p.xs[b * p.xs_stride + m] = scale;
+                }
             }
         }
     };
@@ -319,7 +329,7 @@ template <typename T, int NT, typename X, int FEW_WARPS> __global__ void __launc
     const int low = (c ^ ((r & 1) * 4)) * 16, high = ((c + 4) ^ ((r & 1) * 4)) * 16;
     for (int step = 0, stage = 0; step < steps; ++step) {
         if (FUSED) {
-            quantise(ring[stage]);
+            quantise(ring[stage], step);
             fetch(step + 1);
         }
         if (p.stages == STAGES)
@@ -866,7 +876,7 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
     if (a->m <= 8 || (a->m <= 16 && a->n * a->k <= (1 << 25))) {
         FewParams p = {(const uint8_t *)(uintptr_t)a->xq, (const uint8_t *)(uintptr_t)a->wq, (const float *)(uintptr_t)a->xs,
                        (const float *)(uintptr_t)a->ws, (char *)(uintptr_t)a->y, a->xq_stride, a->wq_stride, a->xs_stride,
-                       a->ws_stride, a->y_stride, (int)a->m, (int)a->n, (int)a->k, 0, 0, 0};
+                       a->ws_stride, a->y_stride, (int)a->m, (int)a->n, (int)a->k};
         const cudaError_t e = a->m <= 8 ? go_few<T, 1>(p, device, stream) : go_few<T, 2>(p, device, stream);
         return ops_cuda(e, "FP8 product of few rows");
     }
@@ -1025,7 +1035,8 @@ EMMY_EXPORT int emmy_ops_blockfp8_linear(const emmy_ops_blockfp8_linear_args *a,
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
     FewParams p = {(const uint8_t *)(uintptr_t)a->x, (const uint8_t *)(uintptr_t)q.wq, nullptr, (const float *)(uintptr_t)q.ws,
                    (char *)(uintptr_t)q.y, 0, q.wq_stride, 0, q.ws_stride, q.y_stride, (int)q.m, (int)q.n, (int)q.k, 0, a->x_stride,
-                   aligned(a->x, 4 * es) && a->x_stride % 4 == 0};
+                   aligned(a->x, 4 * es) && a->x_stride % 4 == 0, (uint8_t *)(uintptr_t)q.xq, (float *)(uintptr_t)q.xs, q.xq_stride,
+                   q.xs_stride};
     const cudaError_t e = q.dtype == EMMY_OPS_F32   ? go_fused<float>(p, a->x_dtype, device, stream)
                           : q.dtype == EMMY_OPS_F16 ? go_fused<__half>(p, a->x_dtype, device, stream)
                                                     : go_fused<__nv_bfloat16>(p, a->x_dtype, device, stream);

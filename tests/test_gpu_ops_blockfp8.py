@@ -197,3 +197,37 @@ def test_graph(runtime):
         again = torch.empty_like(y)
         op(x, again, stream=stream())
         assert torch.equal(again, y)
+
+
+@pytest.mark.parametrize("x_type", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("m,n,k", [(1, 40, 300), (2, 500, 1000), (2, 3000, 2600), (1, 1, 1), (1, 4096, 4096), (3, 40, 300), (40, 300, 700)])
+def test_linear_leaves_the_quantised_x(runtime, x_type, m, n, k):
+    """The C entry's contract: x stands quantised in xq and xs after the call, its padding zero, at sizes that quantise it within
+    the product too, so that a second product can share it."""
+    import ctypes
+    import emmyrt
+    wq, ws = weights(n, k)
+    x = torch.randn(m, k, generator=gen(9), device="cuda").to(TYPES[x_type])
+    x[0, 0] = 100
+    pitch = -(-k // 16) * 16
+    xq = torch.full((m, pitch + 16), 0x55, dtype=torch.uint8, device="cuda")
+    xs = torch.full((-(-k // 128) + 1, -(-m // 4) * 4), -1.0, device="cuda")
+    y, again = (torch.full((m, n), float("nan"), device="cuda") for _ in range(2))
+    status = torch.zeros(1, dtype=torch.int32, device="cuda")
+    a = emmyrt.BlockFp8LinearArgs(xq=xq.data_ptr(), xs=xs.data_ptr(), wq=wq.data_ptr(), ws=ws.data_ptr(), y=y.data_ptr(),
+                                  status=status.data_ptr(), xq_stride=pitch + 16, xs_stride=xs.stride(0), wq_stride=pitch,
+                                  ws_stride=ws.stride(0), y_stride=n, m=m, n=n, k=k, dtype=0, x=x.data_ptr(), x_stride=k,
+                                  x_dtype=["f32", "f16", "bf16"].index(x_type))
+    assert emmyrt.ops_lib().emmy_ops_blockfp8_linear(ctypes.byref(a), 0, stream()) == 0
+    rq, rs = quantised(x, False)
+    assert torch.equal(xs[:-1, :m], rs) and (xs[-1] == -1).all() and (xs[:, m:] == -1).all()
+    assert torch.equal(xq[:, :k].view(E4M3).float(), rq)
+    assert (xq[:, k:pitch] == 0).all() and (xq[:, pitch:] == 0x55).all()
+    # the product alone, of what the call left
+    p = emmyrt.BlockFp8Args(**{f: getattr(a, f) for f, _ in emmyrt.BlockFp8Args._fields_})
+    p.y = again.data_ptr()
+    assert emmyrt.ops_lib().emmy_ops_blockfp8_product(ctypes.byref(p), 0, stream()) == 0
+    ref, bound = reference(x, wq, ws, torch.float32)
+    for out in (y, again):
+        assert ((out.double() - ref).abs() <= bound).all()
+    assert status.item() == 0
