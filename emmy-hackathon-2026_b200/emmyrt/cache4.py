@@ -9,7 +9,7 @@ from __future__ import annotations
 import ctypes
 import math
 
-from . import Cache4AppendArgs, Cache4AttendArgs, DeviceBuffer, EmmyRTError, ops_lib
+from . import Cache4AppendArgs, Cache4AttendArgs, DeviceBuffer, EmmyRTError, check, lib, ops_lib
 from .operands import CODE, FLOATS, INDICES, Array, Operator, apart, contiguous, operand, overlaps, shaped, written
 
 DIMS = (64, 128)
@@ -41,12 +41,14 @@ class Cache4(Operator):
 
     @classmethod
     def allocate(cls, pages: int, heads: int, page: int, dim: int) -> "Cache4":
-        """A cache in new device memory, all of it zero."""
+        """A cache in new device memory, all of it zero when this returns."""
         made = []
         for dtype, last, size in (("u8", dim // 2, 1), ("f16", 2, 2)) * 2:
             buffer = DeviceBuffer(pages * heads * page * last * size)
             buffer.zero()
             made.append(Array(buffer, dtype, (pages, heads, page, last)))
+        # the streams that append need not wait for the default one
+        check(lib.emmy_rt_stream_synchronize(0), "sync")
         return cls(*made)
 
     def _held(self) -> dict:

@@ -99,3 +99,20 @@ def test_allocate(runtime):
     torch.cuda.synchronize()
     held = c.k_meta.owner.download(np.zeros((3, 2, 5, 2), np.float16))
     assert (held[0, :, 0, 0] > 0).all() and (held[2, :, 4, 0] > 0).all() and (held != 0).sum() == 8
+
+
+def test_append_right_after_allocate(runtime):
+    """The zeros of a new cache are there before a stream that does not wait for the default one appends to it."""
+    import numpy as np
+    from emmyrt.cache4 import Cache4
+    pages, heads, page, dim = 20000, 8, 64, 128            # 1.4 GB: its zeros take longer than a call
+    k = torch.randn(2, heads, dim, device="cuda")
+    slots = torch.tensor([0, pages * page - 1], device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    c = Cache4.allocate(pages, heads, page, dim)
+    c.append(k, k, slots, stream=side.cuda_stream)
+    torch.cuda.synchronize()
+    for part in (c.k_meta, c.v_meta):
+        held = part.owner.download(np.zeros((pages, heads, page, 2), np.float16))
+        assert (held[0, :, 0, 0] > 0).all() and (held[-1, :, -1, 0] > 0).all() and (held != 0).sum() == 4 * heads

@@ -247,3 +247,26 @@ def test_many_kinds_of_calls_are_not_kept_for_good(calls):
     for rows in range(1, 2 * op.PLANS):
         op(A(1, "f32", rows, 8), A(2, "f32", rows, 8), A(3, "f32", rows, 8))
     assert len(op._plans) <= op.PLANS and calls[-1][1].rows == 2 * op.PLANS - 1
+
+
+def test_allocate_waits_for_its_zeros(calls, monkeypatch):
+    """The cache is all zero when allocate returns: streams that do not wait for the default stream, where it is zeroed, may append at once."""
+    import emmyrt.cache4
+    order = []
+
+    class Buffer:
+        def __init__(self, nbytes):
+            self.nbytes, self.ptr = nbytes, (1 + len(order)) << 30
+
+        def zero(self, stream=0):
+            order.append(("zero", self.nbytes, stream))
+
+    class Lib:
+        def emmy_rt_stream_synchronize(self, stream):
+            order.append(("wait", stream))
+            return 0
+
+    monkeypatch.setattr(emmyrt.cache4, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(emmyrt.cache4, "lib", Lib(), raising=False)
+    emmyrt.cache4.Cache4.allocate(3, 2, 16, 64)
+    assert order[:-1] == [("zero", 3 * 2 * 16 * 32, 0), ("zero", 3 * 2 * 16 * 4, 0)] * 2 and order[-1] == ("wait", 0)
