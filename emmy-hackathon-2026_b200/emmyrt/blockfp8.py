@@ -104,7 +104,8 @@ class BlockFp8Linear(Operator):
 
     @classmethod
     def from_weight(cls, w, max_rows: int, stream: int = 0) -> "BlockFp8Linear":
-        """Quantises ``w`` [n, k] (f32, f16 or bf16) into memory of its own, on ``stream``."""
+        """Quantises ``w`` [n, k] (f32, f16 or bf16) into memory of its own, on ``stream``, and waits for that: calls may
+        come on any stream."""
         d = cls.__new__(cls)
         Operator.__init__(d)
         w = operand(w, "w", FLOATS, 2, d.device)
@@ -114,6 +115,7 @@ class BlockFp8Linear(Operator):
         wq = Array(DeviceBuffer(n * pitch(k)), "u8", (n, k), (pitch(k), 1))
         ws = Array(DeviceBuffer(blocks(n) * blocks(k) * 4), "f32", (blocks(n), blocks(k)))
         BlockFp8Quantizer(square=True)(w, wq, ws, stream=stream)
+        check(lib.emmy_rt_stream_synchronize(stream), "sync")
         d.__init__(wq, ws, max_rows)
         return d
 

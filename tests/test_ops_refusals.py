@@ -270,3 +270,28 @@ def test_allocate_waits_for_its_zeros(calls, monkeypatch):
     monkeypatch.setattr(emmyrt.cache4, "lib", Lib(), raising=False)
     emmyrt.cache4.Cache4.allocate(3, 2, 16, 64)
     assert order[:-1] == [("zero", 3 * 2 * 16 * 32, 0), ("zero", 3 * 2 * 16 * 4, 0)] * 2 and order[-1] == ("wait", 0)
+
+
+@pytest.mark.parametrize("stream", [0, 77])
+def test_from_weight_waits_for_its_weight(calls, monkeypatch, stream):
+    """The quantised weight is there when from_weight returns, whatever stream it was quantised on and whatever stream calls come on."""
+    import emmyrt.blockfp8
+    order = []
+
+    class Lib:
+        def emmy_rt_stream_synchronize(self, s):
+            order.append((s, len(calls)))
+            return 0
+
+    class Buffer:
+        made = 0
+
+        def __init__(self, nbytes):
+            Buffer.made += 1
+            self.nbytes, self.ptr = nbytes, Buffer.made << 40
+
+    monkeypatch.setattr(emmyrt.blockfp8, "DeviceBuffer", Buffer)
+    monkeypatch.setattr(emmyrt.blockfp8, "lib", Lib())
+    op = emmyrt.blockfp8.BlockFp8Linear.from_weight(A(1, "bf16", 300, 200), 4, stream=stream)
+    assert [n for n, _ in calls] == ["emmy_ops_blockfp8_quantize"] and calls[0][1].square == 1
+    assert (stream, 1) in order and (op.n, op.k) == (300, 200)
