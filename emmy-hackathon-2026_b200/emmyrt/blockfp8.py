@@ -33,8 +33,11 @@ class BlockFp8Quantizer(Operator):
 
     def __call__(self, x, q, s, *, stream: int = 0) -> None:
         """``x`` [rows, cols] (f32, f16 or bf16); ``q`` the same shape, e4m3 or u8, its rows a multiple of 16 bytes apart and
-        at least :func:`pitch` (without ``square`` the columns up to there become zero); ``s`` f32
-        [blocks of cols, rows], with ``square`` [blocks of rows, blocks of cols]."""
+        at least :func:`pitch` (without ``square`` the columns up to there become zero, those of the last row too; a
+        single row that is not that far apart has no such columns); ``s`` f32 [blocks of cols, rows], with ``square``
+        [blocks of rows, blocks of cols]."""
+        if not self.square:
+            _room_for_padding(q)
         self._call((x, q, s), None, stream)
 
     def _plan(self, operands, options) -> tuple:
@@ -47,7 +50,8 @@ class BlockFp8Quantizer(Operator):
         q = _padded(q, "q")
         want = (blocks(rows), blocks(cols)) if self.square else (blocks(cols), rows)
         s = written(shaped(operand(operands[2], "s", ("f32",), 2, d), "s", want), "s")
-        a = BlockFp8QuantizeArgs(x_stride=x.strides[0], q_stride=_stride(q), s_stride=s.strides[0], rows=rows, cols=cols,
+        a = BlockFp8QuantizeArgs(x_stride=x.strides[0], q_stride=_stride(q) if self.square else _row_stride(q),
+                                 s_stride=s.strides[0], rows=rows, cols=cols,
                                  dtype=CODE[x.dtype], square=self.square)
         checks = overlaps([(1, _with_padding(q) if not self.square else q, "q"), (2, s, "s")], [(0, x, "x")])
         return "emmy_ops_blockfp8_quantize", a, ("x", "q", "s"), checks
@@ -64,9 +68,34 @@ def _stride(q: Array) -> int:
     return q.strides[0] if q.shape[0] > 1 else pitch(q.shape[1])
 
 
+def _row_stride(q: Array) -> int:
+    """The row stride for the row quantiser, which pads what it allows: a single row that is not in padded rows has none."""
+    rows, cols = q.shape
+    apart = q.strides[0]
+    return apart if rows > 1 or (apart >= pitch(cols) and apart % 16 == 0) else cols
+
+
 def _with_padding(q: Array) -> Array:
     """``q`` with the columns that the row quantiser fills with zeros."""
-    return Array(q.ptr, q.dtype, (q.shape[0], pitch(q.shape[1])), (_stride(q), 1), q.device)
+    stride = _row_stride(q)
+    return Array(q.ptr, q.dtype, (q.shape[0], min(stride, pitch(q.shape[1]))), (stride, 1), q.device)
+
+
+def _room_for_padding(q) -> None:
+    """Refuses a q whose last row's padding lies past its memory, as far as that is known.  It is no matter of the call's
+    kind, so each call asks."""
+    if type(q) is Array:
+        room, strides = getattr(q.owner, "nbytes", None), q.strides
+    elif hasattr(q, "untyped_storage"):
+        room, strides = q.untyped_storage().nbytes() - q.storage_offset(), q.stride()     # elements of one byte
+    else:
+        return
+    if room is None or len(q.shape) != 2 or q.shape[1] % 16 == 0:
+        return
+    rows, cols = q.shape
+    if rows and (rows > 1 or (strides[0] >= pitch(cols) and strides[0] % 16 == 0)) and \
+            (rows - 1) * strides[0] + pitch(cols) > room:
+        raise ValueError(f"q: the last row's padding, up to {pitch(cols)} columns, lies past its memory")
 
 
 class BlockFp8Linear(Operator):

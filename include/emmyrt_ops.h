@@ -93,7 +93,8 @@ int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint64_t stream);
 /* q = e4m3(x / s), s = amax / 448 (1 where that is 0), over 128 columns of a row (square 0:
  * s is [blocks of columns][rows]) or over 128 x 128 (square 1: s is [blocks of rows][blocks of
  * columns]).  Rows of q are a multiple of 16 bytes apart; without square, columns up to the
- * next multiple of 16 become zero. */
+ * next multiple of 16 become zero, those of the last row too.  A single row whose q_stride is less
+ * than that has no such columns. */
 typedef struct {
     uint64_t x, q, s;
     int64_t x_stride, q_stride, s_stride, rows, cols;

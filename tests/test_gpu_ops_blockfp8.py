@@ -231,3 +231,16 @@ def test_linear_leaves_the_quantised_x(runtime, x_type, m, n, k):
     for out in (y, again):
         assert ((out.double() - ref).abs() <= bound).all()
     assert status.item() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("cols", [1, 7, 8, 9, 15, 16, 17, 100, 130, 1025])
+def test_quantise_a_row_without_padding(runtime, dtype, cols):
+    """A single row in exactly its own bytes: what stands behind it stays."""
+    from emmyrt.blockfp8 import BlockFp8Quantizer
+    x = torch.randn(1, cols, generator=gen(cols), device="cuda").to(TYPES[dtype])
+    held = torch.full((3, cols), 0x55, dtype=torch.uint8, device="cuda")
+    s = torch.empty(-(-cols // 128), 1, device="cuda")
+    BlockFp8Quantizer()(x, held[:1], s, stream=stream())
+    rq, rs = quantised(x, False)
+    assert torch.equal(s, rs) and torch.equal(held[:1].view(E4M3).float(), rq) and (held[1:] == 0x55).all()

@@ -295,3 +295,51 @@ def test_from_weight_waits_for_its_weight(calls, monkeypatch, stream):
     op = emmyrt.blockfp8.BlockFp8Linear.from_weight(A(1, "bf16", 300, 200), 4, stream=stream)
     assert [n for n, _ in calls] == ["emmy_ops_blockfp8_quantize"] and calls[0][1].square == 1
     assert (stream, 1) in order and (op.n, op.k) == (300, 200)
+
+
+def test_padding_stays_in_q(calls):
+    """The row quantiser's zeros behind a row's last column: not where a single row has no room for them, and not past q's memory."""
+    from emmyrt.blockfp8 import BlockFp8Quantizer
+    from emmyrt.operands import Array
+
+    class Owner:
+        def __init__(self, nbytes):
+            self.ptr, self.nbytes = 1 << 40, nbytes
+
+    class Storage:
+        def __init__(self, nbytes):
+            self.size = nbytes
+
+        def nbytes(self):
+            return self.size
+
+    class Held(Tensor):
+        def __init__(self, nbytes, offset, *args):
+            super().__init__(*args)
+            self.memory, self.offset = Storage(nbytes), offset
+
+        def untyped_storage(self):
+            return self.memory
+
+        def storage_offset(self):
+            return self.offset
+
+    quantise = BlockFp8Quantizer()
+    x1, s1 = A(1, "f16", 1, 100), A(3, "f32", 1, 1)
+    for q in (A(2, "u8", 1, 100), Array(Owner(100), "u8", (1, 100)), Tensor(2 << 24, "torch.uint8", (1, 100), (100, 1)),
+              Tensor(2 << 24, "torch.uint8", (1, 100), (200, 1)), Tensor(2 << 24, "torch.uint8", (1, 100), (1, 1))):
+        quantise(x1, q, s1)
+        assert calls[-1][1].q_stride == 100             # of one row: no room for padding
+    quantise(x1, A(2, "u8", 1, 100, strides=(128, 1)), s1)
+    assert calls[-1][1].q_stride == 128
+    quantise(x1, A(2, "u8", 1, 100), Array((2 << 24) + 100, "f32", (1, 1)))    # right behind such a row
+    x, s = A(1, "f16", 3, 100), A(3, "f32", 1, 3)
+    quantise(x, Array(Owner(2 * 112 + 112), "u8", (3, 100), (112, 1)), s)
+    quantise(x, Held(500, 500 - 336, 2 << 24, "torch.uint8", (3, 100), (112, 1)), s)
+    made = len(calls)
+    refuses(lambda: quantise(x, Array(Owner(2 * 112 + 100), "u8", (3, 100), (112, 1)), s), "padding")
+    refuses(lambda: quantise(x, Array(Owner(2 * 112 + 111), "u8", (3, 100), (112, 1)), s), "padding")
+    refuses(lambda: quantise(x, Held(500, 500 - 335, 2 << 24, "torch.uint8", (3, 100), (112, 1)), s), "padding")
+    refuses(lambda: quantise(x1, Array(Owner(100), "u8", (1, 100), (112, 1)), s1), "padding")
+    assert len(calls) == made
+    BlockFp8Quantizer(square=True)(x, Array(Owner(2 * 112 + 100), "u8", (3, 100), (112, 1)), A(3, "f32", 1, 1))
