@@ -551,10 +551,11 @@ template <int BN, bool PAIR> struct ManyShape {
     static constexpr int A_BYTES = 128 * BLOCK, B_BYTES = B_ROWS * BLOCK, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = STAGE > 40960 ? 4 : STAGE >= 32768 ? 6 : 8;
     static constexpr int BUFFERS = 512 / BN > 4 ? 4 : 512 / BN;
-    /* The copies are at most STAGES blocks ahead of the products, and these BUFFERS ahead of the scaling: a place that many
-     * and one more blocks on is free without a barrier of its own. */
-    static constexpr int SCALES = 16;
-    static_assert(STAGES + BUFFERS < SCALES, "the scales' ring");
+    /* x's scales have a ring of their own, in runs of SCALE_RUN places that the scaling warps hand back by a barrier each.  The
+     * copies are at most STAGES blocks ahead of the products, and these BUFFERS ahead of the scaling, so they find the next run
+     * free: nothing waits there. */
+    static constexpr int SCALES = 16, SCALE_RUN = 4;
+    static_assert(STAGES + BUFFERS <= SCALES - SCALE_RUN, "the scales' ring");
     static constexpr int COLUMNS = BN * BUFFERS < 32 ? 32 : BN * BUFFERS;
     static constexpr int SCALE_WARPS = BN >= 128 ? 8 : 4;
     static constexpr int PER = BN / (SCALE_WARPS / 4);                /* columns a scaling thread */
@@ -571,7 +572,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
               const __grid_constant__ TensorMap s_map, ManyParams p) {
     using S = ManyShape<BN, PAIR>;
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS];
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS], scaled[S::SCALES / S::SCALE_RUN];
     __shared__ alignas(128) float scales[S::SCALES][128];      /* of x: a block's 128 rows, copied with its operands */
     __shared__ uint32_t tensor_base;
     __shared__ volatile unsigned abort;
@@ -588,6 +589,8 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&summed[i])));
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&read[i])), "r"(S::SCALE_WARPS * (PAIR ? 2 : 1)));
         }
+        for (int i = 0; i < S::SCALES / S::SCALE_RUN; ++i)
+            asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&scaled[i])), "r"(S::SCALE_WARPS));
         abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -627,15 +630,16 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         if (lane == 0) {
             uint32_t leader = shared_address(&full[0]);
             if (PAIR) asm volatile("mapa.shared::cluster.u32 %0, %0, 0;" : "+r"(leader));
-            int stage = 0, slot = -1;
-            uint32_t phase = 0;
+            int stage = 0, slot = 0;
+            uint32_t phase = 0, slot_phase = 0;
             bool ok = true;
             for (int t = worker; t < tiles && ok; t += workers) {
                 const Unit u = place(t);
                 const int m0 = u.m0 + (PAIR ? 128 * rank : 0), n0 = u.n0 + (PAIR ? S::B_ROWS * rank : 0);
                 for (int b = u.from; b < u.to; ++b) {
                     if (!(ok = wait_for(shared_address(&empty[stage]), phase ^ 1, &abort, p.status, 1))) break;
-                    if (++slot == S::SCALES) slot = 0;
+                    if (slot % S::SCALE_RUN == 0 &&
+                        !(ok = wait_for(shared_address(&scaled[slot / S::SCALE_RUN]), slot_phase ^ 1, &abort, p.status, 1))) break;
                     if (rank == 0)      /* both copies of a pair complete on the leader's barrier */
                         asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;"
                                      ::"r"(shared_address(&full[stage])), "r"((S::STAGE + 512) * (PAIR ? 2 : 1)) : "memory");
@@ -643,6 +647,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     tma_load<PAIR>(to, &x_map, b * BLOCK, m0, barrier);
                     tma_load<PAIR>(to + S::A_BYTES, &w_map, b * BLOCK, n0, barrier);
                     tma_load<PAIR>(shared_address(scales[slot]), &s_map, m0, b, barrier);
+                    if (++slot == S::SCALES) slot = 0, slot_phase ^= 1;
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
             }
@@ -720,6 +725,12 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
 #pragma unroll 1
             for (int b = u.from; b < u.to; ++b) {
                 const float one = next_w * scales[slot][32 * quarter + lane];
+                if (slot % S::SCALE_RUN == S::SCALE_RUN - 1) {
+                    /* the run has been read, by all lanes: copies may write it again */
+                    __syncwarp();
+                    if (lane == 0)
+                        asm volatile("mbarrier.arrive.release.cta.shared::cta.b64 _, [%0];" ::"r"(shared_address(&scaled[slot / S::SCALE_RUN])) : "memory");
+                }
                 if (b + 1 < u.to) next_w = sw[b + 1];
                 slot = slot + 1 == S::SCALES ? 0 : slot + 1;
                 uint64_t s;
@@ -730,7 +741,8 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     if (c + 1 < S::CHUNKS) {
                         tensor_load(mine + buffer * BN + (c + 1) * S::CHUNK, v[(c + 1) & 1]);
                     } else {
-                        /* all of the block is in registers */
+                        /* All of the block is in registers.  A relaxed arrive is enough: the fences of tcgen05 on both sides order the
+                         * loads before the next product, and nothing else rests on it. */
                         asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
                         __syncwarp();
                         if (lane == 0) {
