@@ -211,9 +211,11 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     Shared<DIM, NT> &sh = *(Shared<DIM, NT> *)raw;
     constexpr int ROWS = 8 * NT, WORDS = DIM / 32, ROW_BYTES = DIM / 2, OT = DIM / 16, OUT_ROW = DIM + 4;
     static_assert(ROWS * OUT_ROW * 4 <= (int)sizeof(Stage<DIM>), "a stage holds a warp's results");
-    /* p s_v goes to f16, off by up to 2^-12 of itself.  Beside an f16 result that shows (3.2e-4 of the result's norm against
-     * 2.1e-4 from its own rounding), so there sum p and sum p z take the p that the rounded product stands for: what
-     * is left is 2^-12 of the values' distance from their mean.  A bf16 result's rounding hides it. */
+    /* p s_v goes to f16, off by up to 2^-12 of itself.  Of an f16 result that was 3.2e-4 of the norm beside 2.1e-4 from the result's
+     * own rounding, so there sum p and sum p z take the p that the rounded product stands for: what is left is 2^-12 of the values'
+     * distance from their mean (2.5e-4 in all at 16 sequences of up to 5000).  A bf16 result keeps the 2^-12 of p s n: 1.687e-3 of
+     * the norm in all, where its own rounding alone is 1.658e-3 (64 sequences of up to 16384).  Both halves of p s_v in the
+     * products would leave 1.660e-3 and take 14 us of 150 more. */
     constexpr bool EXACT = sizeof(T) == 2 && !__is_same(T, __nv_bfloat16);
     /* the join may start only when what this kernel waits for is there: it reads the lengths before it waits */
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -295,7 +297,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
     for (int s = 0; s < STAGES - 1; ++s) issue(s);
 
     uint32_t qf[NT][2 * WORDS][2];
-    float o[NT][OT][4], top[NT][2];
+    Two o[NT][OT][2];
+    float top[NT][2];
     Two least[NT], sum[NT], by[NT], base[NT];
     int sees[NT][2];
     int v_exponent = 0, all_see = 0;
@@ -362,7 +365,7 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
 #pragma unroll
                 for (int i = 0; i < OT; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) o[n][i][j] = 0.0f;
+                    for (int j = 0; j < 2; ++j) o[n][i][j] = Two(0.0f, 0.0f);
             }
         }
         issue((stage + STAGES - 1) % STAGES);
@@ -444,7 +447,6 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
         const int from = at.tile * TILE + warp * WARP_TOKENS;
         const uint64_t held = s.held;
         const bool full = held == ~0ull && from + WARP_TOKENS <= all_see;      /* nothing is hidden from any row */
-        bool moved = false;
         float next[NT][2], shrink[NT][2];
 #pragma unroll
         for (int m = 0; m < MT; ++m)
@@ -490,23 +492,18 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                 for (int d = 4; d < 32; d <<= 1) next[n][i] = fmaxf(next[n][i], __shfl_xor_sync(~0u, next[n][i], d));
                 const float ref = next[n][i] == -INFINITY ? 0.0f : next[n][i];
                 shrink[n][i] = exp2_approx((top[n][i] - ref) * (i ? f.y : f.x));
-                moved |= next[n][i] != top[n][i];
                 top[n][i] = next[n][i];
                 next[n][i] = -ref * (i ? f.y : f.x);
             }
             minus[n] = Two(next[n][0], next[n][1]);
         }
-        if (__any_sync(~0u, moved) || rescale != 1.0f) {
+        Two keep[NT];
 #pragma unroll
-            for (int n = 0; n < NT; ++n) {
-                const Two f(shrink[n][0], shrink[n][1]);
-                sum[n] = sum[n] * f;
-                least[n] = least[n] * f;
-                const float f0 = shrink[n][0] * rescale, f1 = shrink[n][1] * rescale;
-#pragma unroll
-                for (int i = 0; i < OT; ++i)
-                    o[n][i][0] *= f0, o[n][i][1] *= f1, o[n][i][2] *= f0, o[n][i][3] *= f1;
-            }
+        for (int n = 0; n < NT; ++n) {
+            const Two f(shrink[n][0], shrink[n][1]);
+            sum[n] = sum[n] * f;
+            least[n] = least[n] * f;
+            keep[n] = f * Two(rescale, rescale);
         }
         if (guarded) {
 #pragma unroll
@@ -548,36 +545,55 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     least[n] = fma2(e2, Two(v.y), least[n]);
                 }
             }
-        /* O^T += V^T P^T */
+        /* V^T P^T of the tile.  The tensor cores' sums lose what lies below their last bit, always towards zero; kept over a
+         * run of 147 tiles that was 3.4e-5 of sum p s n, or 2 % of a result that sum p z nearly cancels (131072 positions).  So a
+         * tile's sums are its own, and join the others by instructions that round to nearest (149 -> 151 us; 157 with all of 128
+         * dims at a time, whose sums registers do not hold beside the others). */
+        constexpr int PARTS = DIM == 128 ? 2 : 1, WORDS_EACH = WORDS / 2 / PARTS;      /* dims in parts */
 #pragma unroll
-        for (int m = 0; m < MT; ++m) {
-            Pack<uint32_t, WORDS / 2> x[4];
+        for (int part = 0; part < PARTS; ++part) {
+            float fresh[NT][OT / PARTS][4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int token = 16 * m + 8 * (i >> 1) + token_of<DIM>(2 * c + (i & 1));
-                x[i] = *(const Pack<uint32_t, WORDS / 2> *)(s.v + token * ROW_BYTES + swizzled<DIM>(token, r * 2 * WORDS));
-            }
+            for (int m = 0; m < MT; ++m) {
+                Pack<uint32_t, WORDS_EACH> x[4];
 #pragma unroll
-            for (int w = 0; w < WORDS / 2; ++w)
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const uint32_t a = __byte_perm(x[0].at[w], x[1].at[w], half ? 0x7632 : 0x5410);
-                    const uint32_t b = __byte_perm(x[2].at[w], x[3].at[w], half ? 0x7632 : 0x5410);
-                    /* bytes 0 and 2, then 1 and 3; the even dim's level alone, and the whole byte,
-                     * 16 times the odd dim's level more: the even sum is taken out at the end */
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t u = __byte_perm(a, 0, i ? 0x4341 : 0x4240), v = __byte_perm(b, 0, i ? 0x4341 : 0x4240);
-#pragma unroll
-                        for (int n = 0; n < NT; ++n)
-                            mma(o[n][4 * w + 2 * half + i], u & 0x000f000f, u, v & 0x000f000f, v, pf[m][n][0], pf[m][n][1]);
-                    }
+                for (int i = 0; i < 4; ++i) {
+                    const int token = 16 * m + 8 * (i >> 1) + token_of<DIM>(2 * c + (i & 1));
+                    x[i] = *(const Pack<uint32_t, WORDS_EACH> *)(s.v + token * ROW_BYTES + swizzled<DIM>(token, r * 2 * WORDS) + 4 * WORDS_EACH * part);
                 }
+#pragma unroll
+                for (int w = 0; w < WORDS_EACH; ++w)
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        const uint32_t a = __byte_perm(x[0].at[w], x[1].at[w], half ? 0x7632 : 0x5410);
+                        const uint32_t b = __byte_perm(x[2].at[w], x[3].at[w], half ? 0x7632 : 0x5410);
+                        /* bytes 0 and 2, then 1 and 3; the even dim's level alone, and the whole byte,
+                         * 16 times the odd dim's level more: the even sum is taken out at the end */
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            const uint32_t u = __byte_perm(a, 0, i ? 0x4341 : 0x4240), v = __byte_perm(b, 0, i ? 0x4341 : 0x4240);
+                            const int d = 4 * w + 2 * half + i;
+#pragma unroll
+                            for (int n = 0; n < NT; ++n) {
+                                if (m == 0)
+                                    mma_first(fresh[n][d], u & 0x000f000f, u, v & 0x000f000f, v, pf[m][n][0], pf[m][n][1]);
+                                else
+                                    mma(fresh[n][d], u & 0x000f000f, u, v & 0x000f000f, v, pf[m][n][0], pf[m][n][1]);
+                                if (m == MT - 1)
+#pragma unroll
+                                    for (int j = 0; j < 2; ++j) {
+                                        Two &to = o[n][OT / PARTS * part + d][j];
+                                        to = fma2(to, keep[n], Two(fresh[n][d][2 * j], fresh[n][d][2 * j + 1]));
+                                    }
+                            }
+                        }
+                    }
+            }
         }
         __syncwarp();                   /* all lanes are done with the stage before it is filled again */
 
         if (at.tile + 1 == at.tiles || t + 1 == last) {
-            /* the four warps' sums joined */
+            /* the warps' sums joined */
             const float down = __uint_as_float((uint32_t)(127 - 14 + v_exponent) << 23);
 #pragma unroll
             for (int n = 0; n < NT; ++n) {
@@ -598,8 +614,10 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                     float *to = (float *)&sh.ring[warp][stage] + (8 * n + 2 * c + i) * OUT_ROW + 2 * OT * r;
 #pragma unroll
                     for (int j = 0; j < OT; ++j) {
-                        to[2 * j] = fmaf(o[n][j][i] * 0x1p24f, down, bottom);
-                        to[2 * j + 1] = fmaf((o[n][j][2 + i] - o[n][j][i]) * 0x1p20f, down, bottom);
+                        const float2 even = o[n][j][0].get(), whole = o[n][j][1].get();
+                        const float a = i ? even.y : even.x, b = i ? whole.y : whole.x;
+                        to[2 * j] = fmaf(a * 0x1p24f, down, bottom);
+                        to[2 * j + 1] = fmaf((b - a) * 0x1p20f, down, bottom);
                     }
                 }
             }

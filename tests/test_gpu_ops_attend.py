@@ -259,3 +259,42 @@ def test_not_finite_behind_a_query(runtime, dtype, dim, heads, group, tokens, pa
     ref, bound = reference(a, q[:, :-1], table, [n - 1 for n in lengths], page, dim ** -0.5)
     close(out[:, :-1], ref, bound)
     assert not out[:, -1].isfinite().any()
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+def test_long_sums_are_not_biased(runtime, dtype):
+    """131072 positions of equal probability whose values nearly cancel: a mean of 4-bit levels about its middle.
+
+    All keys are the same, so every p is 1 and p s exactly an f16 number: nothing is left but the sums.  What they lose must not pile
+    up over the tiles a block takes in a row (147 here).  Tensor cores drop bits below 2^-22 of the sum at each of the 4 products of
+    a tile of 64 tokens, always towards zero: 4 of 2^-22 of sum p s n, whatever the length.  All other sums round to nearest, which
+    averages out: the signed error's mean over 128 heads of 128 is allowed 2^-22 of sum p (s n + |z|) for them (a chain of
+    1200 additions is off by 0.6 sqrt(1200) 2^-24 = 21 of 2^-24 for one thread, and 128 heads of some 80 threads each take its mean
+    below one of 2^-24).  Sums that go through all 590 products of a run are off by 35 times the bound's first part."""
+    from emmyrt.cache4 import Cache4, Cache4Attention
+    batch, heads, dim, page, length = 8, 16, 128, 128, 131072
+    g = torch.Generator(device="cuda").manual_seed(1)
+    per = length // page
+    k = torch.zeros(batch * per, heads, page, dim // 2, dtype=torch.uint8, device="cuda")
+    km = torch.zeros(batch * per, heads, page, 2, dtype=torch.float16, device="cuda")
+    v = torch.randint(0, 256, k.shape, generator=g, device="cuda", dtype=torch.uint8)
+    step = ((1 + torch.rand(k.shape[:3], generator=g, device="cuda")) / 16).half()
+    vm = torch.stack((step, (-7.5 * step.float()).half()), -1)
+    table = torch.arange(batch * per, dtype=torch.int32, device="cuda").view(batch, per)
+    lens = torch.full((batch,), length, dtype=torch.int32, device="cuda")
+    q = torch.randn(batch, 1, heads, dim, generator=g, device="cuda").to(TYPES[dtype])
+    out = torch.empty_like(q)
+    Cache4Attention(Cache4(k, km, v, vm), heads)(q, out, table, lens, stream=stream())
+    error, first, second = 0.0, 0.0, 0.0
+    for b in range(batch):
+        for h in range(heads):
+            bits = v[b * per:(b + 1) * per, h].reshape(length, dim // 2)
+            s, z = vm[b * per:(b + 1) * per, h].reshape(length, 2).double().t()[:, :, None]
+            for half, n in ((0, bits & 15), (1, bits >> 4)):
+                sn = n.double() * s
+                error += (out[b, 0, h, half::2].double() - (sn + z).mean(0)).sum().item()
+                first += sn.mean(0).sum().item()
+                second += (sn.mean(0) + z.abs().mean(0)).sum().item()
+    count = batch * heads * dim
+    error, first, second = error / count, first / count, second / count
+    assert abs(error) <= 4 * 2.0 ** -22 * first + 2.0 ** -22 * second, (error / first, first, second)
