@@ -9,7 +9,7 @@ from __future__ import annotations
 
 import numpy as np
 
-from . import BlockFp8LinearArgs, BlockFp8QuantizeArgs, DeviceBuffer, check, lib
+from . import BlockFp8LinearArgs, BlockFp8QuantizeArgs, DeviceBuffer, check, current_device, lib
 from .operands import CODE, FLOATS, Array, Operator, operand, overlaps, shaped, written
 
 BLOCK = 128
@@ -152,14 +152,26 @@ class BlockFp8Linear(Operator):
         check(lib.emmy_rt_memset(self._status, 0, 4, 0), "memset")
         check(lib.emmy_rt_stream_synchronize(0), "sync")
 
-    def status(self) -> int:
+    def status(self, stream: int | None = None) -> int:
         """The calls' status word (0 = ok; non-zero = a bounded wait inside the kernel gave up and y is not valid).
-        Waits for the legacy default stream; a non-zero word is cleared."""
+        Waits for all work of the operator's device, or for ``stream`` alone where all calls came on it (or before it);
+        a non-zero word is cleared, so no call may be on its way meanwhile."""
         out = np.zeros(1, np.uint32)
-        check(lib.emmy_rt_memcpy_dtoh(out.ctypes.data, self._status, 4, 0), "dtoh")
-        check(lib.emmy_rt_stream_synchronize(0), "sync")
-        if out[0]:
-            self._clear_status()
+        before = current_device()
+        if before != self.device:
+            check(lib.emmy_rt_set_device(self.device), "set device")
+        try:
+            if stream is None:
+                check(lib.emmy_rt_synchronize(), "synchronize")
+                stream = 0
+            check(lib.emmy_rt_memcpy_dtoh(out.ctypes.data, self._status, 4, stream), "dtoh")
+            check(lib.emmy_rt_stream_synchronize(stream), "sync")
+            if out[0]:
+                check(lib.emmy_rt_memset(self._status, 0, 4, stream), "memset")
+                check(lib.emmy_rt_stream_synchronize(stream), "sync")
+        finally:
+            if before != self.device:
+                check(lib.emmy_rt_set_device(before), "set device")
         return int(out[0])
 
     def __call__(self, x, y, *, stream: int = 0) -> None:

@@ -244,3 +244,19 @@ def test_quantise_a_row_without_padding(runtime, dtype, cols):
     BlockFp8Quantizer()(x, held[:1], s, stream=stream())
     rq, rs = quantised(x, False)
     assert torch.equal(s, rs) and torch.equal(held[:1].view(E4M3).float(), rq) and (held[1:] == 0x55).all()
+
+
+def test_status_of_calls_on_other_streams(runtime):
+    """status() waits for a call on a stream that the default one does not wait for: a word that is set behind it is seen, once."""
+    from emmyrt.blockfp8 import BlockFp8Linear
+    wq, ws = weights(2048, 2048)
+    op = BlockFp8Linear(wq, ws, max_rows=4096)
+    x, y = torch.randn(4096, 2048, device="cuda").half(), torch.empty(4096, 2048, device="cuda")
+    word = torch.full((1,), 8, dtype=torch.int32, device="cuda")
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    for named in (None, side.cuda_stream):
+        for _ in range(30):
+            op(x, y, stream=side.cuda_stream)
+        runtime.check(runtime.lib.emmy_rt_memcpy_dtod(op._status, word.data_ptr(), 4, side.cuda_stream), "copy")
+        assert op.status(stream=named) == 8 and op.status(stream=named) == 0

@@ -343,3 +343,47 @@ def test_padding_stays_in_q(calls):
     refuses(lambda: quantise(x1, Array(Owner(100), "u8", (1, 100), (112, 1)), s1), "padding")
     assert len(calls) == made
     BlockFp8Quantizer(square=True)(x, Array(Owner(2 * 112 + 100), "u8", (3, 100), (112, 1)), A(3, "f32", 1, 1))
+
+
+@pytest.mark.parametrize("current", [0, 1])
+def test_status_waits_for_the_calls(calls, monkeypatch, current):
+    """The status word is read when the calls before it are done: of all streams of the operator's device, or on the stream that is named,
+    whichever device is current; a word that is set is cleared in the same order."""
+    import emmyrt
+    import emmyrt.blockfp8
+    order, words = [], []
+
+    class Lib:
+        def emmy_rt_set_device(self, device):
+            order.append(("device", device))
+            return 0
+
+        def emmy_rt_synchronize(self):
+            order.append("all")
+            return 0
+
+        def emmy_rt_stream_synchronize(self, stream):
+            order.append(("wait", stream))
+            return 0
+
+        def emmy_rt_memcpy_dtoh(self, to, at, nbytes, stream):
+            order.append(("read", nbytes, stream))
+            ctypes.c_uint32.from_address(to).value = words.pop(0)
+            return 0
+
+        def emmy_rt_memset(self, at, value, nbytes, stream):
+            order.append(("clear", value, nbytes, stream))
+            return 0
+
+    op = emmyrt.blockfp8.BlockFp8Linear(A(4, "e4m3", 300, 208), A(5, "f32", 3, 2), 8)
+    monkeypatch.setattr(emmyrt.blockfp8, "lib", Lib())
+    monkeypatch.setattr(emmyrt.blockfp8, "current_device", lambda: current, raising=False)
+    there, back = ([], []) if current == 0 else ([("device", 0)], [("device", 1)])
+    words += [0, 5, 0, 6]
+    assert op.status() == 0 and order == there + ["all", ("read", 4, 0), ("wait", 0)] + back
+    order.clear()
+    assert op.status() == 5 and order == there + ["all", ("read", 4, 0), ("wait", 0), ("clear", 0, 4, 0), ("wait", 0)] + back
+    order.clear()
+    assert op.status(stream=77) == 0 and order == there + [("read", 4, 77), ("wait", 77)] + back
+    order.clear()
+    assert op.status(stream=77) == 6 and order == there + [("read", 4, 77), ("wait", 77), ("clear", 0, 4, 77), ("wait", 77)] + back
