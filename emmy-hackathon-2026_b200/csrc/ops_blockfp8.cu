@@ -939,10 +939,11 @@ template <typename T> int product(const emmy_ops_blockfp8_args *a, int device, u
                     "joining the FP8 product's parts");
 }
 
-int check_matrix(const char *name, uint64_t at, int64_t rows, int64_t cols, int64_t stride, int size, int multiple) {
+/* shared: all rows may be one (stride 0) */
+int check_matrix(const char *name, uint64_t at, int64_t rows, int64_t cols, int64_t stride, int size, int multiple, bool shared = false) {
     if (rows < 0 || cols < 1 || rows > 0x7fffff00LL || cols > 0x7fffff00LL)
         return ops_fail(EMMY_RT_EINVAL, "%s of %lld x %lld", name, (long long)rows, (long long)cols);
-    if (rows > 1 && stride < cols) return ops_fail(EMMY_RT_EINVAL, "%s: rows overlap: stride %lld", name, (long long)stride);
+    if (rows > 1 && stride < cols && !(shared && stride == 0)) return ops_fail(EMMY_RT_EINVAL, "%s: rows overlap: stride %lld", name, (long long)stride);
     if (!at || !aligned(at, size * multiple)) return ops_fail(EMMY_RT_EINVAL, "%s is needed, on %d bytes", name, size * multiple);
     if (stride % multiple) return ops_fail(EMMY_RT_EINVAL, "%s: rows are not a multiple of %d elements apart", name, multiple);
     return 0;
@@ -982,7 +983,7 @@ EMMY_EXPORT int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args
     if (!known_dtype(a->dtype)) return ops_fail(EMMY_RT_EINVAL, "element type %d", a->dtype);
     const int es = elem_size(a->dtype);
     const int64_t row_blocks = a->square ? (a->rows + BLOCK - 1) / BLOCK : a->rows, col_blocks = (a->cols + BLOCK - 1) / BLOCK;
-    if (int e = check_matrix("x", a->rows ? a->x : 16, a->rows, a->cols, a->x_stride, es, 1)) return e;
+    if (int e = check_matrix("x", a->rows ? a->x : 16, a->rows, a->cols, a->x_stride, es, 1, true)) return e;
     /* a single row that is not in padded rows: no column past its last one is written */
     const int64_t padded = (a->cols + 15) / 16 * 16;
     const bool bare = a->rows == 1 && a->q_stride < padded;
@@ -1055,7 +1056,7 @@ EMMY_EXPORT int emmy_ops_blockfp8_linear(const emmy_ops_blockfp8_linear_args *a,
         return emmy_ops_blockfp8_product(&q, device, stream);
     }
     const int es = elem_size(a->x_dtype);
-    if (int e = check_matrix("x", q.m ? a->x : 16, q.m, q.k, a->x_stride, es, 1)) return e;
+    if (int e = check_matrix("x", q.m ? a->x : 16, q.m, q.k, a->x_stride, es, 1, true)) return e;
     if (q.m == 0) return 0;
     DeviceScope scope(device);
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");

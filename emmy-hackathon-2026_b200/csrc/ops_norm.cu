@@ -256,8 +256,9 @@ EMMY_EXPORT int emmy_ops_residual_norm(const emmy_ops_norm_args *a, int device, 
     if (!a->x || !a->block || !a->y) return ops_fail(EMMY_RT_EINVAL, "x, block and y are needed");
     if (a->gate && a->rows_per_gate < 1) return ops_fail(EMMY_RT_EINVAL, "rows_per_gate %lld", (long long)a->rows_per_gate);
     const int64_t strides[] = {a->x_stride, a->block_stride, a->y_stride, a->h ? a->h_stride : a->dim};
-    for (int64_t s : strides)
-        if (s < a->dim && a->rows > 1) return ops_fail(EMMY_RT_EINVAL, "rows overlap: stride %lld", (long long)s);
+    for (int i = 0; i < 4; ++i)         /* x and block may be one row for all */
+        if (strides[i] < a->dim && a->rows > 1 && !(i < 2 && strides[i] == 0))
+            return ops_fail(EMMY_RT_EINVAL, "rows overlap: stride %lld", (long long)strides[i]);
     const uint64_t rows_at[] = {a->x, a->block, a->y, a->h};
     const int es = elem_size(a->dtype);
     int bytes = 16;

@@ -10,6 +10,7 @@
  * Conventions (those of emmyrt.h)
  *   - every entry point returns 0, a cudaError_t value (> 0) of the failing call, or a
  *     negative EMMY_RT_E* code; emmy_ops_last_error() then has the text (per thread);
+ *   - rows of an operand do not overlap, but those of an input may all be one (a stride of 0);
  *   - arguments are checked before anything is enqueued, as far as the host can see them;
  *     device pointers are 64-bit handles, strides are in elements, element types are
  *     EMMY_OPS_* codes;

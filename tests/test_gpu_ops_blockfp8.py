@@ -260,3 +260,24 @@ def test_status_of_calls_on_other_streams(runtime):
             op(x, y, stream=side.cuda_stream)
         runtime.check(runtime.lib.emmy_rt_memcpy_dtod(op._status, word.data_ptr(), 4, side.cuda_stream), "copy")
         assert op.status(stream=named) == 8 and op.status(stream=named) == 0
+
+
+@pytest.mark.parametrize("m", [2, 5, 40, 150])
+def test_one_row_for_all(runtime, m):
+    """x broadcast over its rows (stride 0): quantised and multiplied like the rows written out."""
+    from emmyrt.blockfp8 import BlockFp8Linear, BlockFp8Quantizer
+    wq, ws = weights(200, 330)
+    x = torch.randn(1, 330, generator=gen(m), device="cuda").half().expand(m, 330)
+    y, z = (torch.empty(m, 200, device="cuda") for _ in range(2))
+    op = BlockFp8Linear(wq, ws, max_rows=m)
+    op(x, y, stream=stream())
+    op(x.contiguous(), z, stream=stream())
+    assert torch.equal(y, z)
+    for square in (False, True):
+        got = []
+        for v in (x, x.contiguous()):
+            q = torch.zeros(m, 336, dtype=torch.uint8, device="cuda")
+            s = torch.empty((-(-m // 128), 3) if square else (3, m), device="cuda")
+            BlockFp8Quantizer(square)(v, q[:, :330], s, stream=stream())
+            got.append((q, s))
+        assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])

@@ -175,3 +175,18 @@ def test_graph_and_stream(runtime):
         close(y, ry, ty, torch.bfloat16)
         rh, th, _, _ = reference({**new, "x": y, "pre_weight": None}, "rms", 1e-6, 0.5, True, 37)
         close(h, rh, th, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dim", [64, 65, 1032])
+def test_one_row_for_all(runtime, dim):
+    """x or block broadcast over the rows (stride 0)."""
+    from emmyrt.norms import ResidualNorm
+    t = operands(9, dim, "bf16", "rms", True, 0)
+    for name in ("x", "block"):
+        s = {**t, name: t[name][:1].expand(9, dim)}
+        y, h = (torch.empty(9, dim, dtype=torch.bfloat16, device="cuda") for _ in range(2))
+        ResidualNorm(dim, eps=1e-5, scale=0.7)(s["x"], s["block"], y, h, post_weight=s["post_weight"], pre_weight=s["pre_weight"],
+                                               stream=torch.cuda.current_stream().cuda_stream)
+        ry, ty, rh, th = reference(s, "rms", 1e-5, 0.7, True, 9)
+        close(y, ry, ty, torch.bfloat16)
+        close(h, rh, th, torch.bfloat16)
