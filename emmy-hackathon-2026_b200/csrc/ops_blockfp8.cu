@@ -10,6 +10,7 @@
  * tensor cores and the scaled sums beside them; join_parts adds up products that many_rows cut along k.
  */
 #include "ops_common.cuh"
+#include "ops_wait.cuh"
 
 namespace {
 
@@ -406,8 +407,6 @@ template <typename T, int NT, typename X = Quantised> cudaError_t go_few(const F
  * arrive by TMA in 128-byte rows with the 128-byte swizzle; every wait gives up after 2 s.
  * 8192 x 8192 x 8192 takes 483 us (2.28 PFLOP/s), and 418 us without the scaled sums: what is left of the distance to
  * the e4m3 rate is the sums' issue slots and the power limit. */
-constexpr uint64_t TIMEOUT_NS = 2000000000ull;
-
 struct ManyParams {
     const float *sw;
     char *y;
@@ -415,49 +414,6 @@ struct ManyParams {
     int64_t sw_stride, y_stride, split_stride;
     int m, n, k_blocks, m_tiles, n_tiles, wide, even, splits, per_split;
 };
-
-__device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ bool try_wait(uint32_t barrier, uint32_t parity) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred q;\nmbarrier.try_wait.parity.shared::cta.b64 q, [%1], %2;\nselp.u32 %0, 1, 0, q;\n}"
-                 : "=r"(ok) : "r"(barrier), "r"(parity) : "memory");
-    return ok;
-}
-__device__ __forceinline__ uint64_t now_ns() {
-    uint64_t t;
-    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
-    return t;
-}
-/* False when the wait gave up, here or in another role.  The timer is looked at in every 64th try only: most waits here
- * are for one block's product, and reading it is slow. */
-__device__ __forceinline__ bool wait_for(uint32_t barrier, uint32_t parity, volatile unsigned *abort, unsigned *status, unsigned role) {
-    uint64_t start = 0;
-    for (unsigned tries = 0; !try_wait(barrier, parity); ++tries) {
-        if ((tries & 63) != 63) continue;
-        if (*abort) return false;
-        const uint64_t now = now_ns();
-        if (!start) start = now;
-        if (now - start > TIMEOUT_NS) {
-            *abort = 1;
-            atomicOr(status, role);
-            return false;
-        }
-    }
-    return true;
-}
-
-/* both barriers, tried together first: a try takes tens of cycles, and one thread issues all products */
-__device__ __forceinline__ bool wait_for_both(uint32_t a, uint32_t a_parity, uint32_t b, uint32_t b_parity, volatile unsigned *abort,
-                                              unsigned *status, unsigned role) {
-    uint32_t ok;
-    asm volatile("{\n.reg .pred p, q;\n"
-                 "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n"
-                 "mbarrier.try_wait.parity.shared::cta.b64 q, [%3], %4;\n"
-                 "and.pred p, p, q;\nselp.u32 %0, 1, 0, p;\n}"
-                 : "=r"(ok) : "r"(a), "r"(a_parity), "r"(b), "r"(b_parity) : "memory");
-    return ok || (wait_for(a, a_parity, abort, status, role) && wait_for(b, b_parity, abort, status, role));
-}
 
 struct TensorMap {
     alignas(64) unsigned char bytes[128];
