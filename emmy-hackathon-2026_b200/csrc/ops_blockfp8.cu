@@ -458,6 +458,13 @@ template <bool PAIR> __device__ __forceinline__ void commit(uint32_t barrier) {
     else
         asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
 }
+/* to this block's barrier alone */
+template <bool PAIR> __device__ __forceinline__ void commit_here(uint32_t barrier) {
+    if (PAIR)
+        asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(barrier) : "memory");
+    else
+        commit<false>(barrier);
+}
 __device__ __forceinline__ void tensor_load(uint32_t address, uint32_t (&u)[32]) {
     asm volatile("tcgen05.ld.sync.aligned.32x32b.x32.b32 "
                  "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
@@ -528,10 +535,11 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
               const __grid_constant__ TensorMap s_map, ManyParams p) {
     using S = ManyShape<BN, PAIR>;
     extern __shared__ unsigned char raw[];
-    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS], scaled[S::SCALES / S::SCALE_RUN];
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES], summed[S::BUFFERS], read[S::BUFFERS], scaled[S::SCALES / S::SCALE_RUN], ended[2];
     __shared__ alignas(128) float scales[S::SCALES][128];      /* of x: a block's 128 rows, copied with its operands */
     __shared__ uint32_t tensor_base;
     __shared__ volatile unsigned abort;
+    __shared__ uint32_t next_stage, next_phase;         /* of the copies, when they ended */
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const uint32_t ring = (shared_address(raw) + 1023) & ~1023u;
     uint32_t rank = 0;
@@ -547,6 +555,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
         }
         for (int i = 0; i < S::SCALES / S::SCALE_RUN; ++i)
             asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(shared_address(&scaled[i])), "r"(S::SCALE_WARPS));
+        for (int i = 0; i < 2; ++i) asm volatile("mbarrier.init.shared::cta.b64 [%0], 1;" ::"r"(shared_address(&ended[i])));
         abort = 0;
         asm volatile("fence.mbarrier_init.release.cluster;\nfence.proxy.async.shared::cta;" ::: "memory");
     }
@@ -607,15 +616,7 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
                     if (++stage == S::STAGES) stage = 0, phase ^= 1;
                 }
             }
-            /* Where a wait gave up: nothing may arrive in shared memory that is no longer this block's, so the copies under way
-             * are waited for (a pair's all complete on the leader's barriers; what was never copied ends by its limit). */
-            if (!ok && rank == 0) {
-                const uint64_t start = now_ns();
-                for (int i = 0; i < S::STAGES; ++i) {
-                    while (!try_wait(shared_address(&full[stage]), phase ^ 1) && now_ns() - start < TIMEOUT_NS) {}
-                    if (++stage == S::STAGES) stage = 0, phase ^= 1;
-                }
-            }
+            next_stage = stage, next_phase = phase;
         }
     } else if (warp == 1 || warp == 3) {
         /* Two threads issue the products, every other block each: issuing one takes a thread longer than the tensor core
@@ -762,6 +763,25 @@ __global__ void __launch_bounds__(ManyShape<BN, PAIR>::THREADS, 1)
     __syncwarp();
     asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory");
     __syncthreads();
+    /* Where a wait gave up, whoever's: copies under way must not arrive in shared memory that is no longer this block's, nor products
+     * in tensor memory that has been freed, so both are waited for.  A pair's copies all complete on the leader's barriers, and
+     * its products are the leader's; it gives up where the other block does, as each waits for the other.  What was never
+     * copied ends by the limit, which is one for all stages. */
+    if (abort) {
+        if (rank == 0 && lane == 0 && warp == 0) {
+            uint32_t stage = next_stage, phase = next_phase;
+            const uint64_t start = now_ns();
+            for (int i = 0; i < S::STAGES; ++i) {
+                wait_for_end(shared_address(&full[stage]), phase ^ 1, start);
+                if (++stage == S::STAGES) stage = 0, phase ^= 1;
+            }
+        } else if (rank == 0 && lane == 0 && (warp == 1 || warp == 3)) {
+            const uint32_t end = shared_address(&ended[warp >> 1]);
+            commit_here<PAIR>(end);
+            wait_for_end(end, 0, now_ns());
+        }
+        __syncthreads();
+    }
     if (PAIR) asm volatile("barrier.cluster.arrive.release;\nbarrier.cluster.wait.acquire;" ::: "memory");
     asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory");
     if (warp == 1) {

@@ -49,3 +49,8 @@ static __device__ __forceinline__ bool wait_for_both(uint32_t a, uint32_t a_pari
                  : "=r"(ok) : "r"(a), "r"(a_parity), "r"(b), "r"(b_parity) : "memory");
     return ok || (wait_for(a, a_parity, abort, status, role, limit) && wait_for(b, b_parity, abort, status, role, limit));
 }
+
+/* Of one's own work under way, after a wait gave up: until it is done or the limit has passed since `start`. */
+static __device__ __forceinline__ void wait_for_end(uint32_t barrier, uint32_t parity, uint64_t start, uint64_t limit = TIMEOUT_NS) {
+    while (!try_wait(barrier, parity) && now_ns() - start < limit) {}
+}

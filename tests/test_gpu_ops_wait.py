@@ -28,6 +28,8 @@ __global__ void waits(unsigned *status, unsigned *passed, uint64_t limit, int ar
     __syncthreads();
     if (threadIdx.x & 31) return;
     if (warp == 3) {
+        const uint64_t start = now_ns();
+        if (!arrive) wait_for_end(a, 0, start, limit);
         if (arrive) {
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(a) : "memory");
             asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(b) : "memory");

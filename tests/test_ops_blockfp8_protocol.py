@@ -52,8 +52,15 @@ class Race(Exception):
     pass
 
 
-def run(tiles, bn, pair, seed, hand_back=True):
-    """``tiles``: the blocks of each tile that this block of threads takes.  Ends, or raises Race or a deadlock's AssertionError."""
+class UnderWay(Exception):
+    pass
+
+
+def run(tiles, bn, pair, seed, hand_back=True, late=None, drain="whenever a wait gave up"):
+    """``tiles``: the blocks of each tile that this block of threads takes.  Ends, or raises Race or a deadlock's AssertionError.
+
+    ``late``: the block whose copies arrive after the limit of the waits only.  Then some wait gives up, all others learn of it, and
+    what is under way is waited for (``drain``) before the block of threads ends: else UnderWay."""
     stages, buffers, warps = shape(bn, pair)
     full, empty = [Barrier(1) for _ in range(stages)], [Barrier(1) for _ in range(stages)]
     summed, read = [Barrier(1) for _ in range(buffers)], [Barrier(warps) for _ in range(buffers)]
@@ -62,6 +69,8 @@ def run(tiles, bn, pair, seed, hand_back=True):
     holds = [None] * SCALES
     blocks = sum(tiles)
     queue = []                                          # products and arrivals of the tensor core, in order
+    flight = []                                         # copies under way
+    gave_up = []
 
     def copies(me):
         stage = slot = 0
@@ -74,7 +83,7 @@ def run(tiles, bn, pair, seed, hand_back=True):
                 if me["clock"].get(warp, 0) < when:
                     raise Race(f"block {i} overwrites scales that {warp} may still read")
             reads[slot], holds[slot] = {}, i
-            full[stage].arrive({})
+            flight.append((i, stage))
             slot += 1
             if slot == SCALES:
                 slot, slot_phase = 0, slot_phase ^ 1
@@ -122,9 +131,19 @@ def run(tiles, bn, pair, seed, hand_back=True):
         threads.append([me, body(me), None])
     slow = rng.choice([t[0]["name"] for t in threads] + [None])         # one thread that lags behind
     while threads or queue:
+        landing = [f for f in flight if f[0] != late]
         moves = [t for t in threads if t[2] is None or t[2][0].passed(t[2][1])]
         if queue:
             moves.append(None)
+        if landing and (not moves or rng.random() < 0.5):
+            f = rng.choice(landing)
+            flight.remove(f)
+            full[f[1]].arrive({})
+            continue
+        if not moves and late is not None:              # the limit passes: one thread gives up, the others that wait learn of it
+            gave_up.extend(rng.sample([t[0]["name"] for t in threads], len(threads)))
+            threads.clear()
+            break
         assert moves, "deadlock"
         ready = [t for t in moves if t is None or t[0]["name"] != slow] or moves
         t = rng.choice(ready if rng.random() < 0.9 else moves)
@@ -138,6 +157,17 @@ def run(tiles, bn, pair, seed, hand_back=True):
             t[2] = next(t[1])
         except StopIteration:
             threads.remove(t)
+    # every thread is at the block's last barrier: products under way are waited for by those who issued them
+    while queue:
+        barrier, clock = queue.pop(0)
+        barrier.arrive(clock)
+    if drain == "whenever a wait gave up" and gave_up or drain == "where the copies gave up" and "copies" in gave_up:
+        for f in flight:
+            full[f[1]].arrive({})
+        flight.clear()
+    if flight:
+        raise UnderWay(f"copies of blocks {sorted(b for b, _ in flight)} arrive in memory that is no longer the block's")
+    return gave_up
 
 
 SHAPES = [(32, False), (64, False), (128, False), (256, True)]
@@ -161,3 +191,17 @@ def test_copies_never_wait_for_a_run(bn, pair):
     """The ring is long enough that its own barriers hold no copy up: what the other barriers allow lies in earlier runs."""
     stages, buffers, _ = shape(bn, pair)
     assert stages + buffers <= SCALES - RUN and SCALES % RUN == 0
+
+
+@pytest.mark.parametrize("bn,pair", SHAPES)
+@pytest.mark.parametrize("blocks,late", [(1, 0), (3, 2), (16, 0), (64, 40), (64, 63), (64, 60)])
+def test_a_late_copy_ends_the_block_with_nothing_under_way(bn, pair, blocks, late):
+    for seed in range(20):
+        assert run([blocks], bn, pair, seed, late=late)
+
+
+@pytest.mark.parametrize("bn,pair", SHAPES)
+def test_the_model_sees_a_copy_that_nobody_waits_for(bn, pair):
+    """The last copies: the thread that issued them is done and did not give up itself."""
+    with pytest.raises(UnderWay):
+        run([64], bn, pair, 0, late=63, drain="where the copies gave up")
