@@ -158,8 +158,7 @@ class BlockFp8Linear(Operator):
         a non-zero word is cleared, so no call may be on its way meanwhile."""
         out = np.zeros(1, np.uint32)
         before = current_device()
-        if before != self.device:
-            check(lib.emmy_rt_set_device(self.device), "set device")
+        check(lib.emmy_rt_set_device(self.device), "set device")        # a thread may have none yet
         try:
             if stream is None:
                 check(lib.emmy_rt_synchronize(), "synchronize")

@@ -281,3 +281,19 @@ def test_one_row_for_all(runtime, m):
             BlockFp8Quantizer(square)(v, q[:, :330], s, stream=stream())
             got.append((q, s))
         assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1])
+
+
+def test_call_and_status_from_a_new_thread(runtime):
+    """A thread that has used no device yet may call an operator and ask for its status."""
+    import threading
+    op, x, y = check(9, 300, 400)
+    again = torch.empty_like(y)
+    torch.cuda.synchronize()
+    got = []
+    on = stream()
+    threads = [threading.Thread(target=lambda: got.append(op.status())),
+               threading.Thread(target=lambda: (op(x, again, stream=on), got.append(op.status())))]
+    for t in threads:
+        t.start()
+        t.join()
+    assert got == [0, 0] and torch.equal(y, again)

@@ -378,7 +378,7 @@ def test_status_waits_for_the_calls(calls, monkeypatch, current):
     op = emmyrt.blockfp8.BlockFp8Linear(A(4, "e4m3", 300, 208), A(5, "f32", 3, 2), 8)
     monkeypatch.setattr(emmyrt.blockfp8, "lib", Lib())
     monkeypatch.setattr(emmyrt.blockfp8, "current_device", lambda: current, raising=False)
-    there, back = ([], []) if current == 0 else ([("device", 0)], [("device", 1)])
+    there, back = [("device", 0)], [("device", 1)] if current else []
     words += [0, 5, 0, 6]
     assert op.status() == 0 and order == there + ["all", ("read", 4, 0), ("wait", 0)] + back
     order.clear()
