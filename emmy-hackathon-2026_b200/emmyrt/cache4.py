@@ -10,7 +10,7 @@ import ctypes
 import math
 
 from . import Cache4AppendArgs, Cache4AttendArgs, DeviceBuffer, EmmyRTError, check, lib, ops_lib
-from .operands import CODE, FLOATS, INDICES, Array, Operator, apart, contiguous, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, INDICES, Array, Operator, apart, contiguous, f32, operand, overlaps, shaped, written
 
 DIMS = (64, 128)
 
@@ -118,7 +118,7 @@ class Cache4Attention(Operator):
     def _plan(self, operands, scale) -> tuple:
         q, out, table, lengths = operands
         c, d = self.cache, self.device
-        if not math.isfinite(scale):
+        if not f32(scale / math.log(2.0)):          # the kernel's logits are to base 2
             raise ValueError(f"scale {scale}")
         q = operand(q, "q", ("f16", "bf16"), 4, d)
         batch, tokens = q.shape[:2]

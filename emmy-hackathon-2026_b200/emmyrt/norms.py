@@ -7,10 +7,8 @@ residual stream and the block's output once and writes the new stream and the ne
 
 from __future__ import annotations
 
-import math
-
 from . import NormArgs
-from .operands import CODE, FLOATS, Operator, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, Operator, f32, operand, overlaps, shaped, written
 
 KINDS = {"rms": 0, "layer": 1}
 MAX_DIM = 16384
@@ -29,8 +27,10 @@ class ResidualNorm(Operator):
             raise ValueError(f"kind {kind!r} is not one of {', '.join(KINDS)}")
         if not 1 <= dim <= MAX_DIM:
             raise ValueError(f"dim {dim} is not in 1 .. {MAX_DIM}")
-        if not (eps >= 0 and math.isfinite(eps)):
+        if not (eps >= 0 and f32(eps)):
             raise ValueError(f"eps {eps}")
+        if not f32(scale):
+            raise ValueError(f"scale {scale}")
         self.dim, self.kind, self.eps, self.scale, self.post_norm = int(dim), kind, float(eps), float(scale), bool(post_norm)
         super().__init__()
 

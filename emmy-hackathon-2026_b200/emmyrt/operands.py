@@ -9,6 +9,7 @@ enqueued; a call that the library refuses raises :class:`emmyrt.EmmyRTError`.
 from __future__ import annotations
 
 import ctypes
+import math
 
 from . import EmmyRTError, _calls, current_device, ops_lib
 
@@ -20,6 +21,11 @@ INDICES = ("i32", "i64")
 _NAMES = {"torch.float32": "f32", "torch.float16": "f16", "torch.bfloat16": "bf16", "torch.float8_e4m3fn": "e4m3",
           "torch.uint8": "u8", "torch.int32": "i32", "torch.int64": "i64"}
 _seen: dict = {}            # dtype object -> name, as str(dtype) costs more than the rest of a check
+
+
+def f32(value: float) -> bool:
+    """Whether f32 holds a number of this size."""
+    return math.isfinite(ctypes.c_float(value).value)
 
 
 class Array:

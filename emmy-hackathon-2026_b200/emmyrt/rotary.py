@@ -12,7 +12,7 @@ import math
 import numpy as np
 
 from . import DeviceBuffer, RotaryArgs
-from .operands import CODE, FLOATS, INDICES, Operator, operand, overlaps, shaped, written
+from .operands import CODE, FLOATS, INDICES, Operator, f32, operand, overlaps, shaped, written
 
 LAYOUTS = {"half": 0, "interleaved": 1}
 SCALINGS = ("none", "linear", "base", "parts")
@@ -70,7 +70,7 @@ class Rotary(Operator):
         f = frequencies(rotary_dim, base, scaling, factor, original_length, slow, fast)
         if magnitude is None:
             magnitude = 0.1 * math.log(factor) + 1.0 if scaling == "parts" else 1.0
-        if not math.isfinite(magnitude):
+        if not f32(magnitude):
             raise ValueError(f"magnitude {magnitude}")
         self.dim, self.rotary_dim, self.layout, self.magnitude = int(dim), int(rotary_dim), layout, float(magnitude)
         super().__init__()

@@ -387,3 +387,21 @@ def test_status_waits_for_the_calls(calls, monkeypatch, current):
     assert op.status(stream=77) == 0 and order == there + [("read", 4, 77), ("wait", 77)] + back
     order.clear()
     assert op.status(stream=77) == 6 and order == there + [("read", 4, 77), ("wait", 77), ("clear", 0, 4, 77), ("wait", 77)] + back
+
+
+def test_numbers_that_f32_does_not_hold(calls):
+    """Scales travel in f32: one that would become infinite there is refused, not rounded to infinity."""
+    from emmyrt.cache4 import Cache4, Cache4Attention
+    from emmyrt.norms import ResidualNorm
+    from emmyrt.rotary import Rotary
+    op = Cache4Attention(Cache4(*cache_parts()), 8)
+    q, out, table, lengths = A(9, "f16", 4, 1, 8, 64), A(10, "f16", 4, 1, 8, 64), A(11, "i32", 4, 3), A(12, "i32", 4)
+    for scale in (1e39, -1e300, float("inf"), 3e38):        # 3e38 is none in powers of two
+        refuses(lambda: op(q, out, table, lengths, scale=scale), "scale")
+    op(q, out, table, lengths, scale=2e38)
+    for bad in (1e39, float("inf"), float("nan")):
+        refuses(lambda: ResidualNorm(64, scale=bad), "scale")
+        refuses(lambda: ResidualNorm(64, eps=bad), "eps")
+        refuses(lambda: Rotary(64, magnitude=bad), "magnitude")
+    ResidualNorm(64, scale=-3e38, eps=0.0)
+    assert len(calls) == 1
