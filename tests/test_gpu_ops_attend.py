@@ -298,3 +298,11 @@ def test_long_sums_are_not_biased(runtime, dtype):
     count = batch * heads * dim
     error, first, second = error / count, first / count, second / count
     assert abs(error) <= 4 * 2.0 ** -22 * first + 2.0 ** -22 * second, (error / first, first, second)
+
+
+@pytest.mark.parametrize("dtype,dim,heads,group,tokens,page,lengths", [
+    ("bf16", 128, 2, 4, 33, 64, [33, 500, 20]), ("f16", 64, 1, 5, 128, 48, [700, 128, 129]), ("bf16", 64, 1, 1, 130, 16, [1000, 131]),
+    ("f16", 128, 1, 3, 500, 64, [500, 777]), ("bf16", 128, 1, 2, 500, 24, [2100, 400])])
+def test_prompts(runtime, dtype, dim, heads, group, tokens, page, lengths):
+    """Many queries a sequence, over what the cache holds before them and over each other."""
+    check(dtype, dim, heads, group, tokens, page, lengths)
