@@ -233,8 +233,8 @@ template <typename T, int V, int N> cudaError_t go(NormParams &p, uint64_t strea
  * row, of which 32 each would leave half of the 8 lanes idle (200000 rows of 64 in bf16: 44 us, 20 with 8 each); else
  * 32, over which a row's sums and addresses cost little (100000 rows of 200: 44 us, 56 with 8 each); 16 in narrow accesses
  * for rows that 1024 threads of 8 would not hold. */
-template <typename T> cudaError_t dispatch(NormParams &p, int bytes, uint64_t stream) {
-    const bool many = p.dim > 8192 || (p.dim > 128 && p.rows * p.dim > 148 * 4096 * 2);
+template <typename T> cudaError_t dispatch(NormParams &p, int bytes, int sms, uint64_t stream) {
+    const bool many = p.dim > 8192 || (p.dim > 128 && p.rows * p.dim > (int64_t)sms * 4096 * 2);
     constexpr int W = 16 / sizeof(T);
     const bool large = p.dim > 8192;
     if (bytes == 16) return many ? go<T, W, 32 / W>(p, stream) : go<T, W, 8 / W>(p, stream);
@@ -295,10 +295,12 @@ EMMY_EXPORT int emmy_ops_residual_norm(const emmy_ops_norm_args *a, int device, 
     p.gate_stride = a->gate_stride, p.rows = a->rows;
     p.rows_per_gate = (int)(a->rows_per_gate < a->rows ? a->rows_per_gate : a->rows);
     p.dim = (int)a->dim, p.layer = a->kind, p.post_norm = a->post_norm != 0, p.eps = a->eps, p.scale = a->scale;
+    int sms;
+    if (int e = ops_sm_count(device, &sms)) return e;
     DeviceScope scope(device);
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
-    cudaError_t e = a->dtype == EMMY_OPS_F32    ? dispatch<float>(p, bytes, stream)
-                    : a->dtype == EMMY_OPS_F16 ? dispatch<__half>(p, bytes, stream)
-                                               : dispatch<__nv_bfloat16>(p, bytes, stream);
+    cudaError_t e = a->dtype == EMMY_OPS_F32    ? dispatch<float>(p, bytes, sms, stream)
+                    : a->dtype == EMMY_OPS_F16 ? dispatch<__half>(p, bytes, sms, stream)
+                                               : dispatch<__nv_bfloat16>(p, bytes, sms, stream);
     return ops_cuda(e, "residual norm");
 }

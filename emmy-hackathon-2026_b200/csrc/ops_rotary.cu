@@ -118,7 +118,7 @@ __global__ void __launch_bounds__(256) rotary(RotaryParams p) {
     }
 }
 
-template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, bool copies, uint64_t stream) {
+template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, bool copies, int sms, uint64_t stream) {
     /* tokens a block: about two (token, head) pairs for each of its 256 threads where there are many tokens, one token
      * where there are few, as long as the table fits 32 KB.  More would fill the threads better and wait longer for angles: 16384
      * tokens of 40 heads take 69 us with one token a block and 77 with two. */
@@ -127,7 +127,7 @@ template <typename T, int V> cudaError_t go(RotaryParams &p, int layout, bool co
     p.side = per_head < 256 ? 256 / per_head : 1;
     const int64_t per_token = (int64_t)(p.heads[0] + p.heads[1]) * per_head;
     int64_t per = (512 + per_token / 2) / per_token;
-    const int64_t spread = p.tokens / (148 * 4), most = 32768 / ((int64_t)pairs * 8);
+    const int64_t spread = p.tokens / (sms * 4), most = 32768 / ((int64_t)pairs * 8);
     if (per > spread) per = spread;
     if (per > most) per = most;
     p.per_block = per < 1 ? 1 : (int)per;
@@ -182,18 +182,20 @@ EMMY_EXPORT int emmy_ops_rotary(const emmy_ops_rotary_args *a, int device, uint6
     p.turns = (const uint64_t *)(uintptr_t)a->turns;
     p.tokens = a->tokens, p.positions_64 = a->positions_64 != 0, p.transpose = a->transpose != 0;
     p.magnitude = a->magnitude;
+    int sms;
+    if (int e = ops_sm_count(device, &sms)) return e;
     DeviceScope scope(device);
     if (scope.status != cudaSuccess) return ops_cuda(scope.status, "device");
     cudaError_t e;
     if (a->dtype == EMMY_OPS_F32)
-        e = bytes == 16 ? go<float, 4>(p, a->layout, copies, stream) : go<float, 1>(p, a->layout, copies, stream);
+        e = bytes == 16 ? go<float, 4>(p, a->layout, copies, sms, stream) : go<float, 1>(p, a->layout, copies, sms, stream);
     else if (a->dtype == EMMY_OPS_F16)
-        e = bytes == 16  ? go<__half, 8>(p, a->layout, copies, stream)
-            : bytes == 4 ? go<__half, 2>(p, a->layout, copies, stream)
-                         : go<__half, 1>(p, a->layout, copies, stream);
+        e = bytes == 16  ? go<__half, 8>(p, a->layout, copies, sms, stream)
+            : bytes == 4 ? go<__half, 2>(p, a->layout, copies, sms, stream)
+                         : go<__half, 1>(p, a->layout, copies, sms, stream);
     else
-        e = bytes == 16  ? go<__nv_bfloat16, 8>(p, a->layout, copies, stream)
-            : bytes == 4 ? go<__nv_bfloat16, 2>(p, a->layout, copies, stream)
-                         : go<__nv_bfloat16, 1>(p, a->layout, copies, stream);
+        e = bytes == 16  ? go<__nv_bfloat16, 8>(p, a->layout, copies, sms, stream)
+            : bytes == 4 ? go<__nv_bfloat16, 2>(p, a->layout, copies, sms, stream)
+                         : go<__nv_bfloat16, 1>(p, a->layout, copies, sms, stream);
     return ops_cuda(e, "rotary");
 }
