@@ -238,7 +238,8 @@ template <typename T> cudaError_t dispatch(NormParams &p, int bytes, int sms, ui
     constexpr int W = 16 / sizeof(T);
     const bool large = p.dim > 8192;
     if (bytes == 16) return many ? go<T, W, 32 / W>(p, stream) : go<T, W, 8 / W>(p, stream);
-    if (bytes == 4 && sizeof(T) == 2) return large ? go<T, 2, 8>(p, stream) : go<T, 2, 4>(p, stream);
+    if constexpr (sizeof(T) == 2)
+        if (bytes == 4) return large ? go<T, 2, 8>(p, stream) : go<T, 2, 4>(p, stream);
     return large ? go<T, 1, 16>(p, stream) : go<T, 1, 8>(p, stream);
 }
 
