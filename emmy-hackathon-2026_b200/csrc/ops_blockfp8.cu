@@ -514,10 +514,10 @@ template <int BN, bool PAIR> struct ManyShape {
     static constexpr int A_BYTES = 128 * BLOCK, B_BYTES = B_ROWS * BLOCK, STAGE = A_BYTES + B_BYTES;
     static constexpr int STAGES = STAGE > 40960 ? 4 : STAGE >= 32768 ? 6 : 8;
     static constexpr int BUFFERS = 512 / BN > 4 ? 4 : 512 / BN;
-    /* x's scales have a ring of their own, in runs of SCALE_RUN places that the scaling warps hand back by a barrier each.  The
-     * copies are at most STAGES blocks ahead of the products, and these BUFFERS ahead of the scaling, so they find the next run
-     * free: nothing waits there. */
-    static constexpr int SCALES = 16, SCALE_RUN = 4;
+    /* x's scales have a ring of their own, in runs of SCALE_RUN places that the scaling warps hand back by a barrier each (runs of
+     * 2 take 1 % longer at 8192^3, of 4 0.3 %).  The copies are at most STAGES blocks ahead of the products, and these BUFFERS
+     * ahead of the scaling, so they find the next run free: nothing waits there. */
+    static constexpr int SCALES = 24, SCALE_RUN = 8;
     static_assert(STAGES + BUFFERS <= SCALES - SCALE_RUN, "the scales' ring");
     static constexpr int COLUMNS = BN * BUFFERS < 32 ? 32 : BN * BUFFERS;
     static constexpr int SCALE_WARPS = BN >= 128 ? 8 : 4;
