@@ -6,8 +6,9 @@
  * x is quantised per row and 128 columns, W per 128 x 128 block:
  *     s = amax / 448 (1 where that is 0),  q = e4m3(v / s), nearest even.
  *
- * The two quantisers are bound by their bytes, few_rows (up to 16 rows of x) by the bytes of W, and many_rows by the
- * tensor cores and the scaled sums beside them; join_parts adds up products that many_rows cut along k.
+ * The row quantiser is bound by its issue slots as much as by its bytes (65 % and 52 %), few_rows (up to 16 rows of x) by waits for
+ * W and by the conversions that mma.sync makes of e4m3, at half of what DRAM gives, and many_rows by the tensor cores and the
+ * scaled sums beside them; join_parts adds up products that many_rows cut along k.
  */
 #include "ops_common.cuh"
 #include "ops_wait.cuh"
@@ -217,8 +218,9 @@ __device__ __forceinline__ void mma_e4m3(float (&d)[4], uint32_t a0, uint32_t a1
 /* 16 rows of W a block of threads; its 8 or 16 warps take every 8th or 16th block of 128 columns and join at the end.  W and x come
  * through a ring of asynchronous copies in shared memory, FEW_STAGES blocks of a warp ahead: what is under way decides the rate
  * at so little work a byte, and registers for it would halve what runs at once.  A thread takes 16 consecutive bytes of a row;
- * the order of the columns inside a product is the same for x and W, and free.  W's bytes bound it, and at more than
- * 4 rows the conversions of e4m3 that mma.sync is made of here. */
+ * the order of the columns inside a product is the same for x and W, and free.  1 x 16384 x 8192 reads W at 50 % of what DRAM gives
+ * and issues in 45 % of its slots: a warp waits for its own copies and for its chain of products, whose e4m3 is converted
+ * in the general pipes. */
 template <int NT> struct alignas(16) FewStage {
     unsigned char w[16][BLOCK], x[8 * NT][BLOCK];
     float sx[8 * NT], sw, unused[3];
@@ -405,8 +407,8 @@ template <typename T, int NT, typename X = Quantised> cudaError_t go_few(const F
  * the tensor core sums a block of 128 columns into tensor memory, and the scaling warps add scale times that to the
  * tile's sums in registers while the next block's product runs (tensor memory holds 512 / BN blocks).  Operands
  * arrive by TMA in 128-byte rows with the 128-byte swizzle; every wait gives up after 2 s.
- * 8192 x 8192 x 8192 takes 483 us (2.28 PFLOP/s), and 418 us without the scaled sums: what is left of the distance to
- * the e4m3 rate is the sums' issue slots and the power limit. */
+ * 8192 x 8192 x 8192 takes 483 to 512 us from box to box (2.15 to 2.28 PFLOP/s), and took 418 where it took 483 with the scaled sums
+ * left out: what is left of the distance to the e4m3 rate is the sums' issue slots and the power limit. */
 struct ManyParams {
     const float *sw;
     char *y;

@@ -29,8 +29,10 @@
  * tokens of each tile with their own running maxima and sums and their own ring of
  * asynchronous copies, and join at the end of a sequence; a sequence that runs over several
  * blocks leaves 32-bit partial sums in the workspace, which a second kernel joins in order.
- * 64 sequences of up to 16384 tokens, 8 heads of 128 under 32, take 146 us (4.9 TB/s; the loads alone 128, the
- * arithmetic alone 141); one of 1000 tokens takes 6.7 us, most of it the chain from lengths to pages to tokens, twice.
+ * 64 sequences of up to 16384 tokens (10500 on average), 8 heads of 128 under 32, take 151 us (4.8 TB/s; the loads alone 128); one
+ * of 1000 tokens takes 6.9 us, most of it the chain from lengths to pages to tokens, twice.  All of a tile's tokens are
+ * computed for all rows, and every 8 or 16 rows read the cache again, so a prompt is far from what it could be: 2048 tokens
+ * over 8192 held ones take 1.6 ms, 195 TFLOP/s of what they see.
  */
 #include "ops_common.cuh"
 
@@ -401,7 +403,8 @@ __global__ void __launch_bounds__(WARPS * 32, BLOCKS_PER_SM<NT>) cache4_attend(A
                         }
                     }
         }
-        /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14 */
+        /* p times the value's step goes to f16: a power of two brings the largest step met so far near 2^14, so a product is lost
+         * below 2^-39 of that step */
         float rescale = 1.0f;
         /* A hidden token's probability is 0, and 0 times infinity is no 0: where a value of such a tile is not finite, the
          * products leave it out, and the rows that see it take it by itself. */

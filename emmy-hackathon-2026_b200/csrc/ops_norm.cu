@@ -3,15 +3,15 @@
  *
  *     y = x + scale * gate * N(block),   h = N(y)
  *
- * The bytes bound it: x and block are read once, y and h written once; the row stays in
- * registers between its two norms.  A row belongs to 8, 16 or 32 lanes of a warp, or to a
+ * x and block are read once, y and h written once; the row stays in registers between its two norms.  A row belongs to 8, 16 or 32 lanes of a warp, or to a
  * block of threads of its own; a thread holds 8 elements of it, or 32 where there are rows
  * enough to fill the GPU: fewer warps then have to meet at a row's sums (one barrier each), and
  * more bytes are under way for each of them.  32-bit sums: shuffles inside a warp, shared
  * memory across a row's warps.  The layer norm's variance is taken about the mean of the
  * registers' values, not as a difference of two sums, which would lose it when the mean is large.
- * 8192 x 4096 in bf16, both norms layer norms, takes 73 us (3.7 TB/s): 104 registers leave 16 warps an SM, which wait for
- * four sums in sequence and five vectors through L1; 8 rows take 3.1 us.
+ * Few rows are bound by the launch (8 rows 3.1 us), many by latency and not by their bytes: 8192 x 4096 in bf16, both norms layer
+ * norms, takes 73 us (3.7 TB/s), as 104 registers leave 16 warps an SM, which wait for four sums in sequence and five vectors
+ * through L1.
  */
 #include "ops_common.cuh"
 
@@ -232,7 +232,8 @@ template <typename T, int V, int N> cudaError_t go(NormParams &p, uint64_t strea
  * do not fill the GPU (they are bound by the chain from load to store), where accesses are narrow, and up to 128 elements a
  * row, of which 32 each would leave half of the 8 lanes idle (200000 rows of 64 in bf16: 44 us, 20 with 8 each); else
  * 32, over which a row's sums and addresses cost little (100000 rows of 200: 44 us, 56 with 8 each); 16 in narrow accesses
- * for rows that 1024 threads of 8 would not hold. */
+ * for rows that 1024 threads of 8 would not hold.  Those keep to the 64 registers of 1024 threads by spilling, 16 to 24 bytes in
+ * pairs and about 300 in single elements: 2861 rows of 11727 in bf16 take 243 us, of 11728 in 16-byte accesses 85. */
 template <typename T> cudaError_t dispatch(NormParams &p, int bytes, int sms, uint64_t stream) {
     const bool many = p.dim > 8192 || (p.dim > 128 && p.rows * p.dim > (int64_t)sms * 4096 * 2);
     constexpr int W = 16 / sizeof(T);

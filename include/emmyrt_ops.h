@@ -75,7 +75,8 @@ int emmy_ops_residual_norm(const emmy_ops_norm_args *a, int device, uint64_t str
 
 /* Turns pair i of every head of token t by positions[t] * turns[i] / 2^64 of a full turn and
  * multiplies it by magnitude; elements from `rotary` on are copied.  transpose != 0 turns the
- * other way, which is the gradient's map.  x[1] (tokens, heads[1], dim) is optional (0 heads).
+ * other way, which is the gradient's map.  Cosines and sines are f32 of the turn's upper 24 bits (off by up to
+ * 2^-25 of half a turn, whatever the position).  x[1] (tokens, heads[1], dim) is optional (0 heads).
  * out may be x; other overlaps are the caller's error. */
 typedef struct {
     uint64_t x[2], out[2];
@@ -109,8 +110,8 @@ int emmy_ops_blockfp8_quantize(const emmy_ops_blockfp8_quantize_args *a, int dev
  * with).  *status (a word of
  * device memory, zeroed by the caller once) gets a bit when a wait inside the kernel gave
  * up after 2 s; y is then not valid.  parts (0: none, else on 16 bytes) is memory for the parts of a
- * product that is cut along k where y alone has too few tiles for the GPU: 16 times m rows of n f32
- * serve every cut. */
+ * product that is cut along k where y alone has too few tiles for the GPU: 16 times m rows of f32, n
+ * rounded up to a multiple of 4, serve every cut; a cut that they do not hold is not made. */
 typedef struct {
     uint64_t xq, xs, wq, ws, y, status, parts, parts_bytes;
     int64_t xq_stride, xs_stride, wq_stride, ws_stride, y_stride, m, n, k;
